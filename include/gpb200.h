@@ -428,6 +428,96 @@ int gpb_matvec_layout(gpb_provider* p, int64_t ncols, int32_t* layout);
  * race and must be ordered by the caller. */
 int gpb_forward_matvec_noalloc(gpb_provider* p, float* out_dev, const float* v_dev, int64_t ncols);
 
+/* ------------------------------------------------------- feature map
+ * Operators of a learned feature map, the network that brings wide inputs
+ * (more than GPB_MAX_DIM columns) under a GP, plus the kernel's input gradient
+ * its backward pass starts from. No reference counterpart. They take no
+ * provider (the input gradient aside): each call names its device and CUDA
+ * stream (NULL = the legacy default stream), allocates nothing, never
+ * synchronises, leaves the caller's current device as it was and can be
+ * captured into a CUDA graph. Blocks are row-major with a leading dimension
+ * (>= the column count, in elements) and unit column stride. Types are
+ * GPB_DTYPE_*; statistics and sums are float32. A workspace is scratch of the
+ * size the matching *_workspace call gives for the same sizes (it depends on
+ * nothing else), 16-byte aligned; two calls that may run at the same time
+ * need two. Results repeat bit for bit (no atomics). */
+#define GPB_DTYPE_F32 0
+#define GPB_DTYPE_F16 1
+#define GPB_DTYPE_BF16 2
+
+#define GPB_ACT_SILU 0
+#define GPB_ACT_GELU 1    /* z Phi(z), the exact form */
+#define GPB_ACT_SIGMOID 2
+#define GPB_ACT_TANH 3
+
+/* out = (x - mean) rstd weight + bias over each row of x [rows][cols], with
+ * rstd = 1 / sqrt(mean((x - mean)^2) + eps). weight and bias [cols] may be
+ * NULL (1 and 0) and are param_dtype: float32 or x's type. mean_dev and
+ * rstd_dev [rows] float32 are written where not NULL. out may be x itself
+ * (same pointer and leading dimension). */
+int gpb_layer_norm(int32_t device, void* stream, int32_t dtype, int32_t param_dtype, int64_t rows,
+                   int64_t cols, void* out_dev, int64_t out_ld, const void* x_dev, int64_t x_ld,
+                   const void* weight_dev, const void* bias_dev, float eps, float* mean_dev,
+                   float* rstd_dev);
+/* Bytes gpb_layer_norm_backward needs when it writes dweight or dbias. */
+int gpb_layer_norm_workspace(int64_t rows, int64_t cols, int64_t* bytes_out);
+/* Gradients of gpb_layer_norm from dout [rows][cols], x and the forward pass's
+ * mean and rstd; dx, dweight and dbias (param_dtype) are each optional (NULL).
+ * dx may be dout or x itself. rows = 0 writes zero dweight and dbias. */
+int gpb_layer_norm_backward(int32_t device, void* stream, int32_t dtype, int32_t param_dtype,
+                            int64_t rows, int64_t cols, void* dx_dev, int64_t dx_ld,
+                            const void* dout_dev, int64_t dout_ld, const void* x_dev, int64_t x_ld,
+                            const float* mean_dev, const float* rstd_dev, const void* weight_dev,
+                            void* dweight_dev, void* dbias_dev, void* workspace_dev,
+                            int64_t workspace_bytes);
+
+/* out = act(x w_gate' + b_gate) * (x w_up' + b_up), both projections, the
+ * activation and the product in one kernel: x [rows][inner], w_gate and w_up
+ * [outer][inner] with one leading dimension, biases [outer] or NULL, out
+ * [rows][outer], all of one type; `activation` is GPB_ACT_*. out must not
+ * overlap an input. */
+int gpb_gated_unit_workspace(int32_t dtype, int64_t rows, int64_t inner, int64_t outer,
+                             int32_t backward, int64_t* bytes_out);
+int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activation, int64_t rows,
+                   int64_t inner, int64_t outer, void* out_dev, int64_t out_ld, const void* x_dev,
+                   int64_t x_ld, const void* w_gate_dev, const void* w_up_dev, int64_t w_ld,
+                   const void* b_gate_dev, const void* b_up_dev, void* workspace_dev,
+                   int64_t workspace_bytes);
+/* Gradients of gpb_gated_unit from dout [rows][outer] and the forward inputs
+ * (the projections are recomputed, nothing is kept from the forward call):
+ * dx [rows][inner], dw_gate and dw_up [outer][inner], db_gate and db_up
+ * [outer], each optional (NULL). Outputs overlap neither inputs nor one
+ * another. rows = 0 writes zero weight and bias gradients. */
+int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t activation,
+                            int64_t rows, int64_t inner, int64_t outer, const void* dout_dev,
+                            int64_t dout_ld, const void* x_dev, int64_t x_ld,
+                            const void* w_gate_dev, const void* w_up_dev, int64_t w_ld,
+                            const void* b_gate_dev, const void* b_up_dev, void* dx_dev,
+                            int64_t dx_ld, void* dw_gate_dev, void* dw_up_dev, int64_t dw_ld,
+                            void* db_gate_dev, void* db_up_dev, void* workspace_dev,
+                            int64_t workspace_bytes);
+
+/* out = keep ? x / (1 - p) : 0, plus residual where not NULL. Element
+ * e = row * cols + col is kept iff word e % 4 of Philox4x32-10 block
+ * (counter = (e / 4, offset), key = seed) is >= floor(p 2^32), whatever the
+ * strides; the mask is never stored, and the backward pass is this call on
+ * dout with the same p, seed and offset. A dropped element is 0 whatever x
+ * holds. out may be x or residual itself. */
+int gpb_dropout(int32_t device, void* stream, int32_t dtype, int64_t rows, int64_t cols,
+                void* out_dev, int64_t out_ld, const void* x_dev, int64_t x_ld,
+                const void* residual_dev, int64_t residual_ld, double p, uint64_t seed,
+                uint64_t offset);
+
+/* out [n][d] = d/dX sum_c a_c' K(X, X) b_c at the provider's inputs and
+ * parameters (no noise term), a and b column-major [ncols][n]: row i is
+ * sum_j sum_c (a_ci b_cj + b_ci a_cj) dk(x_i, x_j)/dx_i. Beside
+ * gpb_gradient_bilinear, which takes the same form's gradient by the
+ * parameters. stream NULL = the provider's stream; any other stream handle is
+ * used as it is (cudaStreamLegacy names the default stream). out must not
+ * overlap an input. */
+int gpb_input_gradient(gpb_provider* p, float* out_dev, const float* a_dev, const float* b_dev,
+                       int64_t ncols, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

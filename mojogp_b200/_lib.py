@@ -90,6 +90,18 @@ SIGNATURES = {
     "gpb_lmc_build_precond": [P, c_i32, PI32, P],
     "gpb_lmc_precond_apply": [P, P, P, c_i64],
     "gpb_lmc_precond_sample": [P, P, c_i32, C.c_uint64],
+    "gpb_layer_norm": [c_i32, P, c_i32, c_i32, c_i64, c_i64, P, c_i64, P, c_i64, P, P, c_f32, P, P],
+    "gpb_layer_norm_workspace": [c_i64, c_i64, PI64],
+    "gpb_layer_norm_backward": [c_i32, P, c_i32, c_i32, c_i64, c_i64, P, c_i64, P, c_i64, P, c_i64,
+                                P, P, P, P, P, P, c_i64],
+    "gpb_gated_unit_workspace": [c_i32, c_i64, c_i64, c_i64, c_i32, PI64],
+    "gpb_gated_unit": [c_i32, P, c_i32, c_i32, c_i64, c_i64, c_i64, P, c_i64, P, c_i64, P, P, c_i64,
+                       P, P, P, c_i64],
+    "gpb_gated_unit_backward": [c_i32, P, c_i32, c_i32, c_i64, c_i64, c_i64, P, c_i64, P, c_i64, P,
+                                P, c_i64, P, P, P, c_i64, P, P, c_i64, P, P, P, c_i64],
+    "gpb_dropout": [c_i32, P, c_i32, c_i64, c_i64, P, c_i64, P, c_i64, P, c_i64, c_f64, C.c_uint64,
+                    C.c_uint64],
+    "gpb_input_gradient": [P, P, P, P, c_i64, P],
     "gpb_lmc_predict_exact_variance": [P, P, c_i64, c_i32, c_i32, c_f32, P, PI32],
 }
 _RESTYPES = {"gpb_version": C.c_char_p}

@@ -1,0 +1,98 @@
+// Shared by the feature-map operators (layer norm, gated unit, dropout): element types, 16-byte
+// vectors, the device guard of their entry points and their argument checks. These operators take
+// no provider: every call names its device and stream and brings its own workspace, so calls on
+// different streams (or in captured graphs) share nothing that the caller did not pass twice.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "gpb_common.cuh"
+
+namespace gpb {
+
+// B200 has 148 SMs; grids and workspace sizes that depend on the count use the constant, so that a
+// workspace query needs no device.
+constexpr int kFeatSMs = 148;
+
+// Makes `device` current for the scope and restores the caller's device afterwards: these calls
+// are made from programs that own the current device themselves.
+struct DeviceScope {
+  int saved = -1;
+  cudaError_t status;
+  explicit DeviceScope(int device) {
+    status = cudaGetDevice(&saved);
+    if (status == cudaSuccess && saved != device)
+      status = cudaSetDevice(device);
+    else if (status == cudaSuccess)
+      saved = -1;
+  }
+  ~DeviceScope() {
+    if (saved >= 0) cudaSetDevice(saved);
+  }
+};
+
+#define GPB_DEVICE_SCOPE(device)                                                              \
+  ::gpb::DeviceScope gpb_scope_(device);                                                      \
+  GPB_REQUIRE(gpb_scope_.status == cudaSuccess, GPB_ERR_CUDA, "device %d: %s", (int)(device), \
+              cudaGetErrorString(gpb_scope_.status))
+
+inline bool dtype_ok(int32_t dt) {
+  return dt == GPB_DTYPE_F32 || dt == GPB_DTYPE_F16 || dt == GPB_DTYPE_BF16;
+}
+inline int dtype_bytes(int32_t dt) { return dt == GPB_DTYPE_F32 ? 4 : 2; }
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+// Bytes from the first to one past the last element of a [rows][cols] block of leading dimension ld.
+inline int64_t span_bytes(int64_t rows, int64_t cols, int64_t ld, int esize) {
+  return rows > 0 && cols > 0 ? ((rows - 1) * ld + cols) * esize : 0;
+}
+inline bool overlaps(const void* a, int64_t abytes, const void* b, int64_t bbytes) {
+  if (!a || !b || abytes <= 0 || bbytes <= 0) return false;
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + (uintptr_t)bbytes && y < x + (uintptr_t)abytes;
+}
+// Natural alignment of the element type (a view of a byte buffer may miss it).
+inline bool elem_aligned(const void* p, int esize) { return ((uintptr_t)p % (uintptr_t)esize) == 0; }
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// VEC elements moved together: accesses of at most 16 bytes (a float32 weight vector beside 8 16-bit
+// elements is two of them), so 16-byte alignment is enough for every type.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Pack {
+  T v[VEC];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&out)[VEC]) {
+  const Pack<T, VEC> q = *reinterpret_cast<const Pack<T, VEC>*>(p);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) out[i] = to_f(q.v[i]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&in)[VEC]) {
+  Pack<T, VEC> q;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) q.v[i] = from_f<T>(in[i]);
+  *reinterpret_cast<Pack<T, VEC>*>(p) = q;
+}
+
+}  // namespace gpb

@@ -200,6 +200,36 @@ class Provider:
         _lib.call("gpb_gradient_bilinear", self.h, a.cptr, b.cptr, int(ncols), _ptr(data), _ptr(trace))
         return data, trace
 
+    def input_gradient(self, out, a, b, ncols: int, stream: Optional[int] = None) -> None:
+        """out [n, d] = d/dX sum_c a_c' K(X, X) b_c for a and b [ncols][n]
+        (float32): the gradient of gradient_bilinear's form by the inputs.
+        Arrays are DeviceBuffers, or contiguous device arrays with `data_ptr()`.
+        Runs on the provider's stream, or on the CUDA stream handle `stream`
+        (0 = the legacy default stream)."""
+        ncols = int(ncols)
+        if ncols < 1:
+            raise ValueError(f"ncols must be >= 1, got {ncols}")
+        ptrs = []
+        for name, v, count in (("out", out, self.n * self.d), ("a", a, ncols * self.n),
+                               ("b", b, ncols * self.n)):
+            data_ptr = getattr(v, "data_ptr", None)
+            if data_ptr is None:
+                size, kind, device = v.nbytes // v.dtype.itemsize, v.dtype.name, v.device
+                ptr = v.ptr
+            else:
+                if not v.is_contiguous():
+                    raise ValueError(f"{name} must be contiguous")
+                size, kind = v.numel(), str(v.dtype).rsplit(".", 1)[-1]
+                device, ptr = v.device.index if v.device.type == "cuda" else None, data_ptr()
+            if kind != "float32" or size < count:
+                raise ValueError(f"{name} must hold {count} float32 values, got {size} {kind}")
+            if device != self.device:
+                raise ValueError(f"{name} must be on device {self.device}")
+            ptrs.append(ptr)
+        # Handle 0 is the default stream; the C call's NULL means the provider's.
+        handle = None if stream is None else (int(stream) or 1)
+        _lib.call("gpb_input_gradient", self.h, *ptrs, ncols, handle)
+
     # ------------------------------------------------------------ host helpers
     def matvec_host(self, V: np.ndarray) -> np.ndarray:
         """out = (K + noise I) V for a host array V [n] or [n, t] (column layout)."""
