@@ -450,6 +450,13 @@ int gpb_forward_matvec_noalloc(gpb_provider* p, float* out_dev, const float* v_d
 #define GPB_ACT_SIGMOID 2
 #define GPB_ACT_TANH 3
 
+/* Waits for `device` and reports (and clears) the feature-map operators' device
+ * error word: 0, or 1 when a bounded wait inside a gated-unit kernel gave up,
+ * in which case that call's outputs are not valid. Never needed for ordering;
+ * for programs that want the check every so often, as
+ * gpb_provider_synchronize makes for a provider. */
+int gpb_feature_status(int32_t device, int32_t* status_out);
+
 /* out = (x - mean) rstd weight + bias over each row of x [rows][cols], with
  * rstd = 1 / sqrt(mean((x - mean)^2) + eps). weight and bias [cols] may be
  * NULL (1 and 0) and are param_dtype: float32 or x's type. mean_dev and

@@ -90,6 +90,7 @@ SIGNATURES = {
     "gpb_lmc_build_precond": [P, c_i32, PI32, P],
     "gpb_lmc_precond_apply": [P, P, P, c_i64],
     "gpb_lmc_precond_sample": [P, P, c_i32, C.c_uint64],
+    "gpb_feature_status": [c_i32, PI32],
     "gpb_layer_norm": [c_i32, P, c_i32, c_i32, c_i64, c_i64, P, c_i64, P, c_i64, P, P, c_f32, P, P],
     "gpb_layer_norm_workspace": [c_i64, c_i64, PI64],
     "gpb_layer_norm_backward": [c_i32, P, c_i32, c_i32, c_i64, c_i64, P, c_i64, P, c_i64, P, c_i64,
@@ -107,6 +108,7 @@ SIGNATURES = {
 _RESTYPES = {"gpb_version": C.c_char_p}
 
 ERR_INVALID = -1
+ERR_DEVICE = -5
 
 
 class GPBError(RuntimeError):

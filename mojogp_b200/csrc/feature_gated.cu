@@ -4,38 +4,21 @@
 // Backward, with gate and up recomputed (they are never stored):
 //   dgate = dout up act'(gate),  dup = dout act(gate)
 //   dx = dgate Wg + dup Wu,  dWg = dgate' x,  dWu = dup' x,  dbg, dbu = column sums
-// Sums are held in fp32. dgate and dup are rounded once to the element type, as operands of the
-// three products that follow (fp32 inputs keep them in fp32).
+//
+// Up to kFewRows rows read every weight once for a handful of multiply-adds: HBM bound, on the CUDA
+// cores in fp32 (gated_rows_*). More rows run on the tensor cores (gated_gemm.cuh).
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 
-#include "features.cuh"
+#include "gated_gemm.cuh"
 
 namespace gpb {
 
-enum GatedAct : int32_t { ACT_SILU = 0, ACT_GELU = 1, ACT_SIGMOID = 2, ACT_TANH = 3 };
+constexpr int kFewRows = 8;
 
-// act(z) and act'(z). Silu z s(z), gelu z Phi(z), with s the logistic function and Phi the normal
-// distribution function (exact erf form).
-__device__ __forceinline__ void gated_act(int act, float z, float& value, float& slope) {
-  if (act == ACT_GELU) {
-    const float cdf = 0.5f * erfcf(-0.70710678f * z);
-    value = z * cdf;
-    slope = fmaf(z * 0.39894228f, expf(-0.5f * z * z), cdf);
-  } else if (act == ACT_TANH) {
-    value = tanhf(z);
-    slope = fmaf(-value, value, 1.f);
-  } else {
-    const float s = 1.f / (1.f + expf(-z));
-    if (act == ACT_SIGMOID) {
-      value = s;
-      slope = s * (1.f - s);
-    } else {
-      value = z * s;
-      slope = s * fmaf(z, 1.f - s, 1.f);
-    }
-  }
-}
+// Set by a kernel whose bounded wait ran out; read and cleared by gpb_feature_status.
+__device__ int g_feature_err;
 
 struct GatedArgs {
   const void* x;
@@ -44,66 +27,91 @@ struct GatedArgs {
   const void* bg;
   const void* bu;
   const void* dout;
-  void* out;   // forward
-  void* dg;    // backward: [rows][outer] operands of the products
-  void* du;
+  void* out;  // forward
   int64_t x_ld, w_ld, out_ld, dout_ld;
   int64_t rows, inner, outer;
   int32_t act;
 };
 
-constexpr int kTile = 64, kTileK = 16;
+struct GatedGrads {
+  void* dx;
+  int64_t dx_ld;
+  void* dwg;
+  void* dwu;
+  int64_t dw_ld;
+  void* dbg;
+  void* dbu;
+};
 
-// One 64 x 64 tile of both projections per block, 256 threads x 4 x 4 values each; BACK writes dgate
-// and dup instead of the product.
-template <typename T, bool BACK>
-__global__ void __launch_bounds__(256) gated_simt_kernel(const GatedArgs A) {
-  __shared__ float xs[kTileK][kTile + 4], gs[kTileK][kTile + 4], us[kTileK][kTile + 4];
-  const int64_t tiles_n = (A.outer + kTile - 1) / kTile;
-  const int64_t m0 = (blockIdx.x / tiles_n) * kTile, n0 = (blockIdx.x % tiles_n) * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float g[4][4] = {}, u[4][4] = {};
-  for (int64_t k0 = 0; k0 < A.inner; k0 += kTileK) {
-    for (int q = threadIdx.x; q < kTile * kTileK; q += 256) {
-      const int r = q / kTileK, k = q % kTileK;
-      const bool kin = k0 + k < A.inner;
-      xs[k][r] = kin && m0 + r < A.rows ? to_f(((const T*)A.x)[(m0 + r) * A.x_ld + k0 + k]) : 0.f;
-      const bool in = kin && n0 + r < A.outer;
-      const int64_t wi = (n0 + r) * A.w_ld + k0 + k;
-      gs[k][r] = in ? to_f(((const T*)A.wg)[wi]) : 0.f;
-      us[k][r] = in ? to_f(((const T*)A.wu)[wi]) : 0.f;
-    }
-    __syncthreads();
+// ------------------------------------------------------------- few rows
+// One warp (WPO = 1) or one block (WPO = 8) per output column; lanes run along the weight row. BACK
+// writes dgate and dup [rows][outer] in fp32.
+template <typename T, int ROWS, int VEC, int WPO, bool BACK>
+__global__ void __launch_bounds__(256) gated_rows_kernel(const GatedArgs A, float* dg, float* du) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n = WPO == 1 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
+  float g[ROWS], u[ROWS];
 #pragma unroll
-    for (int k = 0; k < kTileK; ++k) {
+  for (int m = 0; m < ROWS; ++m) g[m] = u[m] = 0.f;
+  if (n < A.outer) {
+    const T* wg = (const T*)A.wg + n * A.w_ld;
+    const T* wu = (const T*)A.wu + n * A.w_ld;
+    constexpr int kStep = (WPO == 1 ? 32 : 256) * VEC;
+#pragma unroll 4
+    for (int64_t k = (WPO == 1 ? lane : (int)threadIdx.x) * VEC; k < A.inner; k += kStep) {
+      float a[VEC], b[VEC];
+      load_vec<T, VEC>(wg + k, a);
+      load_vec<T, VEC>(wu + k, b);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = xs[k][ty * 4 + i];
+      for (int m = 0; m < ROWS; ++m) {
+        if (m < A.rows) {
+          float x[VEC];
+          load_vec<T, VEC>((const T*)A.x + m * A.x_ld + k, x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          g[i][j] = fmaf(a, gs[k][tx * 4 + j], g[i][j]);
-          u[i][j] = fmaf(a, us[k][tx * 4 + j], u[i][j]);
+          for (int i = 0; i < VEC; ++i) {
+            g[m] = fmaf(x[i], a[i], g[m]);
+            u[m] = fmaf(x[i], b[i], u[m]);
+          }
         }
       }
     }
-    __syncthreads();
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty * 4 + i;
-    if (m >= A.rows) break;
+  for (int m = 0; m < ROWS; ++m)
+    for (int o = 16; o > 0; o >>= 1) {
+      g[m] += __shfl_xor_sync(0xffffffffu, g[m], o);
+      u[m] += __shfl_xor_sync(0xffffffffu, u[m], o);
+    }
+  if constexpr (WPO == 8) {
+    __shared__ float sums[8][2][ROWS];
+    if (lane == 0)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + tx * 4 + j;
-      if (n >= A.outer) break;
-      const float gate = g[i][j] + (A.bg ? to_f(((const T*)A.bg)[n]) : 0.f);
-      const float up = u[i][j] + (A.bu ? to_f(((const T*)A.bu)[n]) : 0.f);
+      for (int m = 0; m < ROWS; ++m) {
+        sums[warp][0][m] = g[m];
+        sums[warp][1][m] = u[m];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) {
+      g[m] = u[m] = 0.f;
+      for (int w = 0; w < 8; ++w) {
+        g[m] += sums[w][0][m];
+        u[m] += sums[w][1][m];
+      }
+    }
+  }
+  if (n >= A.outer || (WPO == 8 && warp > 0)) return;
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) {
+    if (lane == m && m < A.rows) {
+      const float gate = g[m] + (A.bg ? to_f(((const T*)A.bg)[n]) : 0.f);
+      const float up = u[m] + (A.bu ? to_f(((const T*)A.bu)[n]) : 0.f);
       float value, slope;
       gated_act(A.act, gate, value, slope);
       if constexpr (BACK) {
         const float dy = to_f(((const T*)A.dout)[m * A.dout_ld + n]);
-        ((T*)A.dg)[m * A.outer + n] = from_f<T>(dy * up * slope);
-        ((T*)A.du)[m * A.outer + n] = from_f<T>(dy * value);
+        dg[m * A.outer + n] = dy * up * slope;
+        du[m * A.outer + n] = dy * value;
       } else {
         ((T*)A.out)[m * A.out_ld + n] = from_f<T>(value * up);
       }
@@ -111,97 +119,115 @@ __global__ void __launch_bounds__(256) gated_simt_kernel(const GatedArgs A) {
   }
 }
 
-// C [m][n] = sum over terms and k of A_t(m, k) B_t(k, n), any strides; blockIdx.z = a range of k whose
-// fp32 partial sums go to `partial` (one range: C is written directly).
-struct MmTerm {
-  const void* a;
-  const void* b;
-};
-struct MmArgs {
-  MmTerm term[2];
-  int32_t terms;
-  int64_t a_m, a_k, b_k, b_n;
-  int64_t M, N, K;
-  void* c;
-  int64_t c_ld;
-  float* partial;
-  int64_t k_per;
-};
-
-template <typename T>
-__global__ void __launch_bounds__(256) mm_simt_kernel(const MmArgs A) {
-  __shared__ float as[kTileK][kTile + 4], bs[kTileK][kTile + 4];
-  const int64_t tiles_n = (A.N + kTile - 1) / kTile;
-  const int64_t m0 = (blockIdx.x / tiles_n) * kTile, n0 = (blockIdx.x % tiles_n) * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t kb = blockIdx.z * A.k_per;
-  const int64_t ke = kb + A.k_per < A.K ? kb + A.k_per : A.K;
-  float c[4][4] = {};
-  for (int t = 0; t < A.terms; ++t) {
-    const T* a = (const T*)A.term[t].a;
-    const T* b = (const T*)A.term[t].b;
-    for (int64_t k0 = kb; k0 < ke; k0 += kTileK) {
-      for (int q = threadIdx.x; q < kTile * kTileK; q += 256) {
-        // Neighbouring threads along the unit stride of each operand.
-        const int ar = A.a_k == 1 ? q / kTileK : q % kTile, ak = A.a_k == 1 ? q % kTileK : q / kTile;
-        const int br = A.b_k == 1 ? q / kTileK : q % kTile, bk = A.b_k == 1 ? q % kTileK : q / kTile;
-        as[ak][ar] = k0 + ak < ke && m0 + ar < A.M
-                         ? to_f(a[(m0 + ar) * A.a_m + (k0 + ak) * A.a_k]) : 0.f;
-        bs[bk][br] = k0 + bk < ke && n0 + br < A.N
-                         ? to_f(b[(k0 + bk) * A.b_k + (n0 + br) * A.b_n]) : 0.f;
+// dx of few rows: a thread owns VEC columns of the weights and walks a range of their rows
+// (blockIdx.y); the ranges' sums are joined by mm_join_kernel.
+template <typename T, int ROWS, int VEC>
+__global__ void __launch_bounds__(128) gated_rows_dx_kernel(const GatedArgs A, const float* dg,
+                                                            const float* du, int64_t per,
+                                                            float* partial) {
+  const int64_t k = ((int64_t)blockIdx.x * 128 + threadIdx.x) * VEC;
+  if (k >= A.inner) return;
+  const int64_t n0 = blockIdx.y * per, n1 = n0 + per < A.outer ? n0 + per : A.outer;
+  float acc[ROWS][VEC];
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[m][i] = 0.f;
+#pragma unroll 4
+  for (int64_t n = n0; n < n1; ++n) {
+    float a[VEC], b[VEC];
+    load_vec<T, VEC>((const T*)A.wg + n * A.w_ld + k, a);
+    load_vec<T, VEC>((const T*)A.wu + n * A.w_ld + k, b);
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) {
+      if (m < A.rows) {
+        const float p = dg[m * A.outer + n], q = du[m * A.outer + n];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[m][i] = fmaf(p, a[i], fmaf(q, b[i], acc[m][i]));
       }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kTileK; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            c[i][j] = fmaf(as[k][ty * 4 + i], bs[k][tx * 4 + j], c[i][j]);
-      __syncthreads();
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty * 4 + i;
-    if (m >= A.M) break;
+  for (int m = 0; m < ROWS; ++m)
+    if (m < A.rows)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + tx * 4 + j;
-      if (n >= A.N) break;
-      if (gridDim.z == 1)
-        ((T*)A.c)[m * A.c_ld + n] = from_f<T>(c[i][j]);
-      else
-        A.partial[(blockIdx.z * A.M + m) * A.N + n] = c[i][j];
-    }
-  }
+      for (int i = 0; i < VEC; ++i)
+        partial[((int64_t)blockIdx.y * A.rows + m) * A.inner + k + i] = acc[m][i];
 }
 
-// C = sum of the ranges' partial sums, in range order.
+// dWg, dWu and the bias gradients of few rows: sums of ROWS outer products, written once.
+template <typename T, int ROWS, int VEC>
+__global__ void __launch_bounds__(128) gated_rows_dw_kernel(const GatedArgs A, const GatedGrads G,
+                                                            const float* dg, const float* du) {
+  const int64_t k = ((int64_t)blockIdx.y * 128 + threadIdx.x) * VEC;
+  const int64_t n = blockIdx.x;
+  float p[ROWS], q[ROWS], sp = 0.f, sq = 0.f;
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) {
+    p[m] = m < A.rows ? dg[m * A.outer + n] : 0.f;
+    q[m] = m < A.rows ? du[m * A.outer + n] : 0.f;
+    sp += p[m];
+    sq += q[m];
+  }
+  if (blockIdx.y == 0 && threadIdx.x == 0) {
+    if (G.dbg) ((T*)G.dbg)[n] = from_f<T>(sp);
+    if (G.dbu) ((T*)G.dbu)[n] = from_f<T>(sq);
+  }
+  if (k >= A.inner) return;
+  float a[VEC], b[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) a[i] = b[i] = 0.f;
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m) {
+    if (m < A.rows) {
+      float x[VEC];
+      load_vec<T, VEC>((const T*)A.x + m * A.x_ld + k, x);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        a[i] = fmaf(p[m], x[i], a[i]);
+        b[i] = fmaf(q[m], x[i], b[i]);
+      }
+    }
+  }
+  if (G.dwg) store_vec<T, VEC>((T*)G.dwg + n * G.dw_ld + k, a);
+  if (G.dwu) store_vec<T, VEC>((T*)G.dwu + n * G.dw_ld + k, b);
+}
+
+// ------------------------------------------------------------- helpers
+// C = sum of the ranges' partial sums [range][halves][M][N], in range order.
 template <typename T>
 __global__ void __launch_bounds__(256) mm_join_kernel(const float* __restrict__ partial, int ranges,
-                                                      int64_t M, int64_t N, T* c, int64_t c_ld) {
+                                                      int64_t M, int64_t N, int halves, T* c0, T* c1,
+                                                      int64_t c_ld) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= M * N) return;
+  if (e >= halves * M * N) return;
   float s = 0.f;
-  for (int r = 0; r < ranges; ++r) s += partial[r * M * N + e];
-  c[(e / N) * c_ld + e % N] = from_f<T>(s);
+  for (int r = 0; r < ranges; ++r) s += partial[r * halves * M * N + e];
+  const int half = e >= M * N;
+  T* c = half ? c1 : c0;
+  const int64_t f = e - half * M * N;
+  if (c) c[(f / N) * c_ld + f % N] = from_f<T>(s);
 }
 
-// Column sums of dgate and dup (blockIdx.y picks one): 32 columns x 8 row lanes per block, rows in
-// ranges over blockIdx.z, joined by gated_bias_join.
-template <typename T>
-__global__ void __launch_bounds__(256) gated_bias_kernel(const T* dg, const T* du, int64_t rows,
-                                                         int64_t outer, float* partial) {
+// Column sums of the planes of dgate and dup (blockIdx.y picks one): 32 columns x 8 row lanes per
+// block, rows in ranges over blockIdx.z, joined in range order by gated_bias_join.
+template <typename D>
+__global__ void __launch_bounds__(256) gated_bias_kernel(const D* dg, const D* du, int64_t rows,
+                                                         int64_t outer, int64_t ld, int planes,
+                                                         int64_t plane, float* partial) {
   __shared__ float sums[8][33];
-  const T* d = blockIdx.y == 0 ? dg : du;
+  const D* d = blockIdx.y == 0 ? dg : du;
   const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
   const int part = threadIdx.x >> 5;
   const int64_t per = (rows + gridDim.z - 1) / gridDim.z;
   const int64_t r0 = blockIdx.z * per, r1 = r0 + per < rows ? r0 + per : rows;
   float s = 0.f;
   if (c < outer)
-    for (int64_t r = r0 + part; r < r1; r += 8) s += to_f(d[r * outer + c]);
+    for (int64_t r = r0 + part; r < r1; r += 8) {
+      float v = to_f(d[r * ld + c]);
+      for (int p = 1; p < planes; ++p) v += to_f(d[p * plane + r * ld + c]);
+      s += v;
+    }
   sums[part][threadIdx.x & 31] = s;
   __syncthreads();
   if (part == 0 && c < outer) {
@@ -220,114 +246,389 @@ __global__ void __launch_bounds__(256) gated_bias_join(const float* partial, int
   if (dst) dst[e < outer ? e : e - outer] = from_f<T>(s);
 }
 
+// A matrix to tensor-core operands: fp32 to three bf16 planes, or a 16-bit matrix whose rows are not
+// 16-byte aligned to one plane whose are. 8 output columns per thread; columns up to ld are zeros.
+template <typename T, typename D>
+__global__ void __launch_bounds__(256) gated_pack_kernel(const T* __restrict__ src, int64_t src_ld,
+                                                         int64_t rows, int64_t cols, int64_t ld,
+                                                         int64_t plane, D* __restrict__ dst) {
+  const int64_t run = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t per = ld / 8;
+  if (run >= rows * per) return;
+  const int64_t r = run / per, c = (run - r * per) * 8;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f(src[r * src_ld + c + i]) : 0.f;
+  if constexpr (sizeof(T) == 4) {
+    float h[8], m[8], l[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) gg_split3(v[i], h[i], m[i], l[i]);
+    store_vec<D, 8>(dst + r * ld + c, h);
+    store_vec<D, 8>(dst + plane + r * ld + c, m);
+    store_vec<D, 8>(dst + 2 * plane + r * ld + c, l);
+  } else {
+    store_vec<D, 8>(dst + r * ld + c, v);
+  }
+}
+
 // ------------------------------------------------------------------ host
-// Workspace of the backward pass: dgate | dup | partial sums.
-struct GatedPlan {
-  int64_t dg = 0, du = 0, partial = 0, total = 0;
-  int ranges_w = 1;  // ranges of rows for dWg and dWu
-  int ranges_b = 1;  // ranges of rows for the biases
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static int encode_fn(EncodeTiled* fn) {
+  static EncodeTiled cached = nullptr;  // the same pointer whichever thread writes it
+  if (!cached) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    GPB_CHECK_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
+    GPB_REQUIRE(p && q == cudaDriverEntryPointSuccess, GPB_ERR_CUDA,
+                "cuTensorMapEncodeTiled is not available");
+    cached = (EncodeTiled)p;
+  }
+  *fn = cached;
+  return GPB_OK;
+}
+
+// A 16-bit operand: `planes` matrices [rows][cols] with leading dimension ld (a multiple of 8).
+struct Operand {
+  const void* p = nullptr;
+  int64_t rows = 0, cols = 0, ld = 0, plane = 0;
+  int planes = 1;
 };
+
+static int make_map(const Operand& o, int box_rows, CUtensorMap* map) {
+  EncodeTiled fn;
+  GPB_TRY(encode_fn(&fn));
+  const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+  const int64_t plane = o.planes > 1 ? o.plane : o.rows * o.ld;
+  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)plane * 2};
+  const cuuint32_t box[3] = {kGgBK, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+  const CUresult r =
+      fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(o.p), dims, strides, box, step,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  GPB_REQUIRE(r == CUDA_SUCCESS, GPB_ERR_CUDA, "tensor map of %lld x %lld (stride %lld): error %d",
+              (long long)o.rows, (long long)o.cols, (long long)o.ld, (int)r);
+  return GPB_OK;
+}
+
+// Workspace of a call; every offset is a multiple of 256 bytes.
+struct GatedPlan {
+  bool few = false;                    // CUDA-core path
+  int planes = 1;                      // of packed x and weights
+  int64_t ldk = 0, ldn = 0;            // leading dimensions of packed operands and of dgate / dup
+  int64_t x = 0, wg = 0, wu = 0;       // packed operands
+  int64_t dg = 0, du = 0, plane_d = 0; // dgate and dup (elements between planes)
+  int64_t partial = 0, total = 0;
+  int tile_n = 0;                      // GG_DW column tile
+  int splits = 1, kb_per = 1;          // GG_DW
+  int ranges_b = 1;                    // bias gradients
+  int ranges_x = 1;                    // dx of few rows
+};
+
+static int64_t take(int64_t& at, int64_t bytes) {
+  const int64_t o = at;
+  at += round_up(bytes, 256);
+  return o;
+}
+
+// Column tile of a GG_DX / GG_DW product with n output columns.
+static int plain_tile(int64_t n, bool f32) { return n <= 64 ? 64 : n <= 128 || f32 ? 128 : 256; }
+// MMA width of GG_PROJ: gate and up columns of one tile.
+static int proj_tile(int64_t outer, bool f32) { return outer <= 32 ? 64 : outer <= 64 || f32 ? 128 : 256; }
 
 static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t dtype, bool backward) {
   GatedPlan P;
-  if (!backward) return P;
-  const int64_t op = round_up(rows * outer * dtype_bytes(dtype), 256);
-  P.dg = 0;
-  P.du = op;
-  P.partial = 2 * op;
-  const int64_t tiles = ceil_div(outer, kTile) * ceil_div(inner, kTile);
-  int64_t r = ceil_div(4 * kFeatSMs, tiles);
-  r = std::min<int64_t>(r, ceil_div(rows, 256));
-  P.ranges_w = (int)std::max<int64_t>(1, r);
-  P.ranges_b = (int)std::max<int64_t>(
-      1, std::min<int64_t>(ceil_div(4 * kFeatSMs, ceil_div(outer, 32)), ceil_div(rows, 256)));
-  const int64_t pw = P.ranges_w > 1 ? P.ranges_w * outer * inner : 0;
-  P.total = P.partial + round_up(std::max<int64_t>(pw, P.ranges_b * 2 * outer) * 4, 256);
+  const bool f32 = dtype == GPB_DTYPE_F32;
+  int64_t at = 0;
+  if (rows <= kFewRows) {
+    P.few = true;
+    if (!backward) return P;
+    P.dg = take(at, rows * outer * 4);
+    P.du = take(at, rows * outer * 4);
+    const int vec = 16 / dtype_bytes(dtype);
+    const int64_t cols = ceil_div(inner, 128 * vec);
+    P.ranges_x = (int)std::max<int64_t>(
+        1, std::min<int64_t>(ceil_div(outer, 16), ceil_div(4 * kFeatSMs, cols)));
+    P.partial = take(at, P.ranges_x * rows * inner * 4);
+    P.total = at;
+    return P;
+  }
+  P.planes = f32 ? 3 : 1;
+  P.ldk = round_up(inner, 8);
+  P.ldn = round_up(outer, 8);
+  P.x = take(at, P.planes * rows * P.ldk * 2);
+  P.wg = take(at, P.planes * outer * P.ldk * 2);
+  P.wu = take(at, P.planes * outer * P.ldk * 2);
+  if (backward) {
+    P.plane_d = rows * P.ldn;
+    P.dg = take(at, P.planes * P.plane_d * 2);
+    P.du = take(at, P.planes * P.plane_d * 2);
+    P.tile_n = plain_tile(inner, f32);
+    const int64_t tiles = (outer <= 64 ? 1 : 2 * ceil_div(outer, kGgBM)) * ceil_div(inner, P.tile_n);
+    const int64_t kb = ceil_div(rows, kGgBK);
+    // At least 8 stages per range; as many ranges as fill the SMs twice.
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * kFeatSMs / tiles, kb / 8));
+    P.kb_per = (int)ceil_div(kb, want);
+    P.splits = (int)ceil_div(kb, P.kb_per);
+    P.ranges_b = (int)std::max<int64_t>(
+        1, std::min<int64_t>(ceil_div(4 * kFeatSMs, ceil_div(outer, 32)), ceil_div(rows, 256)));
+    P.partial = take(at, std::max<int64_t>(P.splits > 1 ? P.splits * 2 * outer * inner : 0,
+                                           P.ranges_b * 2 * outer) * 4);
+  }
+  P.total = at;
   return P;
 }
 
-template <typename T>
-static int gated_forward(const GatedArgs& A, cudaStream_t st) {
-  const int64_t grid = ceil_div(A.rows, kTile) * ceil_div(A.outer, kTile);
-  gated_simt_kernel<T, false><<<(unsigned)grid, 256, 0, st>>>(A);
+template <int MODE, int NB, int PA, int PB, typename T, typename D, int PD, bool BACK>
+static int gg_launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0,
+                     const CUtensorMap& b1, GgArgs& G, cudaStream_t st) {
+  using S = GgShape<MODE, NB, PA, PB>;
+  constexpr auto kernel = gated_gemm_kernel<MODE, NB, PA, PB, T, D, PD, BACK>;
+  GPB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  void* err = nullptr;
+  GPB_CHECK_CUDA(cudaGetSymbolAddress(&err, g_feature_err));
+  G.err = (int*)err;
+  G.idesc = gg_idesc(std::is_same<D, __nv_bfloat16>::value, MODE == GG_DW, MODE != GG_PROJ, NB);
+  const int64_t items = (int64_t)G.tiles_m * G.tiles_n * G.splits;
+  kernel<<<(unsigned)std::min<int64_t>(items, kFeatSMs), kGgThreads, S::kSmem, st>>>(a0, a1, b0, b1, G);
   GPB_CHECK_CUDA(cudaGetLastError());
   return GPB_OK;
 }
 
-template <typename T>
-static int mm_launch(MmArgs M, int ranges, cudaStream_t st) {
-  const int64_t grid = ceil_div(M.M, kTile) * ceil_div(M.N, kTile);
-  M.k_per = round_up(ceil_div(M.K, ranges), kTileK);
-  ranges = (int)ceil_div(M.K, M.k_per);
-  mm_simt_kernel<T><<<dim3((unsigned)grid, 1, ranges), 256, 0, st>>>(M);
+// x and the weights as tensor-core operands: where they lie when they are 16-bit with aligned rows,
+// packed into the workspace otherwise.
+template <typename T, typename D>
+static int gated_operand(const void* p, int64_t rows, int64_t cols, int64_t ld, const GatedPlan& P,
+                         char* packed, Operand* o, cudaStream_t st) {
+  o->rows = rows;
+  o->cols = cols;
+  if (sizeof(T) == 2 && aligned16(p) && ld % 8 == 0) {
+    o->p = p;
+    o->ld = ld;
+    return GPB_OK;
+  }
+  o->p = packed;
+  o->ld = P.ldk;
+  o->planes = P.planes;
+  o->plane = rows * P.ldk;
+  gated_pack_kernel<T, D><<<(unsigned)ceil_div(rows * (P.ldk / 8), 256), 256, 0, st>>>(
+      (const T*)p, ld, rows, cols, P.ldk, o->plane, (D*)packed);
   GPB_CHECK_CUDA(cudaGetLastError());
-  if (ranges > 1) {
-    mm_join_kernel<T><<<(unsigned)ceil_div(M.M * M.N, 256), 256, 0, st>>>(M.partial, ranges, M.M,
-                                                                         M.N, (T*)M.c, M.c_ld);
+  return GPB_OK;
+}
+
+template <typename T, typename D, int PL, bool BACK>
+static int gated_project(const GatedArgs& A, const Operand& x, const Operand& wg, const Operand& wu,
+                         GgArgs G, cudaStream_t st) {
+  const int nb = proj_tile(A.outer, PL == 3);
+  const int bn = nb / 2;
+  CUtensorMap mx, mg, mu;
+  GPB_TRY(make_map(x, kGgBM, &mx));
+  GPB_TRY(make_map(wg, bn, &mg));
+  GPB_TRY(make_map(wu, bn, &mu));
+  G.M = A.rows;
+  G.N = A.outer;
+  G.tiles_m = (int32_t)ceil_div(A.rows, kGgBM);
+  G.tiles_n = (int32_t)ceil_div(A.outer, bn);
+  G.kblocks = (int32_t)ceil_div(A.inner, kGgBK);
+  G.segs = G.splits = 1;
+  G.kb_per = G.kblocks;
+  G.bg = A.bg;
+  G.bu = A.bu;
+  G.act = A.act;
+  G.dout = A.dout;
+  G.dout_ld = A.dout_ld;
+  switch (nb) {
+    case 64: return gg_launch<GG_PROJ, 64, PL, PL, T, D, PL, BACK>(mx, mx, mg, mu, G, st);
+    case 128: return gg_launch<GG_PROJ, 128, PL, PL, T, D, PL, BACK>(mx, mx, mg, mu, G, st);
+    default:
+      if constexpr (PL == 1)
+        return gg_launch<GG_PROJ, 256, PL, PL, T, D, PL, BACK>(mx, mx, mg, mu, G, st);
+      return GPB_ERR_UNSUPPORTED;
+  }
+}
+
+template <int MODE, typename T, typename D, int PL>
+static int gated_plain(const CUtensorMap& a0, const CUtensorMap& a1, const Operand& b0,
+                       const Operand& b1, int nb, GgArgs& G, cudaStream_t st) {
+  CUtensorMap m0, m1;
+  GPB_TRY(make_map(b0, kGgBK, &m0));
+  GPB_TRY(make_map(b1, kGgBK, &m1));
+  switch (nb) {
+    case 64: return gg_launch<MODE, 64, PL, PL, T, D, PL, false>(a0, a1, m0, m1, G, st);
+    case 128: return gg_launch<MODE, 128, PL, PL, T, D, PL, false>(a0, a1, m0, m1, G, st);
+    default:
+      if constexpr (PL == 1)
+        return gg_launch<MODE, 256, PL, PL, T, D, PL, false>(a0, a1, m0, m1, G, st);
+      return GPB_ERR_UNSUPPORTED;
+  }
+}
+
+template <typename T, int ROWS, int VEC, bool BACK>
+static int gated_rows_launch(const GatedArgs& A, float* dg, float* du, cudaStream_t st) {
+  // One warp per output column while that gives every SM 16 warps, else a block per column.
+  if (A.outer >= 16 * kFeatSMs)
+    gated_rows_kernel<T, ROWS, VEC, 1, BACK>
+        <<<(unsigned)ceil_div(A.outer, 8), 256, 0, st>>>(A, dg, du);
+  else
+    gated_rows_kernel<T, ROWS, VEC, 8, BACK><<<(unsigned)A.outer, 256, 0, st>>>(A, dg, du);
+  GPB_CHECK_CUDA(cudaGetLastError());
+  return GPB_OK;
+}
+
+template <typename T, int VEC, bool BACK>
+static int gated_rows_pick(const GatedArgs& A, float* dg, float* du, cudaStream_t st) {
+  if (A.rows <= 1) return gated_rows_launch<T, 1, VEC, BACK>(A, dg, du, st);
+  if (A.rows <= 2) return gated_rows_launch<T, 2, VEC, BACK>(A, dg, du, st);
+  if (A.rows <= 4) return gated_rows_launch<T, 4, VEC, BACK>(A, dg, du, st);
+  return gated_rows_launch<T, kFewRows, VEC, BACK>(A, dg, du, st);
+}
+
+template <typename T, int ROWS, int VEC>
+static int gated_rows_grads(const GatedArgs& A, const GatedGrads& G, const GatedPlan& P, float* dg,
+                            float* du, float* partial, cudaStream_t st) {
+  const int64_t cols = ceil_div(A.inner, 128 * VEC);
+  if (G.dx) {
+    const int64_t per = ceil_div(A.outer, P.ranges_x);
+    const int ranges = (int)ceil_div(A.outer, per);
+    gated_rows_dx_kernel<T, ROWS, VEC>
+        <<<dim3((unsigned)cols, ranges), 128, 0, st>>>(A, dg, du, per, partial);
+    GPB_CHECK_CUDA(cudaGetLastError());
+    mm_join_kernel<T><<<(unsigned)ceil_div(A.rows * A.inner, 256), 256, 0, st>>>(
+        partial, ranges, A.rows, A.inner, 1, (T*)G.dx, nullptr, G.dx_ld);
+    GPB_CHECK_CUDA(cudaGetLastError());
+  }
+  if (G.dwg || G.dwu || G.dbg || G.dbu) {
+    const unsigned gy = G.dwg || G.dwu ? (unsigned)cols : 1;
+    gated_rows_dw_kernel<T, ROWS, VEC><<<dim3((unsigned)A.outer, gy), 128, 0, st>>>(A, G, dg, du);
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   return GPB_OK;
 }
 
-struct GatedGrads {
-  void* dx;
-  int64_t dx_ld;
-  void* dwg;
-  void* dwu;
-  int64_t dw_ld;
-  void* dbg;
-  void* dbu;
-};
+template <typename T, int VEC>
+static int gated_rows_backward(const GatedArgs& A, const GatedGrads& G, const GatedPlan& P, char* ws,
+                               cudaStream_t st) {
+  float *dg = (float*)(ws + P.dg), *du = (float*)(ws + P.du), *partial = (float*)(ws + P.partial);
+  GPB_TRY((gated_rows_pick<T, VEC, true>(A, dg, du, st)));
+  if (A.rows <= 1) return gated_rows_grads<T, 1, VEC>(A, G, P, dg, du, partial, st);
+  if (A.rows <= 2) return gated_rows_grads<T, 2, VEC>(A, G, P, dg, du, partial, st);
+  if (A.rows <= 4) return gated_rows_grads<T, 4, VEC>(A, G, P, dg, du, partial, st);
+  return gated_rows_grads<T, kFewRows, VEC>(A, G, P, dg, du, partial, st);
+}
 
+// x and weights readable as 16-byte vectors.
 template <typename T>
-static int gated_backward(GatedArgs A, const GatedGrads& G, char* ws, const GatedPlan& P,
+static bool gated_vec(const GatedArgs& A) {
+  constexpr int V = 16 / sizeof(T);
+  return A.inner % V == 0 && A.x_ld % V == 0 && A.w_ld % V == 0 && aligned16(A.x) &&
+         aligned16(A.wg) && aligned16(A.wu);
+}
+
+template <typename T, typename D, int PL>
+static int gated_forward(const GatedArgs& A, char* ws, const GatedPlan& P, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if (P.few)
+    return gated_vec<T>(A) ? gated_rows_pick<T, V, false>(A, nullptr, nullptr, st)
+                           : gated_rows_pick<T, 1, false>(A, nullptr, nullptr, st);
+  Operand x, wg, wu;
+  GPB_TRY((gated_operand<T, D>(A.x, A.rows, A.inner, A.x_ld, P, ws + P.x, &x, st)));
+  GPB_TRY((gated_operand<T, D>(A.wg, A.outer, A.inner, A.w_ld, P, ws + P.wg, &wg, st)));
+  GPB_TRY((gated_operand<T, D>(A.wu, A.outer, A.inner, A.w_ld, P, ws + P.wu, &wu, st)));
+  GgArgs G{};
+  G.out[0] = A.out;
+  G.out_ld = A.out_ld;
+  G.vec = aligned16(A.out) && A.out_ld % V == 0;
+  return gated_project<T, D, PL, false>(A, x, wg, wu, G, st);
+}
+
+template <typename T, typename D, int PL>
+static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, const GatedPlan& P,
                           cudaStream_t st) {
-  A.dg = ws + P.dg;
-  A.du = ws + P.du;
+  constexpr int V = 16 / sizeof(T);
+  if (P.few) {
+    const bool vec = gated_vec<T>(A) && (!(R.dwg || R.dwu) || R.dw_ld % V == 0) &&
+                     aligned16(R.dwg) && aligned16(R.dwu);
+    return vec ? gated_rows_backward<T, V>(A, R, P, ws, st)
+               : gated_rows_backward<T, 1>(A, R, P, ws, st);
+  }
+  Operand x, wg, wu;
+  GPB_TRY((gated_operand<T, D>(A.x, A.rows, A.inner, A.x_ld, P, ws + P.x, &x, st)));
+  GPB_TRY((gated_operand<T, D>(A.wg, A.outer, A.inner, A.w_ld, P, ws + P.wg, &wg, st)));
+  GPB_TRY((gated_operand<T, D>(A.wu, A.outer, A.inner, A.w_ld, P, ws + P.wu, &wu, st)));
   float* partial = (float*)(ws + P.partial);
-  const int64_t grid = ceil_div(A.rows, kTile) * ceil_div(A.outer, kTile);
-  gated_simt_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(A);
-  GPB_CHECK_CUDA(cudaGetLastError());
-  if (G.dx) {
-    MmArgs M{};
-    M.term[0] = {A.dg, A.wg};
-    M.term[1] = {A.du, A.wu};
-    M.terms = 2;
-    M.a_m = A.outer;
-    M.a_k = 1;
-    M.b_k = A.w_ld;
-    M.b_n = 1;
-    M.M = A.rows;
-    M.N = A.inner;
-    M.K = A.outer;
-    M.c = G.dx;
-    M.c_ld = G.dx_ld;
-    GPB_TRY(mm_launch<T>(M, 1, st));
+  Operand dg, du;
+  dg.p = ws + P.dg;
+  du.p = ws + P.du;
+  dg.rows = du.rows = A.rows;
+  dg.cols = du.cols = A.outer;
+  dg.ld = du.ld = P.ldn;
+  dg.planes = du.planes = PL;
+  dg.plane = du.plane = P.plane_d;
+  {
+    GgArgs G{};
+    G.out[0] = ws + P.dg;
+    G.out[1] = ws + P.du;
+    G.out_ld = P.ldn;
+    G.plane = P.plane_d;
+    G.vec = aligned16(A.dout) && A.dout_ld % V == 0;
+    GPB_TRY((gated_project<T, D, PL, true>(A, x, wg, wu, G, st)));
   }
-  for (int h = 0; h < 2; ++h) {
-    void* dw = h == 0 ? G.dwg : G.dwu;
-    if (!dw) continue;
-    MmArgs M{};
-    M.term[0] = {h == 0 ? A.dg : A.du, A.x};
-    M.terms = 1;
-    M.a_m = 1;
-    M.a_k = A.outer;
-    M.b_k = A.x_ld;
-    M.b_n = 1;
-    M.M = A.outer;
-    M.N = A.inner;
-    M.K = A.rows;
-    M.c = dw;
-    M.c_ld = G.dw_ld;
-    M.partial = partial;
-    GPB_TRY(mm_launch<T>(M, P.ranges_w, st));
+  if (R.dx) {
+    GgArgs G{};
+    const int nb = plain_tile(A.inner, PL == 3);
+    G.M = A.rows;
+    G.N = A.inner;
+    G.tiles_m = (int32_t)ceil_div(A.rows, kGgBM);
+    G.tiles_n = (int32_t)ceil_div(A.inner, nb);
+    G.kblocks = (int32_t)ceil_div(A.outer, kGgBK);
+    G.segs = 2;
+    G.splits = 1;
+    G.kb_per = 2 * G.kblocks;
+    G.out[0] = R.dx;
+    G.out_ld = R.dx_ld;
+    G.vec = aligned16(R.dx) && R.dx_ld % V == 0;
+    CUtensorMap a0, a1;
+    GPB_TRY(make_map(dg, kGgBM, &a0));
+    GPB_TRY(make_map(du, kGgBM, &a1));
+    GPB_TRY((gated_plain<GG_DX, T, D, PL>(a0, a1, wg, wu, nb, G, st)));
   }
-  if (G.dbg || G.dbu) {
-    gated_bias_kernel<T><<<dim3((unsigned)ceil_div(A.outer, 32), 2, P.ranges_b), 256, 0, st>>>(
-        (const T*)A.dg, (const T*)A.du, A.rows, A.outer, partial);
+  if (R.dwg || R.dwu) {
+    GgArgs G{};
+    const bool joined = A.outer <= 64;
+    G.M = A.outer;
+    G.N = A.inner;
+    G.half_tiles = joined ? 0 : (int32_t)ceil_div(A.outer, kGgBM);
+    G.tiles_m = joined ? 1 : 2 * G.half_tiles;
+    G.tiles_n = (int32_t)ceil_div(A.inner, P.tile_n);
+    G.kblocks = (int32_t)ceil_div(A.rows, kGgBK);
+    G.segs = 1;
+    G.splits = P.splits;
+    G.kb_per = P.kb_per;
+    G.out[0] = R.dwg;
+    G.out[1] = R.dwu;
+    G.out_ld = R.dw_ld;
+    G.partial = partial;
+    G.vec = aligned16(R.dwg) && aligned16(R.dwu) && R.dw_ld % V == 0;
+    CUtensorMap a0, a1;
+    GPB_TRY(make_map(dg, kGgBK, &a0));
+    GPB_TRY(make_map(du, kGgBK, &a1));
+    GPB_TRY((gated_plain<GG_DW, T, D, PL>(a0, a1, x, x, P.tile_n, G, st)));
+    if (P.splits > 1) {
+      mm_join_kernel<T><<<(unsigned)ceil_div(2 * A.outer * A.inner, 256), 256, 0, st>>>(
+          partial, P.splits, A.outer, A.inner, 2, (T*)R.dwg, (T*)R.dwu, R.dw_ld);
+      GPB_CHECK_CUDA(cudaGetLastError());
+    }
+  }
+  if (R.dbg || R.dbu) {
+    gated_bias_kernel<D><<<dim3((unsigned)ceil_div(A.outer, 32), 2, P.ranges_b), 256, 0, st>>>(
+        (const D*)dg.p, (const D*)du.p, A.rows, A.outer, P.ldn, PL, P.plane_d, partial);
     GPB_CHECK_CUDA(cudaGetLastError());
     gated_bias_join<T><<<(unsigned)ceil_div(2 * A.outer, 256), 256, 0, st>>>(
-        partial, P.ranges_b, A.outer, (T*)G.dbg, (T*)G.dbu);
+        partial, P.ranges_b, A.outer, (T*)R.dbg, (T*)R.dbu);
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   return GPB_OK;
@@ -351,6 +652,20 @@ static int gated_check(int32_t dtype, int64_t rows, int64_t inner, int64_t outer
 using namespace gpb;
 
 extern "C" {
+
+int gpb_feature_status(int32_t device, int32_t* status_out) {
+  clear_error();
+  GPB_REQUIRE(status_out, GPB_ERR_INVALID, "null output");
+  *status_out = DEV_OK;
+  GPB_DEVICE_SCOPE(device);
+  int word = 0;
+  const int zero = 0;
+  GPB_CHECK_CUDA(cudaDeviceSynchronize());
+  GPB_CHECK_CUDA(cudaMemcpyFromSymbol(&word, g_feature_err, sizeof(word)));
+  if (word != DEV_OK) GPB_CHECK_CUDA(cudaMemcpyToSymbol(g_feature_err, &zero, sizeof(zero)));
+  *status_out = word;
+  return GPB_OK;
+}
 
 int gpb_gated_unit_workspace(int32_t dtype, int64_t rows, int64_t inner, int64_t outer,
                              int32_t backward, int64_t* bytes_out) {
@@ -389,6 +704,14 @@ int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activati
   GPB_REQUIRE(P.total == 0 || (workspace_dev && workspace_bytes >= P.total), GPB_ERR_INVALID,
               "gated unit needs a workspace of %lld bytes, got %lld", (long long)P.total,
               (long long)(workspace_dev ? workspace_bytes : 0));
+  GPB_REQUIRE(aligned16(workspace_dev), GPB_ERR_INVALID, "workspace is not 16-byte aligned");
+  GPB_REQUIRE(!overlaps(workspace_dev, P.total, out_dev, ob) &&
+                  !overlaps(workspace_dev, P.total, x_dev, span_bytes(rows, inner, x_ld, es)) &&
+                  !overlaps(workspace_dev, P.total, w_gate_dev, wb) &&
+                  !overlaps(workspace_dev, P.total, w_up_dev, wb) &&
+                  !overlaps(workspace_dev, P.total, b_gate_dev, outer * es) &&
+                  !overlaps(workspace_dev, P.total, b_up_dev, outer * es),
+              GPB_ERR_INVALID, "the workspace overlaps an input or out");
   GPB_DEVICE_SCOPE(device);
   GatedArgs A{};
   A.x = x_dev;
@@ -406,9 +729,11 @@ int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activati
   A.act = activation;
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
-    case GPB_DTYPE_F32: return gated_forward<float>(A, st);
-    case GPB_DTYPE_F16: return gated_forward<__half>(A, st);
-    default: return gated_forward<__nv_bfloat16>(A, st);
+    case GPB_DTYPE_F32:
+      return gated_forward<float, __nv_bfloat16, 3>(A, (char*)workspace_dev, P, st);
+    case GPB_DTYPE_F16: return gated_forward<__half, __half, 1>(A, (char*)workspace_dev, P, st);
+    default:
+      return gated_forward<__nv_bfloat16, __nv_bfloat16, 1>(A, (char*)workspace_dev, P, st);
   }
 }
 
@@ -453,8 +778,7 @@ int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t
   GPB_REQUIRE(workspace_dev && workspace_bytes >= P.total, GPB_ERR_INVALID,
               "the backward pass needs a workspace of %lld bytes, got %lld", (long long)P.total,
               (long long)(workspace_dev ? workspace_bytes : 0));
-  GPB_REQUIRE(((uintptr_t)workspace_dev & 15u) == 0, GPB_ERR_INVALID,
-              "workspace is not 16-byte aligned");
+  GPB_REQUIRE(aligned16(workspace_dev), GPB_ERR_INVALID, "workspace is not 16-byte aligned");
   {
     // Outputs and the workspace are written while inputs are still read: none may share memory.
     const int64_t wb = span_bytes(outer, inner, w_ld, es), bb = outer * es;
@@ -491,9 +815,11 @@ int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t
   A.act = activation;
   GatedGrads G{dx_dev, dx_ld, dw_gate_dev, dw_up_dev, dw_ld, db_gate_dev, db_up_dev};
   switch (dtype) {
-    case GPB_DTYPE_F32: return gated_backward<float>(A, G, (char*)workspace_dev, P, st);
-    case GPB_DTYPE_F16: return gated_backward<__half>(A, G, (char*)workspace_dev, P, st);
-    default: return gated_backward<__nv_bfloat16>(A, G, (char*)workspace_dev, P, st);
+    case GPB_DTYPE_F32:
+      return gated_backward<float, __nv_bfloat16, 3>(A, G, (char*)workspace_dev, P, st);
+    case GPB_DTYPE_F16: return gated_backward<__half, __half, 1>(A, G, (char*)workspace_dev, P, st);
+    default:
+      return gated_backward<__nv_bfloat16, __nv_bfloat16, 1>(A, G, (char*)workspace_dev, P, st);
   }
 }
 

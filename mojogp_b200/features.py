@@ -117,6 +117,16 @@ def _workspace(a, need: int, like: "_View") -> tuple:
     return ptr, size
 
 
+def check_device(device: int = 0) -> None:
+    """Wait for `device` and raise if a bounded wait inside an operator's kernel
+    gave up since the last check (its outputs are then not valid)."""
+    word = C.c_int32()
+    _lib.call("gpb_feature_status", int(device), C.byref(word))
+    if word.value:
+        raise _lib.GPBError(_lib.ERR_DEVICE, f"device error word {word.value} "
+                            "(bounded wait gave up in a feature-map kernel)")
+
+
 # ------------------------------------------------------------- layer norm
 def layer_norm(out, x, weight=None, bias=None, *, eps: float = 1e-5, mean=None, rstd=None,
                stream=None) -> None:
