@@ -515,6 +515,26 @@ int gpb_dropout(int32_t device, void* stream, int32_t dtype, int64_t rows, int64
                 const void* residual_dev, int64_t residual_ld, double p, uint64_t seed,
                 uint64_t offset);
 
+/* out = x converted to out_dtype, rounded to nearest. */
+int gpb_cast(int32_t device, void* stream, int32_t out_dtype, int32_t x_dtype, int64_t rows,
+             int64_t cols, void* out_dev, int64_t out_ld, const void* x_dev, int64_t x_ld);
+
+/* Replace the provider's training inputs by x_dev [n][d] (float32, contiguous,
+ * on the provider's device): the kernel sees a feature map's new outputs
+ * without a new provider. Ordered after the work queued on `stream` (NULL =
+ * the legacy default stream) and complete on return; work of other streams
+ * that still reads the old inputs must be done. Prediction caches made before
+ * belong to the old inputs. */
+int gpb_set_inputs(gpb_provider* p, const float* x_dev, void* stream);
+/* gpb_bbmm on one GPU that also returns dNLL/dX at the provider's inputs
+ * (x_grad_dev [n][d], complete on return) and sum(alpha), whose negative over
+ * n is the gradient by a constant mean. The trace part uses the same probes as
+ * the parameters' gradients. */
+int gpb_bbmm_inputs(gpb_provider* p, const float* y_centered_host, int64_t n, int32_t num_probes,
+                    int32_t max_cg_iter, int32_t max_tridiag_iter, float cg_tol,
+                    int32_t precond_rank, int32_t iteration, double* nll_out, double* grads_out,
+                    double* sum_alpha_out, int32_t* cg_iters_out, float* x_grad_dev);
+
 /* out [n][d] = d/dX sum_c a_c' K(X, X) b_c at the provider's inputs and
  * parameters (no noise term), a and b column-major [ncols][n]: row i is
  * sum_j sum_c (a_ci b_cj + b_ci a_cj) dk(x_i, x_j)/dx_i. Beside

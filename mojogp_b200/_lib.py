@@ -102,6 +102,9 @@ SIGNATURES = {
                                 P, c_i64, P, P, P, c_i64, P, P, c_i64, P, P, P, c_i64],
     "gpb_dropout": [c_i32, P, c_i32, c_i64, c_i64, P, c_i64, P, c_i64, P, c_i64, c_f64, C.c_uint64,
                     C.c_uint64],
+    "gpb_cast": [c_i32, P, c_i32, c_i32, c_i64, c_i64, P, c_i64, P, c_i64],
+    "gpb_set_inputs": [P, P, P],
+    "gpb_bbmm_inputs": [P, P, c_i64, c_i32, c_i32, c_i32, c_f32, c_i32, c_i32, P, P, P, PI32, P],
     "gpb_input_gradient": [P, P, P, P, c_i64, P],
     "gpb_lmc_predict_exact_variance": [P, P, c_i64, c_i32, c_i32, c_f32, P, PI32],
 }

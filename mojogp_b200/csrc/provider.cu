@@ -597,6 +597,26 @@ int gpb_get_x_ptr(gpb_provider* p, const float** x_dev_out) {
   return GPB_OK;
 }
 
+int gpb_set_inputs(gpb_provider* p, const float* x_dev, void* stream) {
+  clear_error();
+  GPB_REQUIRE(p && x_dev, GPB_ERR_INVALID, "null argument");
+  GPB_REQUIRE(((uintptr_t)x_dev & 3u) == 0, GPB_ERR_INVALID,
+              "pointer is not aligned to its element type");
+  GPB_CHECK_CUDA(cudaSetDevice(p->device));
+  cudaEvent_t ready = nullptr;
+  GPB_CHECK_CUDA(cudaEventCreateWithFlags(&ready, cudaEventDisableTiming));
+  cudaError_t e = cudaEventRecord(ready, (cudaStream_t)stream);
+  if (e == cudaSuccess) e = cudaStreamWaitEvent(p->stream, ready, 0);
+  if (e == cudaSuccess)
+    e = cudaMemcpyAsync(p->X_d, x_dev, (size_t)p->n * p->d * sizeof(float),
+                        cudaMemcpyDeviceToDevice, p->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(p->stream);
+  cudaEventDestroy(ready);
+  GPB_REQUIRE(e == cudaSuccess, GPB_ERR_CUDA, "set inputs: %s", cudaGetErrorString(e));
+  p->xs_dirty = true;
+  return GPB_OK;
+}
+
 int gpb_forward_matvec_rows(gpb_provider* p, float* out_dev, const float* v_dev, int64_t ncols,
                             int64_t row_begin, int64_t row_end) {
   GPB_REQUIRE(p && out_dev && v_dev, GPB_ERR_INVALID, "null argument");

@@ -97,4 +97,8 @@ int provider_bilinear_rows_nd(gpb_provider* p, const float* a_dev, int64_t a_ld,
                               int64_t ncols, int64_t row_begin, int64_t row_end, int64_t ndata,
                               double* data_out, double* trace_out, cudaStream_t st);
 
+// out [n][d] = d/dX sum_c a_c' K b_c for a, b [ncols][n] (input_gradient.cu).
+int provider_input_gradient(gpb_provider* p, float* out, const float* a, const float* b,
+                            int64_t ncols, cudaStream_t st);
+
 }  // namespace gpb

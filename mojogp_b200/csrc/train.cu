@@ -651,6 +651,45 @@ int gpb_bbmm(gpb_provider* p, gpb_comm* comm, const float* y_centered_host, int6
   return provider_check_device_error(p);
 }
 
+int gpb_bbmm_inputs(gpb_provider* p, const float* y_centered_host, int64_t n, int32_t num_probes,
+                    int32_t max_cg_iter, int32_t max_tridiag_iter, float cg_tol,
+                    int32_t precond_rank, int32_t iteration, double* nll_out, double* grads_out,
+                    double* sum_alpha_out, int32_t* cg_iters_out, float* x_grad_dev) {
+  clear_error();
+  GPB_REQUIRE(p && y_centered_host && nll_out && grads_out && sum_alpha_out && x_grad_dev,
+              GPB_ERR_INVALID, "null argument");
+  GPB_REQUIRE(n == p->n && num_probes >= 1 && max_cg_iter >= 1 && max_tridiag_iter >= 0,
+              GPB_ERR_INVALID, "bad sizes");
+  GPB_CHECK_CUDA(cudaSetDevice(p->device));
+  Engine E;
+  GPB_TRY(engine_from_comm(p, nullptr, E));
+  const int t = 1 + num_probes;
+  BBMMState S;
+  GPB_TRY(S.ensure(E, t, max_tridiag_iter));
+  GPB_CHECK_CUDA(cudaMemcpyAsync(S.yc.ptr, y_centered_host, E.nl * sizeof(float),
+                                 cudaMemcpyHostToDevice, E.st));
+  Precond P;
+  GPB_TRY(precond_build(E, precond_rank, P));
+  BBMMResult R;
+  GPB_TRY(bbmm_step(E, precond_rank > 0 ? &P : nullptr, S, num_probes, max_cg_iter,
+                    max_tridiag_iter, cg_tol, iteration, false, R));
+  // The step left [alpha | u_c] in sol and [alpha | P^-1 z_c] in rf. Its gradients weigh the data
+  // column by -1/2 and the probes by 1 / (2 P), per sample; the left factors take these weights.
+  std::vector<float> weight(t, 0.5f / ((float)num_probes * (float)n));
+  weight[0] = -0.5f / (float)n;
+  float* weight_dev = S.scal.f();
+  GPB_CHECK_CUDA(cudaMemcpyAsync(weight_dev, weight.data(), t * sizeof(float),
+                                 cudaMemcpyHostToDevice, E.st));
+  GPB_TRY(k_scale_cols(S.sol.f(), E.nl, E.nl, t, weight_dev, 0, E.st));
+  GPB_TRY(provider_input_gradient(p, x_grad_dev, S.sol.f(), S.rf.f(), t, E.st));
+  GPB_CHECK_CUDA(cudaStreamSynchronize(E.st));
+  *nll_out = R.nll;
+  for (int q = 0; q <= p->dk.nparams; ++q) grads_out[q] = R.grads[q];
+  *sum_alpha_out = R.sum_alpha;
+  if (cg_iters_out) *cg_iters_out = R.cg_iters;
+  return provider_check_device_error(p);
+}
+
 int gpb_precond_pivots(gpb_provider* p, gpb_comm* comm, int32_t rank, int64_t* pivots_out,
                        float* values_out, int32_t* actual_rank_out) {
   clear_error();

@@ -8,12 +8,13 @@ reference's gp.py:1608-2047.
 from __future__ import annotations
 
 import ctypes as C
+import time
 from typing import Optional
 
 import numpy as np
 
 from . import _lib
-from .provider import Provider
+from .provider import DeviceBuffer, Provider
 
 
 class TrainOptions(C.Structure):
@@ -119,6 +120,129 @@ def train(provider: Provider, y: np.ndarray, *, max_iterations: int = 100,
     }
 
 
+def _softplus(x):
+    return np.logaddexp(0.0, x)
+
+
+def _inv_softplus(y):
+    y = np.asarray(y, np.float64)
+    return np.where(y > 20.0, y, np.log(np.expm1(np.minimum(np.maximum(y, 1e-30), 20.0))))
+
+
+class _Adam:
+    """Adam on a list of host arrays, in place (the moments and constants of `train`)."""
+
+    def __init__(self, arrays):
+        self.m = [np.zeros(a.shape) for a in arrays]
+        self.v = [np.zeros(a.shape) for a in arrays]
+        self.t = 0
+
+    def step(self, arrays, grads, lr: float) -> None:
+        self.t += 1
+        c1, c2 = 1.0 - 0.9 ** self.t, 1.0 - 0.999 ** self.t
+        for a, g, m, v in zip(arrays, grads, self.m, self.v):
+            g = np.clip(np.nan_to_num(np.asarray(g, np.float64), nan=0.0, posinf=0.0, neginf=0.0),
+                        -100.0, 100.0)
+            m += 0.1 * (g - m)
+            v += 0.001 * (g * g - v)
+            a -= (lr * (m / c1) / (np.sqrt(v / c2) + 1e-8)).astype(a.dtype)
+
+
+def train_features(provider: Provider, feature_map, X: np.ndarray, y: np.ndarray, *,
+                   max_iterations: int = 100, learning_rate: float = 0.01,
+                   feature_learning_rate: Optional[float] = None, num_probes: int = 10,
+                   max_cg_iter: int = 100, cg_tol: float = 1e-2, precond_rank: int = 100,
+                   max_tridiag_iter: int = 30, use_cosine_lr: bool = False, learn_noise: bool = True,
+                   init_mean: float = 0.0, enable_early_stopping: bool = False,
+                   early_stop_patience: int = 10, early_stop_tol: float = 1e-4,
+                   verbose: bool = False, trainable_mask: Optional[np.ndarray] = None) -> dict:
+    """`train` with a learned feature map under the kernel: every iteration maps
+    X to the provider's inputs, takes one BBMM step with the gradient by those
+    inputs, and follows it back through the map; kernel parameters, noise and
+    mean move as in `train`, the map's weights with `feature_learning_rate`
+    (default: learning_rate). The best iteration's state is restored and the
+    provider left at the map's outputs without dropout. The result's keys are
+    `train`'s; the preconditioner is rebuilt every iteration, since the inputs
+    move."""
+    y = np.ascontiguousarray(y, dtype=np.float32).ravel()
+    if y.shape[0] != provider.n:
+        raise ValueError(f"y has {y.shape[0]} rows, provider has {provider.n}")
+    n, P = provider.n, provider.num_params
+    flr = learning_rate if feature_learning_rate is None else float(feature_learning_rate)
+    mask = np.ones(P) if trainable_mask is None else np.asarray(trainable_mask, np.float64)
+    raw = _inv_softplus(np.append(provider.params.astype(np.float64), provider.get_noise()))
+    mean = np.array([float(init_mean)])
+    kernel_adam, map_adam = _Adam([raw, mean]), _Adam(feature_map.parameters)
+    data = feature_map.upload(X, provider.device)
+    x_grad = DeviceBuffer((n, provider.d), provider.device)
+    best = {"nll": np.inf, "raw": raw.copy(), "mean": float(mean[0]),
+            "map": feature_map.snapshot()}
+    history, times, cg_its = [], [], []
+    stop_best, stale, converged = np.inf, 0, False
+    for it in range(max_iterations):
+        t0 = time.perf_counter()
+        feats = feature_map.forward(data, training=True, step=it)
+        provider.set_inputs(feats)
+        # Untrained parameters (a polynomial's degree) keep their value bit for bit.
+        params = np.where(mask > 0, _softplus(raw[:P]), provider.params).astype(np.float32)
+        provider.update_params(params)
+        provider.update_noise(float(_softplus(raw[P])) if learn_noise else 0.0)
+        res = bbmm_inputs(provider, y - np.float32(mean[0]), x_grad, num_probes=num_probes,
+                          max_cg_iter=max_cg_iter, max_tridiag_iter=max_tridiag_iter,
+                          cg_tol=cg_tol, precond_rank=precond_rank, iteration=it)
+        nll = res["nll"]
+        history.append(nll)
+        cg_its.append(res["cg_iters"])
+        if nll < best["nll"]:
+            best = {"nll": nll, "raw": raw.copy(), "mean": float(mean[0]),
+                    "map": feature_map.snapshot()}
+        if np.isfinite(nll):
+            map_grads = feature_map.backward(x_grad)
+            slope = 1.0 / (1.0 + np.exp(-raw))
+            g = res["grads"] * slope
+            g[:P] *= mask
+            if not learn_noise:
+                g[P] = 0.0
+            scale = 1.0
+            if use_cosine_lr:
+                scale = 0.05 + 0.475 * (1.0 + np.cos(np.pi * it / max(max_iterations, 1)))
+            kernel_adam.step([raw, mean], [g, np.array([res["mean_grad"]])], learning_rate * scale)
+            np.clip(raw, -20.0, 20.0, out=raw)
+            map_adam.step(feature_map.parameters, map_grads, flr * scale)
+        else:  # back to the best state, with smaller steps
+            raw[:], mean[0] = best["raw"], best["mean"]
+            feature_map.restore(best["map"])
+            learning_rate, flr = 0.5 * learning_rate, 0.5 * flr
+        feature_map.parameters_changed()
+        times.append((time.perf_counter() - t0) * 1e3)
+        if verbose and (it % 10 == 0 or it == max_iterations - 1):
+            print(f"Iter {it} : NLL = {nll:g} , noise = {provider.get_noise():g} , "
+                  f"mean = {mean[0]:g}")
+        if enable_early_stopping:
+            if nll < stop_best - early_stop_tol:
+                stop_best, stale = nll, 0
+            else:
+                stale += 1
+                if stale >= early_stop_patience:
+                    converged = True
+                    break
+    feature_map.restore(best["map"])
+    params = np.where(mask > 0, _softplus(best["raw"][:P]), provider.params).astype(np.float32)
+    provider.update_params(params)
+    provider.update_noise(float(_softplus(best["raw"][P])) if learn_noise else 0.0)
+    provider.set_inputs(feature_map.forward(data))
+    feature_map.release()
+    return {
+        "final_nll": float(best["nll"]), "noise": provider.get_noise(), "mean": best["mean"],
+        "iterations": len(history), "converged": converged, "params": params,
+        "iter_times_ms": np.array(times), "nll_history": np.array(history, np.float32),
+        "cg_iterations_history": np.array(cg_its, np.int32), "cached_alpha": None,
+        "precond_build_count": len(history) if precond_rank > 0 else 0,
+        "precond_build_time_ms": 0.0, "precond_rank": int(precond_rank),
+        "tile_kernels": [],
+    }
+
+
 def train_binding(info, y, params, noise, max_iterations=100, learning_rate=0.01, num_probes=10,
                   max_cg_iter=100, cg_tol=1e-2, precond_rank=10, verbose=False,
                   use_cosine_lr=True, use_preconditioner=True, max_tridiag_iter=30,
@@ -190,6 +314,28 @@ def bbmm(provider: Provider, y_centered: np.ndarray, *, num_probes: int = 10,
               provider.n, num_probes, max_cg_iter, max_tridiag_iter, float(cg_tol), precond_rank,
               iteration, C.byref(nll), _p(grads), C.byref(ld), C.byref(iq), C.byref(it))
     return {"nll": nll.value, "grads": grads, "logdet": ld.value, "inv_quad": iq.value,
+            "cg_iters": it.value}
+
+
+def bbmm_inputs(provider: Provider, y_centered: np.ndarray, x_grad: DeviceBuffer, *,
+                num_probes: int = 10, max_cg_iter: int = 100, max_tridiag_iter: int = 30,
+                cg_tol: float = 1e-2, precond_rank: int = 0, iteration: int = 0) -> dict:
+    """`bbmm` that also writes the NLL's gradient by the provider's inputs to
+    the device buffer x_grad [n, d] and returns the gradient by a constant mean."""
+    y = np.ascontiguousarray(y_centered, dtype=np.float32).ravel()
+    if y.shape[0] != provider.n:
+        raise ValueError(f"y has {y.shape[0]} rows, provider has {provider.n}")
+    if tuple(x_grad.shape) != (provider.n, provider.d) or x_grad.dtype != np.float32:
+        raise ValueError(f"x_grad must be float32 [{provider.n}, {provider.d}]")
+    if x_grad.device != provider.device:
+        raise ValueError(f"x_grad must be on device {provider.device}")
+    nll, sum_alpha = C.c_double(), C.c_double()
+    grads = np.zeros(provider.num_params + 1, np.float64)
+    it = C.c_int32()
+    _lib.call("gpb_bbmm_inputs", provider.h, _p(y), provider.n, num_probes, max_cg_iter,
+              max_tridiag_iter, float(cg_tol), precond_rank, iteration, C.byref(nll), _p(grads),
+              C.byref(sum_alpha), C.byref(it), x_grad.cptr)
+    return {"nll": nll.value, "grads": grads, "mean_grad": -sum_alpha.value / provider.n,
             "cg_iters": it.value}
 
 

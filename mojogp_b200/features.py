@@ -279,3 +279,15 @@ def dropout_backward(dx, dout, p: float, seed: int, *, offset: int = 0, stream=N
     """dx = keep ? dout / (1 - p) : 0 with the mask of dropout(p, seed, offset);
     the residual's gradient is dout itself. dx may be dout."""
     dropout(dx, dout, p, seed, offset=offset, stream=stream)
+
+
+def cast(out, x, *, stream=None) -> None:
+    """out = x in out's element type, rounded to nearest ([rows, columns])."""
+    xv = _View(x, "x", 2)
+    ov = _View(out, "out", 2)
+    if ov.shape != xv.shape:
+        raise ValueError(f"out must have shape {xv.shape}, got {ov.shape}")
+    if ov.device != xv.device:
+        raise ValueError(f"out is on device {ov.device}, expected {xv.device}")
+    _lib.call("gpb_cast", xv.device, stream, ov.code, xv.code, *xv.shape, ov.ptr, ov.ld, xv.ptr,
+              xv.ld)

@@ -24,6 +24,7 @@ from typing import Optional
 import numpy as np
 
 from . import engine, prediction
+from .feature_map import FeatureMap
 from .kernel import KernelNode, KernelType, make_ard_kernel
 from .provider import Provider
 
@@ -221,11 +222,18 @@ class SingleOutputGP:
     }
 
     def __init__(self, kernel: KernelNode, *, init_mean: Optional[float] = None,
-                 verbose: bool = False, device: int = 0):
+                 verbose: bool = False, device: int = 0,
+                 feature_map: Optional[FeatureMap] = None):
+        """`feature_map` puts a learned map under the kernel (no reference
+        counterpart): the kernel sees its outputs, and fit() trains it with the
+        kernel's parameters on one GPU (a second fit continues from its weights)."""
         if not isinstance(kernel, KernelNode):
             raise TypeError(
                 f"kernel must be a KernelNode instance (e.g. RBF(), Matern52()), got "
                 f"{type(kernel).__name__}")
+        if feature_map is not None and not isinstance(feature_map, FeatureMap):
+            raise TypeError(f"feature_map must be a FeatureMap, got {type(feature_map).__name__}")
+        self.feature_map = feature_map
         self.kernel_spec = kernel
         self.kernel: Optional[KernelNode] = None
         self.ard = kernel.has_ard()
@@ -277,8 +285,10 @@ class SingleOutputGP:
             lr_schedule: str = "constant", prepare_prediction_cache: bool = False,
             prediction_cache_rank: Optional[int] = None,
             observation_noise: Optional[np.ndarray] = None, learn_noise: bool = True,
-            comm=None) -> TrainingResult:
-        """Train hyperparameters by BBMM (mBCG + SLQ) with Adam on the GPU."""
+            comm=None, feature_learning_rate: Optional[float] = None) -> TrainingResult:
+        """Train hyperparameters by BBMM (mBCG + SLQ) with Adam on the GPU, and
+        the feature map's weights with them (`feature_learning_rate`, default
+        learning_rate) where the model has one."""
         X = np.ascontiguousarray(X, dtype=np.float32)
         y = np.ascontiguousarray(y, dtype=np.float32)
         # Data, then optimiser checks, with the reference's messages (gp.py:995-1004, 1266-1284).
@@ -308,8 +318,19 @@ class SingleOutputGP:
         # than streaming a stored K from HBM at t = 16 (fn_ptr_module.py:363-421).
         if lr_schedule not in ("constant", "cosine"):
             raise ValueError(f"lr_schedule must be 'cosine' or 'constant', got '{lr_schedule}'")
+        fm = self.feature_map
+        if feature_learning_rate is not None:
+            if fm is None:
+                raise ValueError("feature_learning_rate needs a feature_map")
+            if feature_learning_rate <= 0:
+                raise ValueError(f"feature_learning_rate must be > 0, got {feature_learning_rate}")
+        if fm is not None and comm is not None:
+            raise NotImplementedError("a feature map trains on one GPU: comm must be None")
+        if fm is not None:
+            fm.build(X.shape[1])
         n, dim = X.shape
         self.dim = dim
+        dim = dim if fm is None else fm.output_dim
         self._comm = comm
         self.kernel = self._resolved_kernel(dim)
         P = self.kernel.num_params()
@@ -342,20 +363,25 @@ class SingleOutputGP:
         self._destroy()
         self._X_train, self._y_train = X, y
         self._obs_noise = None if observation_noise is None else np.asarray(observation_noise, np.float32)
-        self._provider = Provider(X, self.kernel, params, initial_noise, device=self.device,
-                                  noise_vector=self._obs_noise)
-        res = engine.train(
-            self._provider, y, max_iterations=max_iterations, learning_rate=learning_rate,
+        self._provider = Provider(self._kernel_inputs(X), self.kernel, params, initial_noise,
+                                  device=self.device, noise_vector=self._obs_noise)
+        options = dict(
+            max_iterations=max_iterations, learning_rate=learning_rate,
             num_probes=cg["num_probes"], max_cg_iter=cg["max_cg_iter"], cg_tol=cg["cg_tol"],
             precond_rank=cg["precond_rank"] if use_p else 0,
-            max_tridiag_iter=cg["max_tridiag_iter"],
-            precond_rebuild_threshold=cg["precond_rebuild_threshold"],
-            use_cosine_lr=lr_schedule == "cosine", use_preconditioner=use_p,
+            max_tridiag_iter=cg["max_tridiag_iter"], use_cosine_lr=lr_schedule == "cosine",
             learn_noise=learn_noise, init_mean=init_mean,
             enable_early_stopping=enable_early_stopping, early_stop_patience=early_stop_patience,
             early_stop_tol=early_stop_tol,
             verbose=self.verbose if verbose is None else verbose,
-            trainable_mask=self.kernel.engine_trainable_mask(), comm=comm)
+            trainable_mask=self.kernel.engine_trainable_mask())
+        if fm is None:
+            res = engine.train(self._provider, y,
+                               precond_rebuild_threshold=cg["precond_rebuild_threshold"],
+                               use_preconditioner=use_p, comm=comm, **options)
+        else:
+            res = engine.train_features(self._provider, fm, X, y,
+                                        feature_learning_rate=feature_learning_rate, **options)
         self._train_info = {"max_cg_iterations": cg["max_cg_iter"], "cg_tolerance": cg["cg_tol"],
                             "max_tridiag_iter": cg["max_tridiag_iter"],
                             "precond_rank": res["precond_rank"],
@@ -371,6 +397,10 @@ class SingleOutputGP:
         if prepare_prediction_cache:
             self.prepare_prediction_cache(max_root_decomposition_size=prediction_cache_rank)
         return self._training_result
+
+    def _kernel_inputs(self, X: np.ndarray) -> np.ndarray:
+        """What the kernel sees of input rows: the feature map's outputs, or the rows."""
+        return X if self.feature_map is None else self.feature_map.transform(X, self.device)
 
     # ---------------------------------------------------------------- predict
     def _solver_config(self, max_cg_iterations=None, cg_tolerance=None,
@@ -437,6 +467,7 @@ class SingleOutputGP:
         if Xt.ndim == 1 and self.dim == 1:
             Xt = Xt[:, None]
         _check_test_inputs(Xt, self.dim)
+        Xt = self._kernel_inputs(Xt)
         want_var = variance_method == "love"
         cache = self.prepare_prediction_cache("love" if want_var else "mean_only",
                                               max_root_decomposition_size, max_cg_iterations,
@@ -546,7 +577,9 @@ class SingleOutputGP:
         this continuous-kernel model; keys the reference's load() reads
         (gp.py:3735-3876) carry the same meaning here."""
         tr = self._training_result
+        extra = {} if self.feature_map is None else {"feature_map": self.feature_map.config()}
         return {
+            **extra,
             "schema_version": MODEL_SCHEMA_VERSION,
             "mojogp_version": f"mojogp_b200 {_package_version()}",
             "wrapper": "SingleOutputGP",
@@ -584,7 +617,8 @@ class SingleOutputGP:
         (gp.py:3648-3723): `{path}_config.json` and `{path}_arrays.npz` with
         X_train, y_train, params (and observation_noise_train). A cached LOVE
         root is stored as the extra array `lanczos_root`, which the
-        reference's load ignores. A trailing .json / .npz on `path` is
+        reference's load ignores; a feature map is stored as the extra key
+        `feature_map` and its weights, which only load() here reads. A trailing .json / .npz on `path` is
         dropped, as in the reference."""
         if not self._is_trained:
             raise RuntimeError("GP must be trained before saving.")
@@ -598,6 +632,9 @@ class SingleOutputGP:
             arrays["observation_noise_train"] = self._obs_noise
         if tr.lanczos_root is not None:
             arrays["lanczos_root"] = tr.lanczos_root
+        if self.feature_map is not None:
+            for i, p in enumerate(self.feature_map.parameters):
+                arrays[f"feature_map_{i}"] = p
         np.savez(f"{base}_arrays.npz", **arrays)
 
     @staticmethod
@@ -638,12 +675,17 @@ class SingleOutputGP:
         config, arrays = cls.read_artifact(path)
         if kernel is None:
             kernel = KernelNode.from_dict(config["kernel_tree"])
+        fm = None
+        if config.get("feature_map") is not None:
+            count = sum(k.startswith("feature_map_") for k in arrays)
+            fm = FeatureMap.from_config(config["feature_map"],
+                                        [arrays[f"feature_map_{i}"] for i in range(count)])
         gp = cls(kernel, init_mean=config.get("init_mean"), verbose=config.get("verbose", False),
-                 device=device)
+                 device=device, feature_map=fm)
         X = np.ascontiguousarray(arrays["X_train"], dtype=np.float32)
         y = np.ascontiguousarray(arrays["y_train"], dtype=np.float32)
         gp.dim = X.shape[1]
-        gp.kernel = gp._resolved_kernel(gp.dim)
+        gp.kernel = gp._resolved_kernel(gp.dim if fm is None else fm.output_dim)
         gp._X_train, gp._y_train = X, y
         gp._obs_noise = (np.ascontiguousarray(arrays["observation_noise_train"], np.float32)
                          if "observation_noise_train" in arrays else None)
@@ -657,8 +699,8 @@ class SingleOutputGP:
             params=params, noise=config["noise"], mean=config.get("mean", 0.0),
             nll=config["nll"], iterations=config["iterations"], converged=config["converged"],
             lanczos_root=arrays.get("lanczos_root"), lanczos_rank=config["lanczos_rank"])
-        gp._provider = Provider(X, gp.kernel, params, float(config["noise"]), device=device,
-                                noise_vector=gp._obs_noise)
+        gp._provider = Provider(gp._kernel_inputs(X), gp.kernel, params, float(config["noise"]),
+                                device=device, noise_vector=gp._obs_noise)
         return gp
 
     def _destroy(self) -> None:
@@ -679,10 +721,10 @@ class SingleOutputGP:
 
 
 def fit_gp(X: np.ndarray, y: np.ndarray, kernel: Optional[KernelNode] = None,
-           **kwargs) -> SingleOutputGP:
+           feature_map: Optional[FeatureMap] = None, **kwargs) -> SingleOutputGP:
     """Create and fit a SingleOutputGP in one call (fit_gp, gp.py:3928-3949);
     the kernel defaults to RBF and the keyword arguments go to fit()."""
     from .kernel import Kernel
-    gp = SingleOutputGP(kernel if kernel is not None else Kernel.rbf())
+    gp = SingleOutputGP(kernel if kernel is not None else Kernel.rbf(), feature_map=feature_map)
     gp.fit(X, y, **kwargs)
     return gp

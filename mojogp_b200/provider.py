@@ -200,6 +200,16 @@ class Provider:
         _lib.call("gpb_gradient_bilinear", self.h, a.cptr, b.cptr, int(ncols), _ptr(data), _ptr(trace))
         return data, trace
 
+    def set_inputs(self, x: DeviceBuffer, stream: Optional[int] = None) -> None:
+        """Replace the training inputs by the rows of a float32 device buffer
+        [n, d] (a feature map's outputs), after the work queued on `stream`.
+        Prediction caches made before belong to the old inputs."""
+        if tuple(x.shape) != (self.n, self.d) or x.dtype != np.float32:
+            raise ValueError(f"x must be float32 [{self.n}, {self.d}], got {x.dtype} {tuple(x.shape)}")
+        if x.device != self.device:
+            raise ValueError(f"x must be on device {self.device}")
+        _lib.call("gpb_set_inputs", self.h, x.cptr, stream)
+
     def input_gradient(self, out, a, b, ncols: int, stream: Optional[int] = None) -> None:
         """out [n, d] = d/dX sum_c a_c' K(X, X) b_c for a and b [ncols][n]
         (float32): the gradient of gradient_bilinear's form by the inputs.

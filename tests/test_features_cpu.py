@@ -172,3 +172,52 @@ def test_workspace_sizes_follow_the_sizes_alone(gpb_lib):
     assert ft.gated_unit_workspace(100, 64, 64, "bfloat16", backward=True) >= 2 * 100 * 64 * 2
     # float32 operands are three 16-bit planes
     assert ft.gated_unit_workspace(100, 64, 64, "float32") >= 3 * 2 * (100 * 64 + 2 * 64 * 64)
+
+
+def test_feature_map_refusals_and_shapes():
+    from mojogp_b200 import FeatureMap, RBF, SingleOutputGP
+    for kw, match in [(dict(widths=[]), "widths"), (dict(widths=[0]), "widths"),
+                      (dict(widths=[65]), "at most 64"), (dict(widths=[4], activation="x"), "activation"),
+                      (dict(widths=[4], dropout=1.0), "dropout"), (dict(widths=[4], dtype="f64"), "dtype"),
+                      (dict(widths=[4], seed=-1), "seed")]:
+        refuse(match, FeatureMap, **kw)
+    fm = FeatureMap([100, 8])
+    refuse("at least one", fm.build, 0)
+    fm.build(30)
+    assert [p.shape for p in fm.parameters] == [(30,), (30,), (100, 30), (100, 30), (100,), (100,),
+                                               (100,), (100,), (8, 100), (8, 100), (8,), (8,)]
+    refuse("built for 30", fm.build, 31)
+    same = FeatureMap.from_config(fm.config(), fm.parameters)
+    assert all(np.array_equal(a, b) for a, b in zip(same.parameters, fm.parameters))
+    refuse("do not match", FeatureMap.from_config, fm.config(), fm.parameters[:-1])
+    with pytest.raises(TypeError, match="FeatureMap"):
+        SingleOutputGP(RBF(), feature_map="wide")
+    X, y = np.zeros((4, 30), np.float32), np.zeros(4, np.float32)
+    refuse("needs a feature_map", SingleOutputGP(RBF()).fit, X, y, feature_learning_rate=0.1)
+    refuse("feature_learning_rate", SingleOutputGP(RBF(), feature_map=fm).fit, X, y,
+           feature_learning_rate=0.0)
+    with pytest.raises(NotImplementedError, match="one GPU"):
+        SingleOutputGP(RBF(), feature_map=fm).fit(X, y, comm=object())
+    refuse("built for 30", SingleOutputGP(RBF(), feature_map=fm).fit, X[:, :20], y)
+    refuse("2D", fm.upload, np.zeros(30, np.float32))
+
+
+def test_bfloat16_rounding():
+    from mojogp_b200.feature_map import _to_bfloat16_bits
+    a = np.array([1.0, 1.00390625, 1.01171875, -3.4e38, np.inf, np.nan], np.float32)
+    bits = _to_bfloat16_bits(a)
+    assert list(bits[:3]) == [0x3F80, 0x3F80, 0x3F82]  # ties to even
+    assert bits[3] == 0xFF80 and bits[4] == 0x7F80 and (bits[5] & 0x7FFF) > 0x7F80
+
+
+def test_cast_and_provider_refusals(ft):
+    refuse("shape", ft.cast, arr((4, 7), 2, dtype="float16"), arr((4, 8)))
+    refuse("not one of", ft.cast, arr((4, 8), 2, dtype="int32"), arr((4, 8)))
+    refuse("on device 1", ft.cast, arr((4, 8), 2, dtype="float16", device=1), arr((4, 8)))
+    p, q = C.c_void_p(1 << 20), C.c_void_p(1 << 24)
+    lib = _lib.lib()
+    assert lib.gpb_cast(0, None, 5, 0, 1, 1, p, 1, q, 1) == _lib.ERR_INVALID
+    assert lib.gpb_set_inputs(None, p, None) == _lib.ERR_INVALID
+    z = C.c_double()
+    assert lib.gpb_bbmm_inputs(None, p, 1, 1, 1, 1, 0.1, 0, 0, C.byref(z), C.byref(z), C.byref(z),
+                               None, p) == _lib.ERR_INVALID
