@@ -157,7 +157,9 @@ def check(status: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args))
+    status = getattr(_lib or lib(), name)(*args)
+    if status:
+        check(status)
 
 
 def declared_symbols(header: Path) -> list[str]:

@@ -12,74 +12,85 @@
 
 namespace gpb {
 
-__device__ __forceinline__ uint4 philox(uint64_t block, uint64_t offset, uint64_t seed) {
-  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32);
-  uint32_t c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
-  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t p0 = (uint64_t)0xD2511F53u * c0;
-    const uint64_t p1 = (uint64_t)0xCD9E8D57u * c2;
-    const uint32_t n0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
-    const uint32_t n2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
-    c1 = (uint32_t)p1;
-    c3 = (uint32_t)p0;
-    c0 = n0;
-    c2 = n2;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-  return make_uint4(c0, c1, c2, c3);
-}
-
+// The ten round keys are the same for every thread: the host adds them up once, and each round is
+// two wide multiplies and two three-way xors with a constant-bank operand. The generator is what a
+// plain dropout's arithmetic consists of: 20 wide multiplies per four elements.
 struct DropoutArgs {
   const void* x;
   const void* res;
   void* out;
   int64_t x_ld, res_ld, out_ld;
   int64_t rows, cols, count;
-  uint64_t seed, offset;
+  uint64_t offset;
+  uint32_t key[20];
   uint32_t border;
   float scale;
 };
 
-// One thread per aligned run of VEC elements (VEC a multiple of 4: VEC / 4 generator blocks).
-// FLAT: every operand is contiguous, so the element index is the address; otherwise VEC divides
-// cols and the run stays inside one row.
-template <typename T, int VEC, bool FLAT>
-__global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutArgs A) {
-  const int64_t run = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t e = run * VEC;
-  if (e >= A.count) return;
-  int64_t xi = e, ri = e, oi = e;
-  if constexpr (!FLAT) {
-    const int64_t row = e / A.cols, col = e - row * A.cols;
-    xi = row * A.x_ld + col;
-    ri = row * A.res_ld + col;
-    oi = row * A.out_ld + col;
+__device__ __forceinline__ uint4 philox(uint64_t block, const DropoutArgs& A) {
+  uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32);
+  uint32_t c2 = (uint32_t)A.offset, c3 = (uint32_t)(A.offset >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c0;
+    const uint64_t p1 = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ A.key[2 * r];
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ A.key[2 * r + 1];
+    c1 = (uint32_t)p1;
+    c3 = (uint32_t)p0;
   }
-  float v[VEC], r[VEC];
-  load_vec<T, VEC>((const T*)A.x + xi, v);
-  if (A.res) load_vec<T, VEC>((const T*)A.res + ri, r);
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// RUNS aligned runs of VEC elements per thread, a block's width apart (VEC a multiple of 4: VEC / 4
+// generator blocks each); all their loads are issued before the first generator round. FLAT: every
+// operand is contiguous, so the element index is the address; otherwise VEC divides cols and a run
+// stays inside one row.
+template <typename T, int VEC, int RUNS, bool FLAT>
+__global__ void __launch_bounds__(256) dropout_vec_kernel(const __grid_constant__ DropoutArgs A) {
+  const int64_t run0 = (int64_t)blockIdx.x * (256 * RUNS) + threadIdx.x;
+  Pack<T, VEC> x[RUNS], res[RUNS];
+  int64_t oi[RUNS];
 #pragma unroll
-  for (int b = 0; b < VEC / 4; ++b) {
-    const uint4 w = philox((uint64_t)(e / 4 + b), A.offset, A.seed);
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float kept = ws[q] >= A.border ? v[4 * b + q] * A.scale : 0.f;
-      v[4 * b + q] = A.res ? kept + r[4 * b + q] : kept;
+  for (int u = 0; u < RUNS; ++u) {
+    const int64_t e = (run0 + u * 256) * VEC;
+    if (e >= A.count) break;
+    int64_t xi = e, ri = e;
+    oi[u] = e;
+    if constexpr (!FLAT) {
+      const int64_t row = e / A.cols, col = e - row * A.cols;
+      xi = row * A.x_ld + col;
+      ri = row * A.res_ld + col;
+      oi[u] = row * A.out_ld + col;
     }
+    x[u] = *reinterpret_cast<const Pack<T, VEC>*>((const T*)A.x + xi);
+    if (A.res) res[u] = *reinterpret_cast<const Pack<T, VEC>*>((const T*)A.res + ri);
   }
-  store_vec<T, VEC>((T*)A.out + oi, v);
+#pragma unroll
+  for (int u = 0; u < RUNS; ++u) {
+    const int64_t e = (run0 + u * 256) * VEC;
+    if (e >= A.count) break;
+    float v[VEC];
+#pragma unroll
+    for (int b = 0; b < VEC / 4; ++b) {
+      const uint4 w = philox((uint64_t)(e / 4 + b), A);
+      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float kept = ws[q] >= A.border ? to_f(x[u].v[4 * b + q]) * A.scale : 0.f;
+        v[4 * b + q] = A.res ? kept + to_f(res[u].v[4 * b + q]) : kept;
+      }
+    }
+    store_vec<T, VEC>((T*)A.out + oi[u], v);
+  }
 }
 
 // Any strides, widths and alignments: one thread per generator block, element by element.
 template <typename T>
-__global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs A) {
+__global__ void __launch_bounds__(256) dropout_any_kernel(const __grid_constant__ DropoutArgs A) {
   const int64_t block = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (block * 4 >= A.count) return;
-  const uint4 w = philox((uint64_t)block, A.offset, A.seed);
+  const uint4 w = philox((uint64_t)block, A);
   const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -100,12 +111,19 @@ static int dropout_launch(const DropoutArgs& A, cudaStream_t st) {
   const bool ptrs = aligned16(A.x) && aligned16(A.out) && (!A.res || aligned16(A.res));
   const bool rows_ok = A.cols % VEC == 0 && A.x_ld % VEC == 0 && A.out_ld % VEC == 0 &&
                        (!A.res || A.res_ld % VEC == 0);
+  // Two runs per thread once that still gives every SM its threads.
+  const bool two = A.count / VEC >= (int64_t)kFeatSMs * 4096;
+  const unsigned g1 = (unsigned)ceil_div(A.count / VEC, 256), g2 = (unsigned)ceil_div(A.count / VEC, 512);
   if (ptrs && flat && A.count % VEC == 0) {
-    dropout_vec_kernel<T, VEC, true>
-        <<<(unsigned)ceil_div(A.count / VEC, 256), 256, 0, st>>>(A);
+    if (two)
+      dropout_vec_kernel<T, VEC, 2, true><<<g2, 256, 0, st>>>(A);
+    else
+      dropout_vec_kernel<T, VEC, 1, true><<<g1, 256, 0, st>>>(A);
   } else if (ptrs && rows_ok) {
-    dropout_vec_kernel<T, VEC, false>
-        <<<(unsigned)ceil_div(A.count / VEC, 256), 256, 0, st>>>(A);
+    if (two)
+      dropout_vec_kernel<T, VEC, 2, false><<<g2, 256, 0, st>>>(A);
+    else
+      dropout_vec_kernel<T, VEC, 1, false><<<g1, 256, 0, st>>>(A);
   } else {
     dropout_any_kernel<T><<<(unsigned)ceil_div(ceil_div(A.count, 4), 256), 256, 0, st>>>(A);
   }
@@ -153,8 +171,11 @@ extern "C" int gpb_dropout(int32_t device, void* stream, int32_t dtype, int64_t 
   A.rows = rows;
   A.cols = cols;
   A.count = rows * cols;
-  A.seed = seed;
   A.offset = offset;
+  for (int r = 0; r < 10; ++r) {
+    A.key[2 * r] = (uint32_t)seed + (uint32_t)r * 0x9E3779B9u;
+    A.key[2 * r + 1] = (uint32_t)(seed >> 32) + (uint32_t)r * 0xBB67AE85u;
+  }
   A.border = (uint32_t)std::floor(p * 4294967296.0);
   A.scale = (float)(1.0 / (1.0 - p));
   cudaStream_t st = (cudaStream_t)stream;

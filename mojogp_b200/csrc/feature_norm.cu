@@ -30,25 +30,107 @@ struct NormArgs {
   float eps;
 };
 
-// Sums (a, b) over the TPR threads of a row; every thread of the block takes part. `flip` alternates
-// the shared buffer so that one barrier per call is enough.
-__device__ __forceinline__ void row_sum2(float& a, float& b, int tpr, int flip) {
+// Sums each of N values over the TPR threads of a row; every thread of the block takes part. `flip`
+// alternates the shared buffer so that one barrier per call is enough.
+template <int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int tpr, int flip) {
   const int width = tpr < 32 ? tpr : 32;
-  for (int o = width >> 1; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
+  for (int o = width >> 1; o > 0; o >>= 1)
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
   if (tpr > 32) {
-    __shared__ float2 part[2][32];
-    const int warp = threadIdx.x >> 5, warps = tpr >> 5;
+    __shared__ float part[2][N][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = tpr >> 5;
     const int first = warp & ~(warps - 1);  // first warp of this row
-    if ((threadIdx.x & 31) == 0) part[flip][warp] = make_float2(a, b);
+    if (lane == 0)
+#pragma unroll
+      for (int q = 0; q < N; ++q) part[flip][q][warp] = v[q];
     __syncthreads();
-    a = b = 0.f;
-    for (int w = 0; w < warps; ++w) {
-      const float2 p = part[flip][first + w];
-      a += p.x;
-      b += p.y;
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] = part[flip][q][first + (lane & (warps - 1))];
+    for (int o = warps >> 1; o > 0; o >>= 1)
+#pragma unroll
+      for (int q = 0; q < N; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
+  }
+}
+
+// 1 / sqrt(v), v >= 0: the hardware's estimate and one Newton step (about 1 ulp; a division and a
+// square root cost 30 instructions a row).
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const float r = rsqrtf(v);
+  return v > 0.f ? fmaf(fmaf(-0.5f * v * r, r, 0.5f), r, r) : r;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Rows of at most 32 vectors: TPR threads (part of a warp) hold one vector each of RPT rows, so that
+// RPT loads are in flight where one row's would leave HBM idle.
+template <typename T, typename W, int VEC, int RPT>
+__global__ void __launch_bounds__(128) norm_forward_rows_kernel(const NormArgs A) {
+  const int tpr = A.tpr;
+  const int lane = threadIdx.x & (tpr - 1);
+  const int group = threadIdx.x / tpr, groups = 128 / tpr;
+  const int64_t row0 = (int64_t)blockIdx.x * (groups * RPT) + group;
+  const int c = lane * VEC;
+  const bool in = c < A.cols;
+  float v[RPT][VEC], w[VEC], b[VEC];
+#pragma unroll
+  for (int u = 0; u < RPT; ++u) {
+    const int64_t row = row0 + u * groups;
+    if (in && row < A.rows) {
+      load_vec<T, VEC>((const T*)A.x + row * A.x_ld + c, v[u]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[u][i] = 0.f;
+    }
+  }
+  if (in && A.w) load_vec<W, VEC>((const W*)A.w + c, w);
+  if (in && A.b) load_vec<W, VEC>((const W*)A.b + c, b);
+  const float inv = 1.f / (float)A.cols;
+  float s[RPT], q[RPT];
+#pragma unroll
+  for (int u = 0; u < RPT; ++u) {
+    s[u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s[u] += v[u][i];
+  }
+  row_sum(s, tpr, 0);
+#pragma unroll
+  for (int u = 0; u < RPT; ++u) {
+    s[u] *= inv;
+    q[u] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      v[u][i] -= s[u];
+      q[u] = in ? fmaf(v[u][i], v[u][i], q[u]) : 0.f;
+    }
+  }
+  row_sum(q, tpr, 0);
+#pragma unroll
+  for (int u = 0; u < RPT; ++u) {
+    const int64_t row = row0 + u * groups;
+    if (row >= A.rows) break;
+    const float rstd = inv_sqrt(fmaf(q[u], inv, A.eps));
+    if (lane == 0) {
+      if (A.mean) A.mean[row] = s[u];
+      if (A.rstd) A.rstd[row] = rstd;
+    }
+    if (in) {
+      float o[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        o[i] = v[u][i] * rstd;
+        if (A.w) o[i] *= w[i];
+        if (A.b) o[i] += b[i];
+      }
+      store_vec<T, VEC>((T*)A.out + row * A.out_ld + c, o);
     }
   }
 }
@@ -61,7 +143,7 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs A) {
   const bool live = row < A.rows;
   const T* x = (const T*)A.x + (live ? row : 0) * A.x_ld;
   float v[R][VEC];
-  float s = 0.f, unused = 0.f;
+  float s[1] = {0.f}, q[1] = {0.f};
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int c = (r * tpr + lane) * VEC;
@@ -72,22 +154,21 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs A) {
       for (int i = 0; i < VEC; ++i) v[r][i] = 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) s += v[r][i];
+    for (int i = 0; i < VEC; ++i) s[0] += v[r][i];
   }
-  row_sum2(s, unused, tpr, 0);
-  const float mean = s / (float)A.cols;
-  float q = 0.f;
+  row_sum(s, tpr, 0);
+  const float mean = s[0] / (float)A.cols;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const bool in = (r * tpr + lane) * VEC < A.cols;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       v[r][i] -= mean;
-      q = in ? fmaf(v[r][i], v[r][i], q) : q;
+      q[0] = in ? fmaf(v[r][i], v[r][i], q[0]) : q[0];
     }
   }
-  row_sum2(q, unused, tpr, 1);
-  const float rstd = 1.f / sqrtf(q / (float)A.cols + A.eps);
+  row_sum(q, tpr, 1);
+  const float rstd = inv_sqrt(q[0] / (float)A.cols + A.eps);
   if (!live) return;
   if (lane == 0) {
     if (A.mean) A.mean[row] = mean;
@@ -116,17 +197,16 @@ template <typename T, typename W>
 __global__ void __launch_bounds__(1024) norm_forward_wide_kernel(const NormArgs A) {
   const int64_t row = blockIdx.x;
   const T* x = (const T*)A.x + row * A.x_ld;
-  float s = 0.f, unused = 0.f;
-  for (int c = threadIdx.x; c < A.cols; c += blockDim.x) s += to_f(x[c]);
-  row_sum2(s, unused, blockDim.x, 0);
-  const float mean = s / (float)A.cols;
-  float q = 0.f;
+  float s[1] = {0.f}, q[1] = {0.f};
+  for (int c = threadIdx.x; c < A.cols; c += blockDim.x) s[0] += to_f(x[c]);
+  row_sum(s, blockDim.x, 0);
+  const float mean = s[0] / (float)A.cols;
   for (int c = threadIdx.x; c < A.cols; c += blockDim.x) {
     const float d = to_f(x[c]) - mean;
-    q = fmaf(d, d, q);
+    q[0] = fmaf(d, d, q[0]);
   }
-  row_sum2(q, unused, blockDim.x, 1);
-  const float rstd = 1.f / sqrtf(q / (float)A.cols + A.eps);
+  row_sum(q, blockDim.x, 1);
+  const float rstd = inv_sqrt(q[0] / (float)A.cols + A.eps);
   if (threadIdx.x == 0) {
     if (A.mean) A.mean[row] = mean;
     if (A.rstd) A.rstd[row] = rstd;
@@ -140,19 +220,208 @@ __global__ void __launch_bounds__(1024) norm_forward_wide_kernel(const NormArgs 
   }
 }
 
-// Backward with the weight gradients: a fixed number of blocks walks the rows, each thread adding
-// the dw and db of its columns; the block's sums go to A.partial.
-template <typename T, typename W, int VEC, int R, bool PARAMS>
-__global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs A) {
-  extern __shared__ float row_sums[];  // [slots][2][cols] when the block holds several rows
+// A block's dw and db sums, from every thread's own columns.
+template <int VEC, int R>
+__device__ __forceinline__ void norm_store_partial(const NormArgs& A, float* row_sums,
+                                                   float (&dw)[R][VEC], float (&db)[R][VEC]) {
   const int tpr = A.tpr;
   const int lane = threadIdx.x & (tpr - 1);
   const int groups = blockDim.x / tpr;
-  float dw[R][VEC], db[R][VEC];
+  float* part = A.partial + (int64_t)blockIdx.x * 2 * A.cols;
+  if (groups == 1) {
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      const int c = (r * tpr + lane) * VEC;
+      if (c < A.cols) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) dw[r][i] = db[r][i] = 0.f;
+        for (int i = 0; i < VEC; ++i) {
+          part[c + i] = dw[r][i];
+          part[A.cols + c + i] = db[r][i];
+        }
+      }
+    }
+    return;
+  }
+  // Several rows at a time: add the rows of each warp, then over the slots (a warp, or the warps of
+  // one row).
+  const int slots = tpr < 32 ? blockDim.x >> 5 : groups;
+  float* mine = row_sums + (int64_t)(threadIdx.x / (tpr < 32 ? 32 : tpr)) * 2 * A.cols;
+  __syncthreads();  // the memory may have been a ring
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int c = (r * tpr + lane) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      for (int o = tpr; o < 32; o <<= 1) {
+        dw[r][i] += __shfl_xor_sync(0xffffffffu, dw[r][i], o);
+        db[r][i] += __shfl_xor_sync(0xffffffffu, db[r][i], o);
+      }
+      if ((threadIdx.x & 31) < tpr && c < A.cols) {  // always true for whole warps
+        mine[c + i] = dw[r][i];
+        mine[A.cols + c + i] = db[r][i];
+      }
+    }
+  }
+  __syncthreads();
+  for (int q = threadIdx.x; q < 2 * A.cols; q += blockDim.x) {
+    float s = 0.f;
+    for (int w = 0; w < slots; ++w) s += row_sums[(int64_t)w * 2 * A.cols + q];
+    part[q] = s;
+  }
+}
+
+// Backward with the weight gradients: a fixed number of blocks walks the rows, each thread adding
+// the dw and db of its columns; the block's sums go to A.partial. Vector rows: 16-byte cp.async
+// copies fill a ring that only their own thread reads (no barrier), and the arithmetic is on fp32
+// pairs (FFMA2). Measured at 16384 x 4096 bf16 (403 MB): one column vector per thread on scalar FMAs
+// 125 us, issue-bound at 48 instructions an element; two vectors on pairs, which spread a row's
+// address, reduction and barrier work over twice the columns, 80 us (5.0 TB/s). What is left is the
+// chain of a row's reduction at two blocks per SM (121 registers); a deeper ring changes nothing.
+// Rows in flight per thread: what two resident blocks' rings have room for.
+template <int R>
+constexpr int kNormAhead = R >= 4 ? 2 : 4;
+
+template <typename T, typename W, int VEC, int R, bool PARAMS>
+__global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs A) {
+  constexpr int SLOTS = kNormAhead<R> + 1;
+  constexpr int P = VEC / 2;
+  extern __shared__ __align__(16) float row_sums[];  // the ring, then [slots][2][cols]
+  const int tpr = A.tpr;
+  const int lane = threadIdx.x & (tpr - 1);
+  const int groups = blockDim.x / tpr;
+  const int64_t step = (int64_t)gridDim.x * groups;
+  const int64_t base = (int64_t)blockIdx.x * groups;
+  const int64_t first = base + threadIdx.x / tpr;
+  const int loops = (int)((A.rows - base + step - 1) / step);  // of the block
+  const int mine = first < A.rows ? (int)((A.rows - first + step - 1) / step) : 0;
+  const int c0 = lane * VEC, dc = tpr * VEC;
+  const T* xf = (const T*)A.x + first * A.x_ld + c0;  // next row to fetch
+  const T* df = (const T*)A.dy + first * A.dy_ld + c0;
+  T* out = (T*)A.out + first * A.out_ld + c0;
+  const float* mp = A.mean + first;
+  const float* rp = A.rstd + first;
+  const int64_t x_step = step * A.x_ld, dy_step = step * A.dy_ld, out_step = step * A.out_ld;
+  const uint32_t stride = blockDim.x * 16, span = R * 2 * stride;
+  const uint32_t ring = smem_addr(row_sums) + threadIdx.x * 16;
+  const char* ring_p = reinterpret_cast<const char*>(row_sums) + threadIdx.x * 16;
+  bool in[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) in[r] = c0 + r * dc < A.cols;
+  int fetched = 0;
+  uint32_t fill = 0;  // byte offset of the slot to fill
+  auto fetch = [&]() {
+    if (fetched < mine) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (in[r]) {
+          copy16(ring + fill + (2 * r) * stride, xf + r * dc);
+          copy16(ring + fill + (2 * r + 1) * stride, df + r * dc);
+        }
+      xf += x_step;
+      df += dy_step;
+    }
+    copy_commit();
+    ++fetched;
+    fill = fill + span == SLOTS * span ? 0 : fill + span;
+  };
+  float2 w[R][P], dw[R][P], db[R][P];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float t[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t[i] = 1.f;
+    if (A.w && in[r]) load_vec<W, VEC>((const W*)A.w + c0 + r * dc, t);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      w[r][i] = make_float2(t[2 * i], t[2 * i + 1]);
+      dw[r][i] = db[r][i] = make_float2(0.f, 0.f);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < kNormAhead<R>; ++s) fetch();
+  const float inv = 1.f / (float)A.cols;
+  uint32_t at = 0;
+  float mean = 0 < mine ? *mp : 0.f, rstd = 0 < mine ? *rp : 0.f;
+  for (int k = 0; k < loops; ++k) {
+    copy_wait<kNormAhead<R> - 1>();
+    fetch();  // into the slot of the row before this one, whose values are long used
+    const float scale = rstd, shift = -mean * rstd;
+    if (k + 1 < mine) {
+      mp += step;
+      rp += step;
+      mean = *mp;
+      rstd = *rp;
+    }
+    const bool live = k < mine;
+    float2 xh[R][P], g[R][P];
+    float2 sg = make_float2(0.f, 0.f), sgx = make_float2(0.f, 0.f);
+    const float2 scale2 = make_float2(scale, scale), shift2 = make_float2(shift, shift);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      uint4 xr = make_uint4(0, 0, 0, 0), dr = make_uint4(0, 0, 0, 0);
+      if (live && in[r]) {
+        xr = *reinterpret_cast<const uint4*>(ring_p + at + (2 * r) * stride);
+        dr = *reinterpret_cast<const uint4*>(ring_p + at + (2 * r + 1) * stride);
+      }
+      unpack16(xr, xh[r], (const T*)nullptr);
+      unpack16(dr, g[r], (const T*)nullptr);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        xh[r][i] = __ffma2_rn(xh[r][i], scale2, shift2);
+        if constexpr (PARAMS) {
+          dw[r][i] = __ffma2_rn(g[r][i], xh[r][i], dw[r][i]);
+          db[r][i] = __fadd2_rn(g[r][i], db[r][i]);
+        }
+        g[r][i] = __fmul2_rn(g[r][i], w[r][i]);
+        sg = __fadd2_rn(g[r][i], sg);
+        sgx = __ffma2_rn(g[r][i], xh[r][i], sgx);
+      }
+    }
+    if (A.out) {
+      float sums[2] = {sg.x + sg.y, sgx.x + sgx.y};
+      row_sum(sums, tpr, k & 1);
+      const float mg = -scale * (sums[0] * inv), mgx = -scale * (sums[1] * inv);
+      if (live) {
+        const float2 mg2 = make_float2(mg, mg), mgx2 = make_float2(mgx, mgx);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float2 o[P];
+#pragma unroll
+          for (int i = 0; i < P; ++i)
+            o[i] = __ffma2_rn(xh[r][i], mgx2, __ffma2_rn(g[r][i], scale2, mg2));
+          if (in[r]) *reinterpret_cast<uint4*>(out + r * dc) = pack16(o, (const T*)nullptr);
+        }
+      }
+      out += out_step;
+    }
+    at = at + span == SLOTS * span ? 0 : at + span;
+  }
+  copy_wait<0>();
+  if constexpr (PARAMS) {
+    float a[R][VEC], b[R][VEC];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        a[r][2 * i] = dw[r][i].x;
+        a[r][2 * i + 1] = dw[r][i].y;
+        b[r][2 * i] = db[r][i].x;
+        b[r][2 * i + 1] = db[r][i].y;
+      }
+    norm_store_partial<VEC, R>(A, row_sums, a, b);
+  }
+}
+
+// The same for rows that are not 16-byte aligned: one element at a time.
+template <typename T, typename W, int R, bool PARAMS>
+__global__ void __launch_bounds__(512) norm_backward_scalar_kernel(const NormArgs A) {
+  extern __shared__ __align__(16) float row_sums[];  // [slots][2][cols]
+  const int tpr = A.tpr;
+  const int lane = threadIdx.x & (tpr - 1);
+  const int groups = blockDim.x / tpr;
+  float dw[R][1], db[R][1];
+#pragma unroll
+  for (int r = 0; r < R; ++r) dw[r][0] = db[r][0] = 0.f;
   int flip = 0;
   const float inv = 1.f / (float)A.cols;
   for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows;
@@ -163,90 +432,41 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs A) {
     const T* x = (const T*)A.x + rr * A.x_ld;
     const T* dy = (const T*)A.dy + rr * A.dy_ld;
     const float mean = A.mean[rr], rstd = A.rstd[rr];
-    float xh[R][VEC], g[R][VEC];
-    float sg = 0.f, sgx = 0.f;
+    float xh[R], g[R], sums[2] = {0.f, 0.f};
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int c = (r * tpr + lane) * VEC;
-      if (live && c < A.cols) {
-        load_vec<T, VEC>(x + c, xh[r]);
-        load_vec<T, VEC>(dy + c, g[r]);
-        float w[VEC];
-        if (A.w) load_vec<W, VEC>((const W*)A.w + c, w);
+      const int c = r * tpr + lane;
+      const bool in = live && c < A.cols;
+      xh[r] = in ? to_f(x[c]) : 0.f;
+      g[r] = in ? to_f(dy[c]) : 0.f;
+    }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          xh[r][i] = (xh[r][i] - mean) * rstd;
-          if constexpr (PARAMS) {
-            dw[r][i] = fmaf(g[r][i], xh[r][i], dw[r][i]);
-            db[r][i] += g[r][i];
-          }
-          if (A.w) g[r][i] *= w[i];
-          sg += g[r][i];
-          sgx = fmaf(g[r][i], xh[r][i], sgx);
-        }
+    for (int r = 0; r < R; ++r) {
+      const int c = r * tpr + lane;
+      xh[r] = (xh[r] - mean) * rstd;
+      if constexpr (PARAMS) {
+        dw[r][0] = fmaf(g[r], xh[r], dw[r][0]);
+        db[r][0] += g[r];
       }
+      if (A.w && c < A.cols) g[r] *= to_f(((const W*)A.w)[c]);
+      sums[0] += g[r];
+      sums[1] = fmaf(g[r], xh[r], sums[1]);
     }
     if (A.out) {
-      row_sum2(sg, sgx, tpr, flip);
+      row_sum(sums, tpr, flip);
       flip ^= 1;
-      const float mg = sg * inv, mgx = sgx * inv;
+      const float mg = sums[0] * inv, mgx = sums[1] * inv;
       if (live) {
         T* dx = (T*)A.out + row * A.out_ld;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const int c = (r * tpr + lane) * VEC;
-          if (c < A.cols) {
-            float o[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) o[i] = rstd * (g[r][i] - mg - xh[r][i] * mgx);
-            store_vec<T, VEC>(dx + c, o);
-          }
+          const int c = r * tpr + lane;
+          if (c < A.cols) dx[c] = from_f<T>(rstd * (g[r] - mg - xh[r] * mgx));
         }
       }
     }
   }
-  if constexpr (PARAMS) {
-    float* part = A.partial + (int64_t)blockIdx.x * 2 * A.cols;
-    if (groups == 1) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int c = (r * tpr + lane) * VEC;
-        if (c < A.cols) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            part[c + i] = dw[r][i];
-            part[A.cols + c + i] = db[r][i];
-          }
-        }
-      }
-      return;
-    }
-    // Several rows at a time: add the rows of each warp, then over the slots (a warp, or the warps
-    // of one row).
-    const int slots = tpr < 32 ? blockDim.x >> 5 : groups;
-    float* mine = row_sums + (int64_t)(threadIdx.x / (tpr < 32 ? 32 : tpr)) * 2 * A.cols;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int c = (r * tpr + lane) * VEC;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        for (int o = tpr; o < 32; o <<= 1) {
-          dw[r][i] += __shfl_xor_sync(0xffffffffu, dw[r][i], o);
-          db[r][i] += __shfl_xor_sync(0xffffffffu, db[r][i], o);
-        }
-        if ((threadIdx.x & 31) < tpr && c < A.cols) {  // always true for whole warps
-          mine[c + i] = dw[r][i];
-          mine[A.cols + c + i] = db[r][i];
-        }
-      }
-    }
-    __syncthreads();
-    for (int q = threadIdx.x; q < 2 * A.cols; q += blockDim.x) {
-      float s = 0.f;
-      for (int w = 0; w < slots; ++w) s += row_sums[(int64_t)w * 2 * A.cols + q];
-      part[q] = s;
-    }
-  }
+  if constexpr (PARAMS) norm_store_partial<1, R>(A, row_sums, dw, db);
 }
 
 // dx of rows too wide for registers: x and dy are read twice.
@@ -256,15 +476,15 @@ __global__ void __launch_bounds__(1024) norm_backward_wide_kernel(const NormArgs
   const T* x = (const T*)A.x + row * A.x_ld;
   const T* dy = (const T*)A.dy + row * A.dy_ld;
   const float mean = A.mean[row], rstd = A.rstd[row];
-  float sg = 0.f, sgx = 0.f;
+  float sums[2] = {0.f, 0.f};
   for (int c = threadIdx.x; c < A.cols; c += blockDim.x) {
     float g = to_f(dy[c]);
     if (A.w) g *= to_f(((const W*)A.w)[c]);
-    sg += g;
-    sgx = fmaf(g, (to_f(x[c]) - mean) * rstd, sgx);
+    sums[0] += g;
+    sums[1] = fmaf(g, (to_f(x[c]) - mean) * rstd, sums[1]);
   }
-  row_sum2(sg, sgx, blockDim.x, 0);
-  const float mg = sg / (float)A.cols, mgx = sgx / (float)A.cols;
+  row_sum(sums, blockDim.x, 0);
+  const float mg = sums[0] / (float)A.cols, mgx = sums[1] / (float)A.cols;
   T* dx = (T*)A.out + row * A.out_ld;
   for (int c = threadIdx.x; c < A.cols; c += blockDim.x) {
     float g = to_f(dy[c]);
@@ -294,21 +514,27 @@ __global__ void __launch_bounds__(256) norm_params_wide_kernel(const NormArgs A)
   part[A.cols + c] = db;
 }
 
-// dw and db from the blocks' partial sums: 32 columns per block, 8 threads along the blocks of each.
+// dw and db from the blocks' partial sums: 32 columns per block, 32 threads along the blocks of each.
 template <typename W>
-__global__ void __launch_bounds__(256) norm_params_sum_kernel(const float* __restrict__ partial,
-                                                              int blocks, int cols, W* dw, W* db) {
-  __shared__ float sums[8][33];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) norm_params_sum_kernel(const float* __restrict__ partial,
+                                                               int blocks, int cols, W* dw, W* db) {
+  __shared__ float sums[32][33];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < 2 * cols)
-    for (int b = part; b < blocks; b += 8) s += partial[(int64_t)b * 2 * cols + c];
-  sums[part][threadIdx.x & 31] = s;
+  if (c < 2 * cols) {
+#pragma unroll 8
+    for (int b = part; b < blocks; b += 32) s += partial[(int64_t)b * 2 * cols + c];
+  }
+  sums[part][lane] = s;
   __syncthreads();
-  if (part == 0 && c < 2 * cols) {
-    for (int q = 1; q < 8; ++q) s += sums[q][threadIdx.x & 31];
-    W* dst = c < cols ? dw : db;
-    if (dst) dst[c < cols ? c : c - cols] = from_f<W>(s);
+  s = sums[lane][part];  // transposed: warp `part` sums column `part`
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int col = blockIdx.x * 32 + part;
+  if (lane == 0 && col < 2 * cols) {
+    W* dst = col < cols ? dw : db;
+    if (dst) dst[col < cols ? col : col - cols] = from_f<W>(s);
   }
 }
 
@@ -328,7 +554,7 @@ static int norm_shape(int64_t nvec, int max_tpr, int max_r, int* tpr) {
 // Blocks of the backward pass (each writes one partial row of 2 cols sums), a function of the sizes
 // alone so that the workspace query and the launch agree.
 static int norm_blocks(int64_t rows, int64_t cols) {
-  int64_t b = kFeatSMs * (cols <= 1024 ? 8 : cols <= 4096 ? 4 : 2);
+  const int64_t b = kFeatSMs * (cols <= 256 ? 4 : 2);
   return (int)(b < rows ? b : (rows > 0 ? rows : 1));
 }
 
@@ -340,6 +566,9 @@ static int norm_forward_launch(NormArgs A, cudaStream_t st) {
   A.tpr = tpr;
   if (r == 0) {
     norm_forward_wide_kernel<T, W><<<(unsigned)A.rows, 1024, 0, st>>>(A);
+  } else if (tpr <= 32 && A.rows >= 4096) {
+    norm_forward_rows_kernel<T, W, VEC, 4>
+        <<<(unsigned)ceil_div(A.rows, 128 / tpr * 4), 128, 0, st>>>(A);
   } else {
     const int threads = tpr > 128 ? tpr : 128;
     const unsigned grid = (unsigned)ceil_div(A.rows, threads / tpr);
@@ -354,28 +583,47 @@ static int norm_forward_launch(NormArgs A, cudaStream_t st) {
   return GPB_OK;
 }
 
-template <typename T, typename W, int VEC, bool PARAMS>
-static int norm_backward_vec(NormArgs A, int* blocks, cudaStream_t st, bool* done) {
-  constexpr int kMaxR = VEC == 1 ? 8 : 16 / VEC;
-  int tpr = 1;
-  const int r = norm_shape(ceil_div(A.cols, VEC), 512, kMaxR, &tpr);
-  *done = r != 0;
-  if (r == 0) return GPB_OK;
-  A.tpr = tpr;
-  const int threads = tpr > 256 ? tpr : 256;
-  // At most 16 KB: a row of fewer threads than the block has one vector per thread.
-  const int slots = tpr < 32 ? threads / 32 : threads / tpr;
-  const size_t smem = PARAMS && tpr < threads ? (size_t)slots * 2 * A.cols * sizeof(float) : 0;
-  const int grid = (int)std::min<int64_t>(*blocks, ceil_div(A.rows, threads / tpr));
-  *blocks = grid;
-  switch (r) {
-    case 1: norm_backward_kernel<T, W, VEC, 1, PARAMS><<<grid, threads, smem, st>>>(A); break;
-    case 2: norm_backward_kernel<T, W, VEC, 2, PARAMS><<<grid, threads, smem, st>>>(A); break;
-    case 4: norm_backward_kernel<T, W, VEC, 4 <= kMaxR ? 4 : kMaxR, PARAMS><<<grid, threads, smem, st>>>(A); break;
-    default: norm_backward_kernel<T, W, VEC, kMaxR, PARAMS><<<grid, threads, smem, st>>>(A);
+template <typename T, typename W, int VEC, int R, bool PARAMS>
+static int norm_backward_run(const NormArgs& A, int grid, int threads, cudaStream_t st) {
+  // The ring, or afterwards the slots' sums.
+  const int slots = A.tpr < 32 ? threads / 32 : threads / A.tpr;
+  size_t smem = PARAMS && A.tpr < threads ? (size_t)slots * 2 * A.cols * sizeof(float) : 0;
+  if constexpr (VEC > 1) {
+    smem = std::max<size_t>(smem, (size_t)(kNormAhead<R> + 1) * R * 2 * threads * 16);
+    constexpr auto kernel = norm_backward_kernel<T, W, VEC, R, PARAMS>;
+    if (smem > 40 * 1024)  // with the static part, 48 KB need no opt-in
+      GPB_CHECK_CUDA(
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<grid, threads, smem, st>>>(A);
+  } else {
+    norm_backward_scalar_kernel<T, W, R, PARAMS><<<grid, threads, smem, st>>>(A);
   }
   GPB_CHECK_CUDA(cudaGetLastError());
   return GPB_OK;
+}
+
+template <typename T, typename W, int VEC, bool PARAMS>
+static int norm_backward_vec(NormArgs A, int* blocks, cudaStream_t st, bool* done) {
+  // 16 columns per thread in vectors, 8 otherwise (registers). A row takes as few threads as that
+  // allows, but a warp before a second vector.
+  constexpr int kMaxR = VEC == 1 ? 8 : 16 / VEC;
+  const int64_t nvec = ceil_div(A.cols, VEC);
+  int tpr = 1, r = 1;
+  while (tpr < 32 && tpr < nvec) tpr <<= 1;
+  while (r < kMaxR && (int64_t)tpr * r < nvec) r <<= 1;
+  while (tpr < 512 && (int64_t)tpr * r < nvec) tpr <<= 1;
+  *done = (int64_t)tpr * r >= nvec;
+  if (!*done) return GPB_OK;
+  A.tpr = tpr;
+  const int threads = tpr > 256 ? tpr : 256;
+  const int grid = (int)std::min<int64_t>(*blocks, ceil_div(A.rows, threads / tpr));
+  *blocks = grid;
+  switch (r) {
+    case 1: return norm_backward_run<T, W, VEC, 1, PARAMS>(A, grid, threads, st);
+    case 2: return norm_backward_run<T, W, VEC, 2 <= kMaxR ? 2 : kMaxR, PARAMS>(A, grid, threads, st);
+    case 4: return norm_backward_run<T, W, VEC, 4 <= kMaxR ? 4 : kMaxR, PARAMS>(A, grid, threads, st);
+    default: return norm_backward_run<T, W, VEC, kMaxR, PARAMS>(A, grid, threads, st);
+  }
 }
 
 template <typename T, typename W, int VEC>
@@ -401,7 +649,7 @@ static int norm_backward_launch(NormArgs A, W* dw, W* db, cudaStream_t st) {
     }
   }
   if (params) {
-    norm_params_sum_kernel<W><<<(unsigned)ceil_div(2 * (int64_t)A.cols, 32), 256, 0, st>>>(
+    norm_params_sum_kernel<W><<<(unsigned)ceil_div(2 * (int64_t)A.cols, 32), 1024, 0, st>>>(
         A.partial, blocks, A.cols, dw, db);
     GPB_CHECK_CUDA(cudaGetLastError());
   }

@@ -95,4 +95,37 @@ __device__ __forceinline__ void store_vec(T* p, const float (&in)[VEC]) {
   *reinterpret_cast<Pack<T, VEC>*>(p) = q;
 }
 
+// The VEC elements of 16 raw bytes as fp32 pairs, and back (rounded to nearest).
+__device__ __forceinline__ void unpack16(const uint4& q, float2 (&o)[2], const float*) {
+  o[0] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+  o[1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
+}
+__device__ __forceinline__ void unpack16(const uint4& q, float2 (&o)[4], const __nv_bfloat16*) {
+  const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    o[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
+}
+__device__ __forceinline__ void unpack16(const uint4& q, float2 (&o)[4], const __half*) {
+  const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+}
+__device__ __forceinline__ uint4 pack16(const float2 (&v)[2], const float*) {
+  return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x),
+                    __float_as_uint(v[1].y));
+}
+template <typename H2>
+__device__ __forceinline__ uint32_t bits32(const H2& h) {
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 pack16(const float2 (&v)[4], const __nv_bfloat16*) {
+  return make_uint4(bits32(__float22bfloat162_rn(v[0])), bits32(__float22bfloat162_rn(v[1])),
+                    bits32(__float22bfloat162_rn(v[2])), bits32(__float22bfloat162_rn(v[3])));
+}
+__device__ __forceinline__ uint4 pack16(const float2 (&v)[4], const __half*) {
+  return make_uint4(bits32(__float22half2_rn(v[0])), bits32(__float22half2_rn(v[1])),
+                    bits32(__float22half2_rn(v[2])), bits32(__float22half2_rn(v[3])));
+}
+
 }  // namespace gpb

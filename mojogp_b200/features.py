@@ -18,6 +18,7 @@ the same time. Argument errors raise ValueError before any device work.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -45,41 +46,42 @@ class _View:
     __slots__ = ("ptr", "shape", "ld", "code", "device")
 
     def __init__(self, a, name: str, ndim: int):
-        shape = tuple(a.shape)
+        self.shape = shape = a.shape
         if len(shape) != ndim:
             raise ValueError(f"{name} must be {ndim}-D, got shape {shape}")
-        data_ptr = getattr(a, "data_ptr", None)
-        if data_ptr is not None:
-            dev = a.device
-            if dev.type != "cuda":
-                raise ValueError(f"{name} must be on a CUDA device, got {dev}")
-            self.device = dev.index
-            self.ptr = data_ptr()
-            strides = a.stride()
-            if strides[-1] != 1 and shape[-1] > 1:
-                raise ValueError(f"{name} must have unit column stride, got strides {strides}")
-            self.ld = strides[0] if ndim == 2 and shape[0] > 1 else shape[-1]
-            self.code = _dtype_code(a.dtype)
-        elif hasattr(a, "ptr") and hasattr(a, "nbytes"):
-            self.device = a.device
-            self.ptr = a.ptr
-            self.ld = shape[-1]
-            self.code = _dtype_code(getattr(a, "element_type", None) or a.dtype)
+        try:
+            self.ptr = a.data_ptr()
+        except AttributeError:
+            if not (hasattr(a, "ptr") and hasattr(a, "nbytes")):
+                raise ValueError(f"{name} must be a device array, got {type(a).__name__}") from None
+            self.ptr, self.device, self.ld = a.ptr, a.device, shape[-1]
+            self.code = _element_code(a)
             if self.ptr is None:
-                raise ValueError(f"{name} was freed")
-        else:
-            raise ValueError(f"{name} must be a device array, got {type(a).__name__}")
-        self.shape = shape
+                raise ValueError(f"{name} was freed") from None
+            return
+        self.device = index = a.device.index
+        if index is None or a.device.type != "cuda":
+            raise ValueError(f"{name} must be on a CUDA device, got {a.device}")
+        strides = a.stride()
+        if strides[-1] != 1 and shape[-1] > 1:
+            raise ValueError(f"{name} must have unit column stride, got strides {strides}")
+        self.ld = strides[0] if ndim == 2 and shape[0] > 1 else shape[-1]
+        dtype = a.dtype
+        self.code = _CODES[dtype] if dtype in _CODES else _dtype_code(dtype)
 
 
-def _vector(a, name: str, size: int, like: "_View", codes) -> int | None:
-    """Pointer of a [size] vector of one of the element types `codes`, or None."""
+def _element_code(a) -> int:
+    return _dtype_code(getattr(a, "element_type", None) or a.dtype)
+
+
+def _vector(a, name: str, size: int, like: "_View", code: int) -> int | None:
+    """Pointer of a [size] vector of element type `code`, or None."""
     if a is None:
         return None
     v = _View(a, name, 1)
     if v.shape[0] != size:
         raise ValueError(f"{name} must have {size} entries, got {v.shape[0]}")
-    if v.code not in codes:
+    if v.code != code:
         raise ValueError(f"{name} has a different element type")
     if v.device != like.device:
         raise ValueError(f"{name} is on device {v.device}, expected {like.device}")
@@ -97,12 +99,10 @@ def _matrix(a, name: str, shape: tuple, like: "_View") -> "_View":
     return v
 
 
-def _workspace(a, need: int, like: "_View") -> tuple:
-    """(pointer, bytes) of a scratch array."""
-    if need == 0 and a is None:
-        return None, 0
+def _workspace(a, like: "_View") -> tuple:
+    """(pointer, bytes) of a scratch array; the call itself checks the size."""
     if a is None:
-        raise ValueError(f"a workspace of {need} bytes is needed")
+        return None, 0
     data_ptr = getattr(a, "data_ptr", None)
     if data_ptr is not None:
         if a.device.type != "cuda":
@@ -141,16 +141,17 @@ def layer_norm(out, x, weight=None, bias=None, *, eps: float = 1e-5, mean=None, 
     pcode = xv.code
     for a in (weight, bias):
         if a is not None:
-            pcode = _dtype_code(getattr(a, "element_type", None) or a.dtype)
+            pcode = _element_code(a)
             break
     if pcode not in (0, xv.code):
         raise ValueError("weight and bias must be float32 or of x's type")
     _lib.call("gpb_layer_norm", xv.device, stream, xv.code, pcode, rows, cols, ov.ptr, ov.ld,
-              xv.ptr, xv.ld, _vector(weight, "weight", cols, xv, (pcode,)),
-              _vector(bias, "bias", cols, xv, (pcode,)), eps,
-              _vector(mean, "mean", rows, xv, (0,)), _vector(rstd, "rstd", rows, xv, (0,)))
+              xv.ptr, xv.ld, _vector(weight, "weight", cols, xv, pcode),
+              _vector(bias, "bias", cols, xv, pcode), eps,
+              _vector(mean, "mean", rows, xv, 0), _vector(rstd, "rstd", rows, xv, 0))
 
 
+@functools.lru_cache(maxsize=256)
 def layer_norm_workspace(rows: int, cols: int) -> int:
     """Workspace bytes of layer_norm_backward with weight or bias gradients."""
     n = C.c_int64()
@@ -172,18 +173,17 @@ def layer_norm_backward(dx, dout, x, mean, rstd, weight=None, *, dweight=None, d
     pcode = xv.code
     for a in (weight, dweight, dbias):
         if a is not None:
-            pcode = _dtype_code(getattr(a, "element_type", None) or a.dtype)
+            pcode = _element_code(a)
             break
     if pcode not in (0, xv.code):
         raise ValueError("weight and its gradient must be float32 or of x's type")
-    need = layer_norm_workspace(rows, cols) if dweight is not None or dbias is not None else 0
-    wptr, wbytes = _workspace(workspace, need, xv)
+    wptr, wbytes = _workspace(workspace, xv)
     _lib.call("gpb_layer_norm_backward", xv.device, stream, xv.code, pcode, rows, cols,
               ov.ptr if ov else None, ov.ld if ov else 0, dv.ptr, dv.ld, xv.ptr, xv.ld,
-              _vector(mean, "mean", rows, xv, (0,)), _vector(rstd, "rstd", rows, xv, (0,)),
-              _vector(weight, "weight", cols, xv, (pcode,)),
-              _vector(dweight, "dweight", cols, xv, (pcode,)),
-              _vector(dbias, "dbias", cols, xv, (pcode,)), wptr, wbytes)
+              _vector(mean, "mean", rows, xv, 0), _vector(rstd, "rstd", rows, xv, 0),
+              _vector(weight, "weight", cols, xv, pcode),
+              _vector(dweight, "dweight", cols, xv, pcode),
+              _vector(dbias, "dbias", cols, xv, pcode), wptr, wbytes)
 
 
 # ------------------------------------------------------------- gated unit
@@ -194,6 +194,7 @@ def _activation(name: str) -> int:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {name!r}") from None
 
 
+@functools.lru_cache(maxsize=256)
 def gated_unit_workspace(rows: int, inner: int, outer: int, dtype, backward: bool = False) -> int:
     """Workspace bytes of gated_unit (or of its backward pass) for x [rows,
     inner] and weights [outer, inner] of element type `dtype`."""
@@ -211,8 +212,8 @@ def _gated_inputs(x, w_gate, w_up, b_gate, b_up):
     u = _matrix(w_up, "w_up", (outer, xv.shape[1]), xv)
     if g.ld != u.ld:
         raise ValueError(f"w_gate and w_up must have one row stride, got {g.ld} and {u.ld}")
-    return (xv, g, u, _vector(b_gate, "b_gate", outer, xv, (xv.code,)),
-            _vector(b_up, "b_up", outer, xv, (xv.code,)))
+    return (xv, g, u, _vector(b_gate, "b_gate", outer, xv, xv.code),
+            _vector(b_up, "b_up", outer, xv, xv.code))
 
 
 def gated_unit(out, x, w_gate, w_up, b_gate=None, b_up=None, *, activation: str = "silu",
@@ -227,7 +228,7 @@ def gated_unit(out, x, w_gate, w_up, b_gate=None, b_up=None, *, activation: str 
     rows, inner = xv.shape
     outer = g.shape[0]
     ov = _matrix(out, "out", (rows, outer), xv)
-    wptr, wbytes = _workspace(workspace, 0, xv)
+    wptr, wbytes = _workspace(workspace, xv)
     _lib.call("gpb_gated_unit", xv.device, stream, xv.code, act, rows, inner, outer, ov.ptr, ov.ld,
               xv.ptr, xv.ld, g.ptr, u.ptr, g.ld, bg, bu, wptr, wbytes)
 
@@ -249,13 +250,13 @@ def gated_unit_backward(dout, x, w_gate, w_up, b_gate=None, b_up=None, *, dx=Non
     if go and uo and go.ld != uo.ld:
         raise ValueError(f"dw_gate and dw_up must have one row stride, got {go.ld} and {uo.ld}")
     wo = go or uo
-    wptr, wbytes = _workspace(workspace, 0, xv)
+    wptr, wbytes = _workspace(workspace, xv)
     _lib.call("gpb_gated_unit_backward", xv.device, stream, xv.code, act, rows, inner, outer,
               dv.ptr, dv.ld, xv.ptr, xv.ld, g.ptr, u.ptr, g.ld, bg, bu,
               xo.ptr if xo else None, xo.ld if xo else 0, go.ptr if go else None,
               uo.ptr if uo else None, wo.ld if wo else 0,
-              _vector(db_gate, "db_gate", outer, xv, (xv.code,)),
-              _vector(db_up, "db_up", outer, xv, (xv.code,)), wptr, wbytes)
+              _vector(db_gate, "db_gate", outer, xv, xv.code),
+              _vector(db_up, "db_up", outer, xv, xv.code), wptr, wbytes)
 
 
 # ---------------------------------------------------------------- dropout
