@@ -106,14 +106,15 @@ __global__ void __launch_bounds__(256) gated_rows_kernel(const GatedArgs A, floa
     if (lane == m && m < A.rows) {
       const float gate = g[m] + (A.bg ? to_f(((const T*)A.bg)[n]) : 0.f);
       const float up = u[m] + (A.bu ? to_f(((const T*)A.bu)[n]) : 0.f);
-      float value, slope;
-      gated_act(A.act, gate, value, slope);
+      const float z[1] = {gate};
+      float value[1], slope[1];
+      gated_act<BACK>(A.act, z, value, slope);
       if constexpr (BACK) {
         const float dy = to_f(((const T*)A.dout)[m * A.dout_ld + n]);
-        dg[m * A.outer + n] = dy * up * slope;
-        du[m * A.outer + n] = dy * value;
+        dg[m * A.outer + n] = dy * up * slope[0];
+        du[m * A.outer + n] = dy * value[0];
       } else {
-        ((T*)A.out)[m * A.out_ld + n] = from_f<T>(value * up);
+        ((T*)A.out)[m * A.out_ld + n] = from_f<T>(value[0] * up);
       }
     }
   }
@@ -209,43 +210,6 @@ __global__ void __launch_bounds__(256) mm_join_kernel(const float* __restrict__ 
   if (c) c[(f / N) * c_ld + f % N] = from_f<T>(s);
 }
 
-// Column sums of the planes of dgate and dup (blockIdx.y picks one): 32 columns x 8 row lanes per
-// block, rows in ranges over blockIdx.z, joined in range order by gated_bias_join.
-template <typename D>
-__global__ void __launch_bounds__(256) gated_bias_kernel(const D* dg, const D* du, int64_t rows,
-                                                         int64_t outer, int64_t ld, int planes,
-                                                         int64_t plane, float* partial) {
-  __shared__ float sums[8][33];
-  const D* d = blockIdx.y == 0 ? dg : du;
-  const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-  const int part = threadIdx.x >> 5;
-  const int64_t per = (rows + gridDim.z - 1) / gridDim.z;
-  const int64_t r0 = blockIdx.z * per, r1 = r0 + per < rows ? r0 + per : rows;
-  float s = 0.f;
-  if (c < outer)
-    for (int64_t r = r0 + part; r < r1; r += 8) {
-      float v = to_f(d[r * ld + c]);
-      for (int p = 1; p < planes; ++p) v += to_f(d[p * plane + r * ld + c]);
-      s += v;
-    }
-  sums[part][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (part == 0 && c < outer) {
-    for (int q = 1; q < 8; ++q) s += sums[q][threadIdx.x & 31];
-    partial[((int64_t)blockIdx.z * 2 + blockIdx.y) * outer + c] = s;
-  }
-}
-template <typename T>
-__global__ void __launch_bounds__(256) gated_bias_join(const float* partial, int ranges,
-                                                       int64_t outer, T* dbg, T* dbu) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= 2 * outer) return;
-  float s = 0.f;
-  for (int r = 0; r < ranges; ++r) s += partial[r * 2 * outer + e];
-  T* dst = e < outer ? dbg : dbu;
-  if (dst) dst[e < outer ? e : e - outer] = from_f<T>(s);
-}
-
 // A matrix to tensor-core operands: fp32 to three bf16 planes, or a 16-bit matrix whose rows are not
 // 16-byte aligned to one plane whose are. 8 output columns per thread; columns up to ld are zeros.
 template <typename T, typename D>
@@ -324,7 +288,7 @@ struct GatedPlan {
   int64_t partial = 0, total = 0;
   int tile_n = 0;                      // GG_DW column tile
   int splits = 1, kb_per = 1;          // GG_DW
-  int ranges_b = 1;                    // bias gradients
+  int64_t sums = 0;                    // column sums of dgate and dup
   int ranges_x = 1;                    // dx of few rows
 };
 
@@ -373,10 +337,8 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * kFeatSMs / tiles, kb / 8));
     P.kb_per = (int)ceil_div(kb, want);
     P.splits = (int)ceil_div(kb, P.kb_per);
-    P.ranges_b = (int)std::max<int64_t>(
-        1, std::min<int64_t>(ceil_div(4 * kFeatSMs, ceil_div(outer, 32)), ceil_div(rows, 256)));
-    P.partial = take(at, std::max<int64_t>(P.splits > 1 ? P.splits * 2 * outer * inner : 0,
-                                           P.ranges_b * 2 * outer) * 4);
+    P.partial = take(at, P.splits > 1 ? P.splits * 2 * outer * inner * 4 : 0);
+    P.sums = take(at, 4 * ceil_div(rows, kGgBM) * 2 * outer * 4);
   }
   P.total = at;
   return P;
@@ -575,6 +537,7 @@ static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, con
     G.out_ld = P.ldn;
     G.plane = P.plane_d;
     G.vec = aligned16(A.dout) && A.dout_ld % V == 0;
+    if (R.dbg || R.dbu) G.col_sums = (float*)(ws + P.sums);
     GPB_TRY((gated_project<T, D, PL, true>(A, x, wg, wu, G, st)));
   }
   if (R.dx) {
@@ -624,11 +587,8 @@ static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, con
     }
   }
   if (R.dbg || R.dbu) {
-    gated_bias_kernel<D><<<dim3((unsigned)ceil_div(A.outer, 32), 2, P.ranges_b), 256, 0, st>>>(
-        (const D*)dg.p, (const D*)du.p, A.rows, A.outer, P.ldn, PL, P.plane_d, partial);
-    GPB_CHECK_CUDA(cudaGetLastError());
-    gated_bias_join<T><<<(unsigned)ceil_div(2 * A.outer, 256), 256, 0, st>>>(
-        partial, P.ranges_b, A.outer, (T*)R.dbg, (T*)R.dbu);
+    column_join_kernel<T><<<(unsigned)ceil_div(2 * A.outer, 32), 1024, 0, st>>>(
+        (const float*)(ws + P.sums), 4 * ceil_div(A.rows, kGgBM), A.outer, (T*)R.dbg, (T*)R.dbu);
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   return GPB_OK;

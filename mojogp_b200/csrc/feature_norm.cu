@@ -514,30 +514,6 @@ __global__ void __launch_bounds__(256) norm_params_wide_kernel(const NormArgs A)
   part[A.cols + c] = db;
 }
 
-// dw and db from the blocks' partial sums: 32 columns per block, 32 threads along the blocks of each.
-template <typename W>
-__global__ void __launch_bounds__(1024) norm_params_sum_kernel(const float* __restrict__ partial,
-                                                               int blocks, int cols, W* dw, W* db) {
-  __shared__ float sums[32][33];
-  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
-  float s = 0.f;
-  if (c < 2 * cols) {
-#pragma unroll 8
-    for (int b = part; b < blocks; b += 32) s += partial[(int64_t)b * 2 * cols + c];
-  }
-  sums[part][lane] = s;
-  __syncthreads();
-  s = sums[lane][part];  // transposed: warp `part` sums column `part`
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  const int col = blockIdx.x * 32 + part;
-  if (lane == 0 && col < 2 * cols) {
-    W* dst = col < cols ? dw : db;
-    if (dst) dst[col < cols ? col : col - cols] = from_f<W>(s);
-  }
-}
-
 // ------------------------------------------------------------------ host
 // Threads per row and vectors per thread for `nvec` vectors: the widest part of a warp first, then
 // blocks of warps, growing R only once the row has `max_tpr` threads. Returns R, or 0 when the row
@@ -649,7 +625,7 @@ static int norm_backward_launch(NormArgs A, W* dw, W* db, cudaStream_t st) {
     }
   }
   if (params) {
-    norm_params_sum_kernel<W><<<(unsigned)ceil_div(2 * (int64_t)A.cols, 32), 1024, 0, st>>>(
+    column_join_kernel<W><<<(unsigned)ceil_div(2 * (int64_t)A.cols, 32), 1024, 0, st>>>(
         A.partial, blocks, A.cols, dw, db);
     GPB_CHECK_CUDA(cudaGetLastError());
   }

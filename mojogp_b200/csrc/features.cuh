@@ -128,4 +128,29 @@ __device__ __forceinline__ uint4 pack16(const float2 (&v)[4], const __half*) {
                     bits32(__float22half2_rn(v[2])), bits32(__float22half2_rn(v[3])));
 }
 
+// Column sums of `blocks` partial rows [2][cols] to two vectors (either may be null): 32 columns per
+// block, 32 threads along the rows of each, in a fixed order.
+template <typename W>
+__global__ void __launch_bounds__(1024) column_join_kernel(const float* __restrict__ partial,
+                                                           int64_t blocks, int64_t cols, W* a, W* b) {
+  __shared__ float sums[32][33];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < 2 * cols) {
+#pragma unroll 8
+    for (int64_t r = part; r < blocks; r += 32) s += partial[r * 2 * cols + c];
+  }
+  sums[part][lane] = s;
+  __syncthreads();
+  s = sums[lane][part];  // transposed: warp `part` sums column `part`
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int64_t col = (int64_t)blockIdx.x * 32 + part;
+  if (lane == 0 && col < 2 * cols) {
+    W* dst = col < cols ? a : b;
+    if (dst) dst[col < cols ? col : col - cols] = from_f<W>(s);
+  }
+}
+
 }  // namespace gpb
