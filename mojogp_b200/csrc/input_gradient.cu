@@ -6,16 +6,24 @@
 // inputs, which a learned feature map's backward pass starts from.
 //
 // One stationary leaf (with or without a scale node): d1 k = -psi (x_i - x_j) / l^2 with
-// psi = -2 dk/ds, s the scaled squared distance. Differences are taken between the raw inputs and
-// scaled after: prescaled inputs would lose the direction of near pairs to their rounding, which
-// Matern-1/2 does not damp. A thread owns two rows and a cluster of 8 blocks splits the columns of a
-// row tile and joins through distributed shared memory, in block order: no workspace (a captured
-// graph owns nothing) and no atomics.
+// psi = -2 dk/ds, s the scaled squared distance. Two kernels:
+//   few columns (up to 4): G_ij on the CUDA cores, two rows per thread;
+//   more: G = [a | b]' [b | a] is a product of depth 32, formed on the tensor cores (bf16 planes, six
+//     products, fp32-accurate) into TMEM while the CUDA cores run psi and the sums over j. On the CUDA
+//     cores G was 32 of the 74 FMAs of a pair: 2.0 ms at 20000 points in 8 dimensions.
+// Both work on fp32 pairs (FFMA2), split the columns of a row tile over a cluster of 8 blocks and
+// join through distributed shared memory, in block order: no workspace (a captured graph owns
+// nothing) and no atomics.
+//
+// Differences are taken between prescaled inputs x / l, except for Matern-1/2: its psi grows as 1 / r,
+// so the direction of near pairs counts, which rounding x / l would lose; there the raw inputs are
+// subtracted and the difference scaled.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cmath>
 
-#include "features.cuh"
+#include "gated_gemm.cuh"
 #include "provider.cuh"
 
 namespace gpb {
@@ -29,33 +37,35 @@ struct InputGradArgs {
   float* out;        // [n][d]
   int64_t n;
   int32_t d, nd, cols, accumulate;
-  float os, alpha;   // effective output scale, RQ alpha
+  float power;       // RQ: alpha + 1
   int32_t clamp12;   // Matern-1/2 ARD bounds its exponent
   int32_t dims[GPB_MAX_DIM];
-  float inv_l[GPB_MAX_DIM];
+  float scale[GPB_MAX_DIM];      // of the inputs; 0 past nd
+  float out_scale[GPB_MAX_DIM];  // of the sums
+  int* err;                  // the provider's device error word
 };
 
-// psi of the leaf at scaled squared distance s, without the output scale; the same clamps as the
-// leaf's own value and parameter gradients (kernel_program.cuh).
+// psi of the leaf at squared distance s of inputs scaled by 1 / l and the leaf's own constant (which
+// leaves one multiplication between a square root and an exponential), without the factor that
+// provider_input_gradient folds into out_scale; the same clamps as the leaf's value and parameter
+// gradients (kernel_program.cuh).
 template <int LEAF>
-__device__ __forceinline__ float leaf_psi(float s, float alpha, int clamp12) {
-  if constexpr (LEAF == GPB_KERNEL_RBF) {
-    return ex2_approx(s * (-0.5f * kLog2e));
-  } else if constexpr (LEAF == GPB_KERNEL_RQ) {
-    const float base = 1.f + s / (2.f * alpha);
-    return ex2_approx(-(alpha + 1.f) * lg2_approx(base));
+__device__ __forceinline__ float pair_psi(float s, const InputGradArgs& A) {
+  if constexpr (LEAF == GPB_KERNEL_RBF) {  // s / (2 ln 2)
+    return ex2_approx(-s);
+  } else if constexpr (LEAF == GPB_KERNEL_RQ) {  // s / (2 alpha)
+    return ex2_approx(-A.power * lg2_approx(1.f + s));
   } else {
     const float ss = fmaxf(s, 1e-20f);
-    const float rinv = rsqrtf(ss);
+    float rinv;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(rinv) : "f"(ss));
     const float r = ss * rinv;
     if constexpr (LEAF == GPB_KERNEL_MATERN12) {
-      const float e = ex2_approx((clamp12 ? fmaxf(-r, -20.f) : -r) * kLog2e);
-      return e * rinv;
-    } else if constexpr (LEAF == GPB_KERNEL_MATERN32) {
-      return 3.f * ex2_approx(fmaxf(-1.7320508075688772f * r, -20.f) * kLog2e);
+      const float x = r * -kLog2e;
+      return ex2_approx(A.clamp12 ? fmaxf(x, -20.f * kLog2e) : x) * rinv;
     } else {
-      const float r5 = 2.23606797749979f * r;
-      return (5.f / 3.f) * (1.f + r5) * ex2_approx(fmaxf(-r5, -20.f) * kLog2e);
+      const float e = ex2_approx(fmaxf(r * -kLog2e, -20.f * kLog2e));  // 3 s, 5 s
+      return LEAF == GPB_KERNEL_MATERN32 ? e : fmaf(r, e, e);
     }
   }
 }
@@ -64,101 +74,379 @@ constexpr int kIgThreads = 128;
 constexpr int kIgTile = 32;     // columns staged per step
 constexpr int kIgCluster = 8;   // blocks along the columns of one row tile
 
-// T right-hand-side pairs, D input dims (padded with zeros), R rows per thread.
-template <int LEAF, int D, int T, int R>
-__global__ void __cluster_dims__(1, kIgCluster, 1) __launch_bounds__(kIgThreads)
-    input_gradient_kernel(const __grid_constant__ InputGradArgs A) {
-  constexpr int W = (D + 2 * T + 3) / 4 * 4;
-  __shared__ __align__(16) float tile[kIgTile * W];
-  extern __shared__ float sums[];  // [R * kIgThreads][D]
-  const int64_t row0 = (int64_t)blockIdx.x * (kIgThreads * R) + threadIdx.x;
-  float xi[R][D], ai[R][T], bi[R][T], acc[R][D];
+// x (a row's coordinates as pairs) minus a column's, scaled where the inputs are raw.
+template <int LEAF, int D2>
+__device__ __forceinline__ void ig_diff(const InputGradArgs& A, const float2 (&x)[D2],
+                                        const float2* col, float2 (&diff)[D2]) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int64_t i = row0 + r * kIgThreads;
-    const bool in = i < A.n;
-#pragma unroll
-    for (int q = 0; q < D; ++q) {
-      xi[r][q] = in && q < A.nd ? A.X[i * A.d + A.dims[q]] : 0.f;
-      acc[r][q] = 0.f;
-    }
-#pragma unroll
-    for (int c = 0; c < T; ++c) {
-      ai[r][c] = in && c < A.cols ? A.a[c * A.n + i] : 0.f;
-      bi[r][c] = in && c < A.cols ? A.b[c * A.n + i] : 0.f;
-    }
+  for (int q = 0; q < D2; ++q) {
+    const float2 c = col[q];  // negated
+    diff[q] = __fadd2_rn(x[q], c);
+    if constexpr (LEAF == GPB_KERNEL_MATERN12)
+      diff[q] = __fmul2_rn(diff[q], make_float2(A.scale[2 * q], A.scale[2 * q + 1]));
   }
-  const int64_t tiles = (A.n + kIgTile - 1) / kIgTile;
-  for (int64_t t = blockIdx.y; t < tiles; t += kIgCluster) {
-    const int64_t j0 = t * kIgTile;
-    __syncthreads();
-    for (int q = threadIdx.x; q < kIgTile * (D + 2 * T); q += kIgThreads) {
-      const int f = q / kIgTile, j = q % kIgTile;
-      const bool in = j0 + j < A.n;
-      float v = 0.f;
-      if (f < D) {
-        if (in && f < A.nd) v = A.X[(j0 + j) * A.d + A.dims[f]];
-      } else if (f < D + T) {
-        if (in && f - D < A.cols) v = A.a[(int64_t)(f - D) * A.n + j0 + j];
-      } else {
-        if (in && f - D - T < A.cols) v = A.b[(int64_t)(f - D - T) * A.n + j0 + j];
-      }
-      tile[j * W + f] = v;
-    }
-    __syncthreads();
-    // Columns past n carry zero a and b, so their weight is 0 at whatever finite psi; none is
-    // evaluated all the same.
-    const int jn = (int)(A.n - j0 < kIgTile ? A.n - j0 : kIgTile);
-    for (int j = 0; j < jn; ++j) {
-      float col[W];
-#pragma unroll
-      for (int q = 0; q < W / 4; ++q) {
-        const float4 v = *reinterpret_cast<const float4*>(tile + j * W + 4 * q);
-        col[4 * q] = v.x;
-        col[4 * q + 1] = v.y;
-        col[4 * q + 2] = v.z;
-        col[4 * q + 3] = v.w;
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float diff[D], s = 0.f, g = 0.f;
-#pragma unroll
-        for (int q = 0; q < D; ++q) {
-          diff[q] = (xi[r][q] - col[q]) * A.inv_l[q];
-          s = fmaf(diff[q], diff[q], s);
-        }
-#pragma unroll
-        for (int c = 0; c < T; ++c) {
-          g = fmaf(ai[r][c], col[D + T + c], g);
-          g = fmaf(bi[r][c], col[D + c], g);
-        }
-        g *= leaf_psi<LEAF>(s, A.alpha, A.clamp12);
-#pragma unroll
-        for (int q = 0; q < D; ++q) acc[r][q] = fmaf(g, diff[q], acc[r][q]);
-      }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int q = 0; q < D; ++q) sums[(r * kIgThreads + threadIdx.x) * D + q] = acc[r][q];
+}
+
+// Input coordinate f of point i as the kernels subtract it.
+template <int LEAF>
+__device__ __forceinline__ float ig_coord(const InputGradArgs& A, int64_t i, int f) {
+  if (i >= A.n || f >= A.nd) return 0.f;
+  const float x = A.X[i * A.d + A.dims[f]];
+  return LEAF == GPB_KERNEL_MATERN12 ? x : x * A.scale[f];
+}
+
+// Adds the cluster's sums [parts][rows][D] in block order and writes rows congruent to this block's
+// rank. Every thread of the cluster takes part.
+template <int D, int PARTS>
+__device__ __forceinline__ void ig_join(const InputGradArgs& A, float* sums, int rows, int64_t row0) {
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
-  // Each block of the cluster writes the rows congruent to its rank: one thread per row.
-  for (int lr = blockIdx.y + threadIdx.x * kIgCluster; lr < R * kIgThreads;
-       lr += kIgThreads * kIgCluster) {
-    const int64_t i = (int64_t)blockIdx.x * (kIgThreads * R) + lr;
+  for (int lr = blockIdx.y + threadIdx.x * kIgCluster; lr < rows; lr += blockDim.x * kIgCluster) {
+    const int64_t i = row0 + lr;
     if (i >= A.n) continue;
     float* o = A.out + i * A.d;
     if (!A.accumulate)
       for (int q = 0; q < A.d; ++q) o[q] = 0.f;
     for (int q = 0; q < A.nd; ++q) {
       float s = 0.f;
-      for (int k = 0; k < kIgCluster; ++k) s += cluster.map_shared_rank(sums, k)[lr * D + q];
-      o[A.dims[q]] -= s * A.os * A.inv_l[q];
+#pragma unroll
+      for (int k = 0; k < kIgCluster; ++k) {
+        const float* remote = cluster.map_shared_rank(sums, k);
+        for (int p = 0; p < PARTS; ++p) s += remote[(p * rows + lr) * D + q];
+      }
+      o[A.dims[q]] -= s * A.out_scale[q];
     }
   }
   cluster.sync();
+}
+
+// Up to 4 right-hand-side pairs; D input dims (an even number, padded with zeros), R rows per thread.
+template <int LEAF, int D, int R>
+__global__ void __cluster_dims__(1, kIgCluster, 1) __launch_bounds__(kIgThreads)
+    input_gradient_kernel(const __grid_constant__ InputGradArgs A) {
+  constexpr int T = 4, D2 = D / 2;
+  constexpr int W = D + 2 * T;
+  __shared__ __align__(16) float tile[2][kIgTile * W];
+  extern __shared__ float sums[];  // [R * kIgThreads][D]
+  const int64_t row0 = (int64_t)blockIdx.x * (kIgThreads * R) + threadIdx.x;
+  float2 xi[R][D2], acc[R][D2];
+  float2 ai[R][T / 2], bi[R][T / 2];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t i = row0 + r * kIgThreads;
+#pragma unroll
+    for (int q = 0; q < D2; ++q) {
+      xi[r][q] = make_float2(ig_coord<LEAF>(A, i, 2 * q), ig_coord<LEAF>(A, i, 2 * q + 1));
+      acc[r][q] = make_float2(0.f, 0.f);
+    }
+    auto rhs = [&](const float* v, int c) { return i < A.n && c < A.cols ? v[c * A.n + i] : 0.f; };
+#pragma unroll
+    for (int c = 0; c < T / 2; ++c) {
+      ai[r][c] = make_float2(rhs(A.a, 2 * c), rhs(A.a, 2 * c + 1));
+      bi[r][c] = make_float2(rhs(A.b, 2 * c), rhs(A.b, 2 * c + 1));
+    }
+  }
+  const int64_t tiles = (A.n + kIgTile - 1) / kIgTile;
+  // Columns past n carry zero a and b, so they add psi * 0.
+  constexpr int PER = (kIgTile * W + kIgThreads - 1) / kIgThreads;
+  float next[PER];
+  auto load = [&](int64_t t) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int q = threadIdx.x + u * kIgThreads;
+      const int f = q / kIgTile;
+      const int64_t j = t * kIgTile + q % kIgTile;
+      float v = 0.f;
+      if (t < tiles && j < A.n) {
+        if (f < D)
+          v = -ig_coord<LEAF>(A, j, f);
+        else if (f < D + T)
+          v = f - D < A.cols ? A.b[(int64_t)(f - D) * A.n + j] : 0.f;
+        else if (f < W)
+          v = f - D - T < A.cols ? A.a[(int64_t)(f - D - T) * A.n + j] : 0.f;
+      }
+      next[u] = v;
+    }
+  };
+  load(blockIdx.y);
+  int buf = 0;
+  for (int64_t t = blockIdx.y; t < tiles; t += kIgCluster, buf ^= 1) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int q = threadIdx.x + u * kIgThreads;
+      if (q < kIgTile * W) tile[buf][(q % kIgTile) * W + q / kIgTile] = next[u];
+    }
+    __syncthreads();
+    load(t + kIgCluster);
+    // The tile's own sums first: fewer terms per running sum, half the rounding error.
+    float2 part[R][D2];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int q = 0; q < D2; ++q) part[r][q] = make_float2(0.f, 0.f);
+#pragma unroll 2
+    for (int j = 0; j < kIgTile; ++j) {
+      const float2* col = reinterpret_cast<const float2*>(tile[buf] + j * W);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float2 diff[D2], s = make_float2(0.f, 0.f), g = make_float2(0.f, 0.f);
+        ig_diff<LEAF, D2>(A, xi[r], col, diff);
+#pragma unroll
+        for (int q = 0; q < D2; ++q) s = __ffma2_rn(diff[q], diff[q], s);
+#pragma unroll
+        for (int c = 0; c < T / 2; ++c) {
+          g = __ffma2_rn(ai[r][c], col[D2 + c], g);
+          g = __ffma2_rn(bi[r][c], col[D2 + T / 2 + c], g);
+        }
+        const float w = (g.x + g.y) * pair_psi<LEAF>(s.x + s.y, A);
+        const float2 w2 = make_float2(w, w);
+#pragma unroll
+        for (int q = 0; q < D2; ++q) part[r][q] = __ffma2_rn(w2, diff[q], part[r][q]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int q = 0; q < D2; ++q) acc[r][q] = __fadd2_rn(acc[r][q], part[r][q]);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int q = 0; q < D2; ++q) {
+      sums[(r * kIgThreads + threadIdx.x) * D + 2 * q] = acc[r][q].x;
+      sums[(r * kIgThreads + threadIdx.x) * D + 2 * q + 1] = acc[r][q].y;
+    }
+  ig_join<D, 1>(A, sums, R * kIgThreads, (int64_t)blockIdx.x * (kIgThreads * R));
+}
+
+// ------------------------------------------------------- tensor-core G
+// 8 warps run the pairs (TMEM lane quadrant = warp % 4, two warps share a tile's columns), 4 warps
+// split a and b of the next 128 columns into bf16 planes and issue its 12 MMAs; two tiles are in
+// flight, each with its own operand planes, coordinates and 128 TMEM columns.
+constexpr int kIgcThreads = 384;
+constexpr int kIgcCols = 128;
+constexpr int kIgcPlane = 128 * 32 * 2;       // bytes: 128 points, depth 32, 16-bit
+constexpr int kIgcOperand = 3 * kIgcPlane;
+
+// Byte offset of (point p, depth 8 q) in a plane: 8-point x 16-byte core matrices, points adjacent
+// at 128 bytes, depth at 2048.
+__device__ __forceinline__ int igc_offset(int p, int q) {
+  return q * 2048 + (p >> 3) * 128 + (p & 7) * 16;
+}
+
+// Depth 8 q .. 8 q + 7 of one point: right-hand sides 8 (q % 2) .. of `lo` (q < 2) or `hi`, which
+// point at the point's column 0. Each value is the exact sum of three bf16 parts (rounded to nearest);
+// one past bf16's range or not finite makes its products NaN.
+__device__ __forceinline__ void igc_split(const InputGradArgs& A, const float* lo, const float* hi,
+                                          bool in, int q, int p, char* planes) {
+  const int c0 = (q & 1) * 8;
+  const float* v = (q < 2 ? lo : hi) + c0 * A.n;
+  float2 x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i].x = in && c0 + 2 * i < A.cols ? *v : 0.f;
+    v += A.n;
+    x[i].y = in && c0 + 2 * i + 1 < A.cols ? *v : 0.f;
+    v += A.n;
+  }
+  char* dst = planes + igc_offset(p, q);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = bits32(__float22bfloat162_rn(x[i]));
+      x[i].x -= __uint_as_float(h[i] << 16);
+      x[i].y -= __uint_as_float(h[i] & 0xFFFF0000u);
+    }
+    *reinterpret_cast<uint4*>(dst + k * kIgcPlane) = make_uint4(h[0], h[1], h[2], h[3]);
+  }
+}
+
+__device__ __forceinline__ void igc_load(uint32_t addr, uint32_t (&r)[16]) { tmem_ld16_async(addr, r); }
+__device__ __forceinline__ void igc_load(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <int D>
+struct IgcShape {
+  static constexpr int kCoords = kIgcCols * D * 4;
+  static constexpr int kSmem = 3 * kIgcOperand + 2 * kCoords;  // rows, two column tiles
+  // The join's sums [2][128][D] reuse the column tiles.
+  static_assert(2 * 128 * D * 4 <= 2 * kIgcOperand + 2 * kCoords, "join fits");
+  static constexpr int kBlocks = D <= 8 ? 2 : 1;    // per SM (registers)
+  static constexpr int kChunk = D <= 16 ? 16 : 4;   // columns per TMEM load
+};
+
+template <int LEAF, int D>
+__global__ void __cluster_dims__(1, kIgCluster, 1)
+    __launch_bounds__(kIgcThreads, IgcShape<D>::kBlocks)
+        input_gradient_tc_kernel(const __grid_constant__ InputGradArgs A) {
+  constexpr int D2 = D / 2, CH = IgcShape<D>::kChunk;
+  extern __shared__ __align__(128) char ig_smem[];
+  char* row_planes = ig_smem;
+  char* col_planes = ig_smem + kIgcOperand;
+  float* coords = reinterpret_cast<float*>(ig_smem + 3 * kIgcOperand);
+  __shared__ __align__(8) uint64_t full[2], empty[2];
+  __shared__ uint32_t tmem_base;
+  __shared__ int failed;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&full[s], 4 + 1);  // the producer warps and the MMAs' completion
+      mbar_init(&empty[s], 8);
+    }
+    fence_barrier_init();
+    failed = 0;
+  }
+  if (warp == 8) tmem_alloc(&tmem_base, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  const int64_t row0 = (int64_t)blockIdx.x * 128;
+  const int64_t tiles = (A.n + kIgcCols - 1) / kIgcCols;
+  const int mine = blockIdx.y < tiles ? (int)((tiles - blockIdx.y + kIgCluster - 1) / kIgCluster) : 0;
+  float2 acc[D2];
+#pragma unroll
+  for (int q = 0; q < D2; ++q) acc[q] = make_float2(0.f, 0.f);
+
+  if (warp >= 8) {
+    const int p = threadIdx.x - 256;
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q)
+      igc_split(A, A.a + row0 + p, A.b + row0 + p, row0 + p < A.n, q, p, row_planes);
+    constexpr uint32_t idesc = gg_idesc(true, false, false, kIgcCols);
+    bool ok = true;
+    for (int t = 0; t < mine; ++t) {
+      const int s = t & 1;
+      const int64_t j = ((int64_t)blockIdx.y + (int64_t)t * kIgCluster) * kIgcCols + p;
+      if (t >= 2) ok = mbar_wait_bounded(&empty[s], ((t >> 1) & 1) ^ 1);
+      // The four warps stay together: a wait that ran out in one ends all of them.
+      if (!ok) failed = 1;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (*(volatile int*)&failed) break;
+      char* planes = col_planes + s * kIgcOperand;
+#pragma unroll 1
+      for (int q = 0; q < 4; ++q) igc_split(A, A.b + j, A.a + j, j < A.n, q, p, planes);
+      float* x = coords + (s * kIgcCols + p) * D;
+#pragma unroll 1
+      for (int f = 0; f < D; ++f) x[f] = -ig_coord<LEAF>(A, j, f);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[s]);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (threadIdx.x == 256) {
+        tc_fence_after();
+        const uint32_t d = tmem + s * kIgcCols;
+        uint64_t da[3], db[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          da[k] = make_smem_desc(row_planes + k * kIgcPlane, 2048, 128);
+          db[k] = make_smem_desc(planes + k * kIgcPlane, 2048, 128);
+        }
+        constexpr uint32_t next = 4096 >> 4;  // 16 deeper
+        // Small products first: the accumulator truncates, and only the last two MMAs are large.
+        gg_mma(d, da[2], db[0], idesc, 0);
+        gg_mma(d, da[2] + next, db[0] + next, idesc, 1);
+        gg_mma(d, da[1], db[1], idesc, 1);
+        gg_mma(d, da[1] + next, db[1] + next, idesc, 1);
+        gg_mma(d, da[0], db[2], idesc, 1);
+        gg_mma(d, da[0] + next, db[2] + next, idesc, 1);
+        gg_mma(d, da[1], db[0], idesc, 1);
+        gg_mma(d, da[1] + next, db[0] + next, idesc, 1);
+        gg_mma(d, da[0], db[1], idesc, 1);
+        gg_mma(d, da[0] + next, db[1] + next, idesc, 1);
+        gg_mma(d, da[0], db[0], idesc, 1);
+        gg_mma(d, da[0] + next, db[0] + next, idesc, 1);
+        mma_commit(&full[s]);
+      }
+    }
+    if (!ok) atomicExch(A.err, DEV_WAIT_TIMEOUT);
+  } else {
+    const int quad = warp & 3, half = warp >> 2;
+    const int64_t i = row0 + quad * 32 + lane;
+    float2 xi[D2];
+#pragma unroll
+    for (int q = 0; q < D2; ++q)
+      xi[q] = make_float2(ig_coord<LEAF>(A, i, 2 * q), ig_coord<LEAF>(A, i, 2 * q + 1));
+    bool ok = true;
+    for (int t = 0; t < mine; ++t) {
+      const int s = t & 1;
+      ok = mbar_wait_bounded(&full[s], (t >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t g_addr = tmem + s * kIgcCols + ((uint32_t)quad << 21) + half * 64;
+      const float* x = coords + (s * kIgcCols + half * 64) * D;
+#pragma unroll 1
+      for (int c = 0; c < 64; c += CH) {
+        uint32_t g[CH];
+        igc_load(g_addr + c, g);
+        tmem_wait_ld();
+        // These columns' own sums first: fewer terms per running sum, less rounding error.
+        float2 part[D2];
+#pragma unroll
+        for (int q = 0; q < D2; ++q) part[q] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+          const float2* col = reinterpret_cast<const float2*>(x + (c + k) * D);
+          float2 sq = make_float2(0.f, 0.f);
+          if constexpr (D <= 16) {
+            float2 diff[D2];
+            ig_diff<LEAF, D2>(A, xi, col, diff);
+#pragma unroll
+            for (int q = 0; q < D2; ++q) sq = __ffma2_rn(diff[q], diff[q], sq);
+            const float w = __uint_as_float(g[k]) * pair_psi<LEAF>(sq.x + sq.y, A);
+            const float2 w2 = make_float2(w, w);
+#pragma unroll
+            for (int q = 0; q < D2; ++q) part[q] = __ffma2_rn(w2, diff[q], part[q]);
+          } else {
+            // The differences twice, eight at a time: together they would not fit the registers.
+#pragma unroll
+            for (int q = 0; q < D2; ++q) {
+              float2 diff = __fadd2_rn(xi[q], col[q]);
+              if constexpr (LEAF == GPB_KERNEL_MATERN12)
+                diff = __fmul2_rn(diff, make_float2(A.scale[2 * q], A.scale[2 * q + 1]));
+              sq = __ffma2_rn(diff, diff, sq);
+            }
+            const float w = __uint_as_float(g[k]) * pair_psi<LEAF>(sq.x + sq.y, A);
+            const float2 w2 = make_float2(w, w);
+#pragma unroll
+            for (int q = 0; q < D2; ++q) {
+              float2 diff = __fadd2_rn(xi[q], col[q]);
+              if constexpr (LEAF == GPB_KERNEL_MATERN12)
+                diff = __fmul2_rn(diff, make_float2(A.scale[2 * q], A.scale[2 * q + 1]));
+              acc[q] = __ffma2_rn(w2, diff, acc[q]);
+            }
+          }
+        }
+        if constexpr (D <= 16)
+#pragma unroll
+          for (int q = 0; q < D2; ++q) acc[q] = __fadd2_rn(acc[q], part[q]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+    }
+    if (!ok) atomicExch(A.err, DEV_WAIT_TIMEOUT);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 256);
+  float* sums = reinterpret_cast<float*>(col_planes);  // [2][128][D]
+  if (warp < 8) {
+    float* o = sums + ((warp >> 2) * 128 + (warp & 3) * 32 + lane) * D;
+#pragma unroll
+    for (int q = 0; q < D2; ++q) {
+      o[2 * q] = acc[q].x;
+      o[2 * q + 1] = acc[q].y;
+    }
+  }
+  ig_join<D, 2>(A, sums, 128, row0);
 }
 
 // -------------------------------------------------------- any kernel tree
@@ -174,13 +462,18 @@ __device__ __noinline__ void leaf_input_grad(const DevKernel& K, const LeafDesc&
       const float dk = (xi[L.dims[k]] - xj[L.dims[k]]) / p[L.ard ? k : 0];
       s = fmaf(dk, dk, s);
     }
+    const float r = sqrtf(fmaxf(s, 1e-20f));
     float psi;
     switch (L.type) {
-      case GPB_KERNEL_RBF: psi = leaf_psi<GPB_KERNEL_RBF>(s, 0.f, 0); break;
-      case GPB_KERNEL_MATERN12: psi = leaf_psi<GPB_KERNEL_MATERN12>(s, 0.f, L.ard); break;
-      case GPB_KERNEL_MATERN32: psi = leaf_psi<GPB_KERNEL_MATERN32>(s, 0.f, 0); break;
-      case GPB_KERNEL_MATERN52: psi = leaf_psi<GPB_KERNEL_MATERN52>(s, 0.f, 0); break;
-      default: psi = leaf_psi<GPB_KERNEL_RQ>(s, p[nl], 0);
+      case GPB_KERNEL_RBF: psi = expf(-0.5f * s); break;
+      case GPB_KERNEL_MATERN12: psi = expf(L.ard ? fmaxf(-r, -20.f) : -r) / r; break;
+      case GPB_KERNEL_MATERN32: psi = 3.f * expf(fmaxf(-1.7320508075688772f * r, -20.f)); break;
+      case GPB_KERNEL_MATERN52: {
+        const float r5 = 2.23606797749979f * r;
+        psi = (5.f / 3.f) * (1.f + r5) * expf(fmaxf(-r5, -20.f));
+        break;
+      }
+      default: psi = powf(1.f + s / (2.f * p[nl]), -p[nl] - 1.f);
     }
     const float os = p[L.type == GPB_KERNEL_RQ ? nl + 1 : nl];
     for (int k = 0; k < nd; ++k) {
@@ -275,31 +568,31 @@ __global__ void __launch_bounds__(128) input_gradient_tree_kernel(
 }
 
 // ------------------------------------------------------------------ host
-template <int LEAF, int D, int T>
-static int launch_ig(const InputGradArgs& A, cudaStream_t st) {
-  // Two rows per thread where their state (2 D + 2 T values a row) fits the registers.
-  constexpr int R = D <= 16 ? 2 : 1;
-  const size_t smem = (size_t)R * kIgThreads * D * sizeof(float);
-  const unsigned gx = (unsigned)ceil_div(A.n, R * kIgThreads);
-  input_gradient_kernel<LEAF, D, T, R><<<dim3(gx, kIgCluster), kIgThreads, smem, st>>>(A);
+template <int LEAF, int D>
+static int launch_ig(InputGradArgs& A, cudaStream_t st) {
+  if (A.cols > 4) {
+    constexpr auto kernel = input_gradient_tc_kernel<LEAF, D>;
+    GPB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        IgcShape<D>::kSmem));
+    kernel<<<dim3((unsigned)ceil_div(A.n, 128), kIgCluster), kIgcThreads, IgcShape<D>::kSmem, st>>>(A);
+  } else {
+    constexpr int R = D <= 16 ? 2 : 1;  // a row's state is 2 D + 8 values
+    const size_t smem = (size_t)R * kIgThreads * D * sizeof(float);
+    input_gradient_kernel<LEAF, D, R>
+        <<<dim3((unsigned)ceil_div(A.n, R * kIgThreads), kIgCluster), kIgThreads, smem, st>>>(A);
+  }
   GPB_CHECK_CUDA(cudaGetLastError());
   return GPB_OK;
 }
 
-template <int LEAF, int T>
-static int launch_ig_d(const InputGradArgs& A, cudaStream_t st) {
-  if (A.nd <= 1) return launch_ig<LEAF, 1, T>(A, st);
-  if (A.nd <= 2) return launch_ig<LEAF, 2, T>(A, st);
-  if (A.nd <= 4) return launch_ig<LEAF, 4, T>(A, st);
-  if (A.nd <= 8) return launch_ig<LEAF, 8, T>(A, st);
-  if (A.nd <= 16) return launch_ig<LEAF, 16, T>(A, st);
-  if (A.nd <= 32) return launch_ig<LEAF, 32, T>(A, st);
-  return launch_ig<LEAF, 64, T>(A, st);
-}
-
 template <int LEAF>
-static int launch_ig_t(const InputGradArgs& A, cudaStream_t st) {
-  return A.cols <= 4 ? launch_ig_d<LEAF, 4>(A, st) : launch_ig_d<LEAF, 16>(A, st);
+static int launch_ig_d(InputGradArgs& A, cudaStream_t st) {
+  if (A.nd <= 2) return launch_ig<LEAF, 2>(A, st);
+  if (A.nd <= 4) return launch_ig<LEAF, 4>(A, st);
+  if (A.nd <= 8) return launch_ig<LEAF, 8>(A, st);
+  if (A.nd <= 16) return launch_ig<LEAF, 16>(A, st);
+  if (A.nd <= 32) return launch_ig<LEAF, 32>(A, st);
+  return launch_ig<LEAF, 64>(A, st);
 }
 
 int provider_input_gradient(gpb_provider* p, float* out, const float* a, const float* b,
@@ -324,13 +617,24 @@ int provider_input_gradient(gpb_provider* p, float* out, const float* a, const f
   A.n = p->n;
   A.d = p->d;
   A.nd = L.ndims;
-  A.os = L.type == GPB_KERNEL_RQ ? prm[nl + 1] : prm[nl];
-  A.alpha = L.type == GPB_KERNEL_RQ ? prm[nl] : 0.f;
-  if (K.nnodes == 2) A.os *= K.params[K.node_arg[1]];
+  double os = L.type == GPB_KERNEL_RQ ? prm[nl + 1] : prm[nl];
+  if (K.nnodes == 2) os *= K.params[K.node_arg[1]];
+  // Input scale beyond 1 / l, and psi's constant factor.
+  double c = 1.0, factor = 1.0;
+  switch (L.type) {
+    case GPB_KERNEL_RBF: c = std::sqrt(0.5 / std::log(2.0)); break;
+    case GPB_KERNEL_MATERN32: c = std::sqrt(3.0), factor = 3.0; break;
+    case GPB_KERNEL_MATERN52: c = std::sqrt(5.0), factor = 5.0 / 3.0; break;
+    case GPB_KERNEL_RQ: c = std::sqrt(0.5 / (double)prm[nl]), A.power = prm[nl] + 1.f; break;
+    default: break;
+  }
   A.clamp12 = L.ard;
+  A.err = p->err_d;
   for (int q = 0; q < L.ndims; ++q) {
     A.dims[q] = L.dims[q];
-    A.inv_l[q] = 1.f / prm[L.ard ? q : 0];
+    const double l = prm[L.ard ? q : 0];
+    A.scale[q] = (float)(c / l);
+    A.out_scale[q] = (float)(os * factor / (c * l));
   }
   for (int64_t c = 0; c < ncols; c += 16) {
     A.a = a + c * p->n;
@@ -339,11 +643,11 @@ int provider_input_gradient(gpb_provider* p, float* out, const float* a, const f
     A.accumulate = c > 0;
     int s;
     switch (L.type) {
-      case GPB_KERNEL_RBF: s = launch_ig_t<GPB_KERNEL_RBF>(A, st); break;
-      case GPB_KERNEL_MATERN12: s = launch_ig_t<GPB_KERNEL_MATERN12>(A, st); break;
-      case GPB_KERNEL_MATERN32: s = launch_ig_t<GPB_KERNEL_MATERN32>(A, st); break;
-      case GPB_KERNEL_MATERN52: s = launch_ig_t<GPB_KERNEL_MATERN52>(A, st); break;
-      default: s = launch_ig_t<GPB_KERNEL_RQ>(A, st);
+      case GPB_KERNEL_RBF: s = launch_ig_d<GPB_KERNEL_RBF>(A, st); break;
+      case GPB_KERNEL_MATERN12: s = launch_ig_d<GPB_KERNEL_MATERN12>(A, st); break;
+      case GPB_KERNEL_MATERN32: s = launch_ig_d<GPB_KERNEL_MATERN32>(A, st); break;
+      case GPB_KERNEL_MATERN52: s = launch_ig_d<GPB_KERNEL_MATERN52>(A, st); break;
+      default: s = launch_ig_d<GPB_KERNEL_RQ>(A, st);
     }
     GPB_TRY(s);
   }
