@@ -282,6 +282,7 @@ static int make_map(const Operand& o, int box_rows, CUtensorMap* map) {
 struct GatedPlan {
   bool few = false;                    // CUDA-core path
   int planes = 1;                      // of packed x and weights
+  int planes_d = 1;                    // of dgate and dup
   int64_t ldk = 0, ldn = 0;            // leading dimensions of packed operands and of dgate / dup
   int64_t x = 0, wg = 0, wu = 0;       // packed operands
   int64_t dg = 0, du = 0, plane_d = 0; // dgate and dup (elements between planes)
@@ -297,6 +298,12 @@ static int64_t take(int64_t& at, int64_t bytes) {
   at += round_up(bytes, 256);
   return o;
 }
+
+// 16-bit dgate and dup are kept as two planes (16 and more significant bits) up to this many
+// multiply-adds per product, as one above. One plane's rounding adds to the outputs' own: 1.4 times
+// their error, and more where few terms or few outputs average it. The second plane doubles the MMAs
+// of three of the four products: KTWO_NOTE
+constexpr int64_t kTwoPlanes = (int64_t)1 << 31;
 
 // Column tile of a GG_DX / GG_DW product with n output columns.
 static int plain_tile(int64_t n, bool f32) { return n <= 64 ? 64 : n <= 128 || f32 ? 128 : 256; }
@@ -327,9 +334,10 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
   P.wg = take(at, P.planes * outer * P.ldk * 2);
   P.wu = take(at, P.planes * outer * P.ldk * 2);
   if (backward) {
+    P.planes_d = f32 ? 3 : rows * inner * outer <= kTwoPlanes ? 2 : 1;
     P.plane_d = rows * P.ldn;
-    P.dg = take(at, P.planes * P.plane_d * 2);
-    P.du = take(at, P.planes * P.plane_d * 2);
+    P.dg = take(at, P.planes_d * P.plane_d * 2);
+    P.du = take(at, P.planes_d * P.plane_d * 2);
     P.tile_n = plain_tile(inner, f32);
     const int64_t tiles = (outer <= 64 ? 1 : 2 * ceil_div(outer, kGgBM)) * ceil_div(inner, P.tile_n);
     const int64_t kb = ceil_div(rows, kGgBK);
@@ -382,7 +390,7 @@ static int gated_operand(const void* p, int64_t rows, int64_t cols, int64_t ld, 
   return GPB_OK;
 }
 
-template <typename T, typename D, int PL, bool BACK>
+template <typename T, typename D, int PL, int PD, bool BACK>
 static int gated_project(const GatedArgs& A, const Operand& x, const Operand& wg, const Operand& wu,
                          GgArgs G, cudaStream_t st) {
   const int nb = proj_tile(A.outer, PL == 3);
@@ -404,27 +412,27 @@ static int gated_project(const GatedArgs& A, const Operand& x, const Operand& wg
   G.dout = A.dout;
   G.dout_ld = A.dout_ld;
   switch (nb) {
-    case 64: return gg_launch<GG_PROJ, 64, PL, PL, T, D, PL, BACK>(mx, mx, mg, mu, G, st);
-    case 128: return gg_launch<GG_PROJ, 128, PL, PL, T, D, PL, BACK>(mx, mx, mg, mu, G, st);
+    case 64: return gg_launch<GG_PROJ, 64, PL, PL, T, D, PD, BACK>(mx, mx, mg, mu, G, st);
+    case 128: return gg_launch<GG_PROJ, 128, PL, PL, T, D, PD, BACK>(mx, mx, mg, mu, G, st);
     default:
       if constexpr (PL == 1)
-        return gg_launch<GG_PROJ, 256, PL, PL, T, D, PL, BACK>(mx, mx, mg, mu, G, st);
+        return gg_launch<GG_PROJ, 256, PL, PL, T, D, PD, BACK>(mx, mx, mg, mu, G, st);
       return GPB_ERR_UNSUPPORTED;
   }
 }
 
-template <int MODE, typename T, typename D, int PL>
+template <int MODE, typename T, typename D, int PL, int PD>
 static int gated_plain(const CUtensorMap& a0, const CUtensorMap& a1, const Operand& b0,
                        const Operand& b1, int nb, GgArgs& G, cudaStream_t st) {
   CUtensorMap m0, m1;
   GPB_TRY(make_map(b0, kGgBK, &m0));
   GPB_TRY(make_map(b1, kGgBK, &m1));
   switch (nb) {
-    case 64: return gg_launch<MODE, 64, PL, PL, T, D, PL, false>(a0, a1, m0, m1, G, st);
-    case 128: return gg_launch<MODE, 128, PL, PL, T, D, PL, false>(a0, a1, m0, m1, G, st);
+    case 64: return gg_launch<MODE, 64, PD, PL, T, D, PD, false>(a0, a1, m0, m1, G, st);
+    case 128: return gg_launch<MODE, 128, PD, PL, T, D, PD, false>(a0, a1, m0, m1, G, st);
     default:
       if constexpr (PL == 1)
-        return gg_launch<MODE, 256, PL, PL, T, D, PL, false>(a0, a1, m0, m1, G, st);
+        return gg_launch<MODE, 256, PD, PL, T, D, PD, false>(a0, a1, m0, m1, G, st);
       return GPB_ERR_UNSUPPORTED;
   }
 }
@@ -504,19 +512,13 @@ static int gated_forward(const GatedArgs& A, char* ws, const GatedPlan& P, cudaS
   G.out[0] = A.out;
   G.out_ld = A.out_ld;
   G.vec = aligned16(A.out) && A.out_ld % V == 0;
-  return gated_project<T, D, PL, false>(A, x, wg, wu, G, st);
+  return gated_project<T, D, PL, PL, false>(A, x, wg, wu, G, st);
 }
 
-template <typename T, typename D, int PL>
-static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, const GatedPlan& P,
+template <typename T, typename D, int PL, int PD>
+static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, const GatedPlan& P,
                           cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  if (P.few) {
-    const bool vec = gated_vec<T>(A) && (!(R.dwg || R.dwu) || R.dw_ld % V == 0) &&
-                     aligned16(R.dwg) && aligned16(R.dwu);
-    return vec ? gated_rows_backward<T, V>(A, R, P, ws, st)
-               : gated_rows_backward<T, 1>(A, R, P, ws, st);
-  }
   Operand x, wg, wu;
   GPB_TRY((gated_operand<T, D>(A.x, A.rows, A.inner, A.x_ld, P, ws + P.x, &x, st)));
   GPB_TRY((gated_operand<T, D>(A.wg, A.outer, A.inner, A.w_ld, P, ws + P.wg, &wg, st)));
@@ -528,7 +530,7 @@ static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, con
   dg.rows = du.rows = A.rows;
   dg.cols = du.cols = A.outer;
   dg.ld = du.ld = P.ldn;
-  dg.planes = du.planes = PL;
+  dg.planes = du.planes = PD;
   dg.plane = du.plane = P.plane_d;
   {
     GgArgs G{};
@@ -538,7 +540,7 @@ static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, con
     G.plane = P.plane_d;
     G.vec = aligned16(A.dout) && A.dout_ld % V == 0;
     if (R.dbg || R.dbu) G.col_sums = (float*)(ws + P.sums);
-    GPB_TRY((gated_project<T, D, PL, true>(A, x, wg, wu, G, st)));
+    GPB_TRY((gated_project<T, D, PL, PD, true>(A, x, wg, wu, G, st)));
   }
   if (R.dx) {
     GgArgs G{};
@@ -557,7 +559,7 @@ static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, con
     CUtensorMap a0, a1;
     GPB_TRY(make_map(dg, kGgBM, &a0));
     GPB_TRY(make_map(du, kGgBM, &a1));
-    GPB_TRY((gated_plain<GG_DX, T, D, PL>(a0, a1, wg, wu, nb, G, st)));
+    GPB_TRY((gated_plain<GG_DX, T, D, PL, PD>(a0, a1, wg, wu, nb, G, st)));
   }
   if (R.dwg || R.dwu) {
     GgArgs G{};
@@ -579,7 +581,7 @@ static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, con
     CUtensorMap a0, a1;
     GPB_TRY(make_map(dg, kGgBK, &a0));
     GPB_TRY(make_map(du, kGgBK, &a1));
-    GPB_TRY((gated_plain<GG_DW, T, D, PL>(a0, a1, x, x, P.tile_n, G, st)));
+    GPB_TRY((gated_plain<GG_DW, T, D, PL, PD>(a0, a1, x, x, P.tile_n, G, st)));
     if (P.splits > 1) {
       mm_join_kernel<T><<<(unsigned)ceil_div(2 * A.outer * A.inner, 256), 256, 0, st>>>(
           partial, P.splits, A.outer, A.inner, 2, (T*)R.dwg, (T*)R.dwu, R.dw_ld);
@@ -592,6 +594,21 @@ static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, con
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   return GPB_OK;
+}
+
+template <typename T, typename D, int PL>
+static int gated_backward(const GatedArgs& A, const GatedGrads& R, char* ws, const GatedPlan& P,
+                          cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  if (P.few) {
+    const bool vec = gated_vec<T>(A) && (!(R.dwg || R.dwu) || R.dw_ld % V == 0) &&
+                     aligned16(R.dwg) && aligned16(R.dwu);
+    return vec ? gated_rows_backward<T, V>(A, R, P, ws, st)
+               : gated_rows_backward<T, 1>(A, R, P, ws, st);
+  }
+  if constexpr (PL == 1)
+    if (P.planes_d == 2) return gated_backward_tc<T, D, 1, 2>(A, R, ws, P, st);
+  return gated_backward_tc<T, D, PL, PL>(A, R, ws, P, st);
 }
 
 static int gated_check(int32_t dtype, int64_t rows, int64_t inner, int64_t outer) {

@@ -370,7 +370,7 @@ __device__ __forceinline__ void gg_plain_store(const GgArgs& A, const GgItem& I,
 }
 
 // T: the caller's element type; D: the operands' 16-bit type; PA, PB: planes of the two operands;
-// PD: planes of dgate and dup that a backward GG_PROJ writes.
+// PD: planes of dgate and dup that a backward GG_PROJ writes (their products take PA = PD).
 template <int MODE, int NB, int PA, int PB, typename T, typename D, int PD, bool BACK>
 __global__ void __launch_bounds__(kGgThreads, 1)
     gated_gemm_kernel(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,

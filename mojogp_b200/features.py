@@ -40,80 +40,91 @@ def _dtype_code(dtype) -> int:
     return code
 
 
-class _View:
-    """Pointer, sizes, leading dimension, element type and device of an array."""
-
-    __slots__ = ("ptr", "shape", "ld", "code", "device")
-
-    def __init__(self, a, name: str, ndim: int):
-        self.shape = shape = a.shape
-        if len(shape) != ndim:
-            raise ValueError(f"{name} must be {ndim}-D, got shape {shape}")
-        try:
-            self.ptr = a.data_ptr()
-        except AttributeError:
-            if not (hasattr(a, "ptr") and hasattr(a, "nbytes")):
-                raise ValueError(f"{name} must be a device array, got {type(a).__name__}") from None
-            self.ptr, self.device, self.ld = a.ptr, a.device, shape[-1]
-            self.code = _element_code(a)
-            if self.ptr is None:
-                raise ValueError(f"{name} was freed") from None
-            return
-        self.device = index = a.device.index
-        if index is None or a.device.type != "cuda":
-            raise ValueError(f"{name} must be on a CUDA device, got {a.device}")
-        strides = a.stride()
-        if strides[-1] != 1 and shape[-1] > 1:
-            raise ValueError(f"{name} must have unit column stride, got strides {strides}")
-        self.ld = strides[0] if ndim == 2 and shape[0] > 1 else shape[-1]
-        dtype = a.dtype
-        self.code = _CODES[dtype] if dtype in _CODES else _dtype_code(dtype)
-
-
 def _element_code(a) -> int:
     return _dtype_code(getattr(a, "element_type", None) or a.dtype)
 
 
-def _vector(a, name: str, size: int, like: "_View", code: int) -> int | None:
-    """Pointer of a [size] vector of element type `code`, or None."""
+def _where(a, name: str) -> tuple:
+    """(pointer, device, strides) of a device array; a DeviceBuffer is contiguous."""
+    try:
+        ptr = a.data_ptr()
+    except AttributeError:
+        if not (hasattr(a, "ptr") and hasattr(a, "nbytes")):
+            raise ValueError(f"{name} must be a device array, got {type(a).__name__}") from None
+        if a.ptr is None:
+            raise ValueError(f"{name} was freed") from None
+        return a.ptr, a.device, None
+    device = a.device.index
+    if device is None or a.device.type != "cuda":
+        raise ValueError(f"{name} must be on a CUDA device, got {a.device}")
+    return ptr, device, a.stride()
+
+
+def _matrix(a, name: str, rows: int = -1, cols: int = -1, code: int = -1, device: int = -1) -> tuple:
+    """(pointer, rows, columns, leading dimension, type, device) of a matrix; sizes, type and
+    device that are given (not -1) have to agree."""
+    ptr, dev, strides = _where(a, name)
+    shape = a.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} must be 2-D, got shape {tuple(shape)}")
+    r, c = shape
+    if rows >= 0 and (r != rows or c != cols):
+        raise ValueError(f"{name} must have shape ({rows}, {cols}), got {tuple(shape)}")
+    ld = c
+    if strides is not None:
+        if strides[1] != 1 and c > 1:
+            raise ValueError(f"{name} must have unit column stride, got strides {strides}")
+        if r > 1:
+            ld = strides[0]
+        dtype = a.dtype
+        kind = _CODES[dtype] if dtype in _CODES else _dtype_code(dtype)
+    else:
+        kind = _element_code(a)
+    if code >= 0:
+        if kind != code:
+            raise ValueError(f"{name} has a different element type")
+        if dev != device:
+            raise ValueError(f"{name} is on device {dev}, expected {device}")
+    return ptr, r, c, ld, kind, dev
+
+
+def _vector(a, name: str, size: int, code: int, device: int) -> int | None:
+    """Pointer of a [size] vector of element type `code` on `device`, or None."""
     if a is None:
         return None
-    v = _View(a, name, 1)
-    if v.shape[0] != size:
-        raise ValueError(f"{name} must have {size} entries, got {v.shape[0]}")
-    if v.code != code:
+    ptr, dev, strides = _where(a, name)
+    shape = a.shape
+    if len(shape) != 1:
+        raise ValueError(f"{name} must be 1-D, got shape {tuple(shape)}")
+    if shape[0] != size:
+        raise ValueError(f"{name} must have {size} entries, got {shape[0]}")
+    if strides is not None:
+        if strides[0] != 1 and size > 1:
+            raise ValueError(f"{name} must have unit stride, got {strides}")
+        dtype = a.dtype
+        kind = _CODES[dtype] if dtype in _CODES else _dtype_code(dtype)
+    else:
+        kind = _element_code(a)
+    if kind != code:
         raise ValueError(f"{name} has a different element type")
-    if v.device != like.device:
-        raise ValueError(f"{name} is on device {v.device}, expected {like.device}")
-    return v.ptr
+    if dev != device:
+        raise ValueError(f"{name} is on device {dev}, expected {device}")
+    return ptr
 
 
-def _matrix(a, name: str, shape: tuple, like: "_View") -> "_View":
-    v = _View(a, name, 2)
-    if v.shape != shape:
-        raise ValueError(f"{name} must have shape {shape}, got {v.shape}")
-    if v.code != like.code:
-        raise ValueError(f"{name} has a different element type")
-    if v.device != like.device:
-        raise ValueError(f"{name} is on device {v.device}, expected {like.device}")
-    return v
-
-
-def _workspace(a, like: "_View") -> tuple:
+def _workspace(a, device: int) -> tuple:
     """(pointer, bytes) of a scratch array; the call itself checks the size."""
     if a is None:
         return None, 0
-    data_ptr = getattr(a, "data_ptr", None)
-    if data_ptr is not None:
-        if a.device.type != "cuda":
-            raise ValueError(f"workspace must be on a CUDA device, got {a.device}")
-        if not a.is_contiguous():
-            raise ValueError("workspace must be contiguous")
-        ptr, size, device = data_ptr(), a.numel() * a.element_size(), a.device.index
+    ptr, dev, strides = _where(a, "workspace")
+    if strides is None:
+        size = a.nbytes
+    elif a.is_contiguous():
+        size = a.numel() * a.element_size()
     else:
-        ptr, size, device = a.ptr, a.nbytes, a.device
-    if device != like.device:
-        raise ValueError(f"workspace is on device {device}, expected {like.device}")
+        raise ValueError("workspace must be contiguous")
+    if dev != device:
+        raise ValueError(f"workspace is on device {dev}, expected {device}")
     return ptr, size
 
 
@@ -135,20 +146,18 @@ def layer_norm(out, x, weight=None, bias=None, *, eps: float = 1e-5, mean=None, 
     weight and bias [columns] are float32 or of x's type; `mean` and `rstd`
     [rows], float32, are written where given (the backward pass needs them).
     out may be x itself."""
-    xv = _View(x, "x", 2)
-    rows, cols = xv.shape
-    ov = _matrix(out, "out", xv.shape, xv)
-    pcode = xv.code
+    xp, rows, cols, x_ld, code, dev = _matrix(x, "x")
+    op, _, _, out_ld, _, _ = _matrix(out, "out", rows, cols, code, dev)
+    pcode = code
     for a in (weight, bias):
         if a is not None:
             pcode = _element_code(a)
             break
-    if pcode not in (0, xv.code):
+    if pcode not in (0, code):
         raise ValueError("weight and bias must be float32 or of x's type")
-    _lib.call("gpb_layer_norm", xv.device, stream, xv.code, pcode, rows, cols, ov.ptr, ov.ld,
-              xv.ptr, xv.ld, _vector(weight, "weight", cols, xv, pcode),
-              _vector(bias, "bias", cols, xv, pcode), eps,
-              _vector(mean, "mean", rows, xv, 0), _vector(rstd, "rstd", rows, xv, 0))
+    _lib.call("gpb_layer_norm", dev, stream, code, pcode, rows, cols, op, out_ld, xp, x_ld,
+              _vector(weight, "weight", cols, pcode, dev), _vector(bias, "bias", cols, pcode, dev),
+              eps, _vector(mean, "mean", rows, 0, dev), _vector(rstd, "rstd", rows, 0, dev))
 
 
 @functools.lru_cache(maxsize=256)
@@ -166,24 +175,24 @@ def layer_norm_backward(dx, dout, x, mean, rstd, weight=None, *, dweight=None, d
     dx (None, dout or x themselves allowed), dweight and dbias are written
     where given; dweight and dbias are of weight's type (float32 or x's type
     when there is no weight) and need a workspace."""
-    xv = _View(x, "x", 2)
-    rows, cols = xv.shape
-    dv = _matrix(dout, "dout", xv.shape, xv)
-    ov = _matrix(dx, "dx", xv.shape, xv) if dx is not None else None
-    pcode = xv.code
+    xp, rows, cols, x_ld, code, dev = _matrix(x, "x")
+    dp, _, _, dout_ld, _, _ = _matrix(dout, "dout", rows, cols, code, dev)
+    op, out_ld = None, 0
+    if dx is not None:
+        op, _, _, out_ld, _, _ = _matrix(dx, "dx", rows, cols, code, dev)
+    pcode = code
     for a in (weight, dweight, dbias):
         if a is not None:
             pcode = _element_code(a)
             break
-    if pcode not in (0, xv.code):
+    if pcode not in (0, code):
         raise ValueError("weight and its gradient must be float32 or of x's type")
-    wptr, wbytes = _workspace(workspace, xv)
-    _lib.call("gpb_layer_norm_backward", xv.device, stream, xv.code, pcode, rows, cols,
-              ov.ptr if ov else None, ov.ld if ov else 0, dv.ptr, dv.ld, xv.ptr, xv.ld,
-              _vector(mean, "mean", rows, xv, 0), _vector(rstd, "rstd", rows, xv, 0),
-              _vector(weight, "weight", cols, xv, pcode),
-              _vector(dweight, "dweight", cols, xv, pcode),
-              _vector(dbias, "dbias", cols, xv, pcode), wptr, wbytes)
+    wptr, wbytes = _workspace(workspace, dev)
+    _lib.call("gpb_layer_norm_backward", dev, stream, code, pcode, rows, cols, op, out_ld, dp,
+              dout_ld, xp, x_ld, _vector(mean, "mean", rows, 0, dev),
+              _vector(rstd, "rstd", rows, 0, dev), _vector(weight, "weight", cols, pcode, dev),
+              _vector(dweight, "dweight", cols, pcode, dev),
+              _vector(dbias, "dbias", cols, pcode, dev), wptr, wbytes)
 
 
 # ------------------------------------------------------------- gated unit
@@ -205,15 +214,18 @@ def gated_unit_workspace(rows: int, inner: int, outer: int, dtype, backward: boo
 
 
 def _gated_inputs(x, w_gate, w_up, b_gate, b_up):
-    xv = _View(x, "x", 2)
-    g = _View(w_gate, "w_gate", 2)
-    outer = g.shape[0]
-    g = _matrix(w_gate, "w_gate", (outer, xv.shape[1]), xv)
-    u = _matrix(w_up, "w_up", (outer, xv.shape[1]), xv)
-    if g.ld != u.ld:
-        raise ValueError(f"w_gate and w_up must have one row stride, got {g.ld} and {u.ld}")
-    return (xv, g, u, _vector(b_gate, "b_gate", outer, xv, xv.code),
-            _vector(b_up, "b_up", outer, xv, xv.code))
+    """x, w_gate and w_up as matrices and the biases' pointers, checked against one another."""
+    xm = _matrix(x, "x")
+    inner, code, dev = xm[2], xm[4], xm[5]
+    if len(w_gate.shape) != 2:
+        raise ValueError(f"w_gate must be 2-D, got shape {tuple(w_gate.shape)}")
+    outer = w_gate.shape[0]
+    g = _matrix(w_gate, "w_gate", outer, inner, code, dev)
+    u = _matrix(w_up, "w_up", outer, inner, code, dev)
+    if g[3] != u[3]:
+        raise ValueError(f"w_gate and w_up must have one row stride, got {g[3]} and {u[3]}")
+    return (xm, g, u, _vector(b_gate, "b_gate", outer, code, dev),
+            _vector(b_up, "b_up", outer, code, dev))
 
 
 def gated_unit(out, x, w_gate, w_up, b_gate=None, b_up=None, *, activation: str = "silu",
@@ -224,13 +236,12 @@ def gated_unit(out, x, w_gate, w_up, b_gate=None, b_up=None, *, activation: str 
     out [rows, outer], all of one element type. `activation` is "silu",
     "gelu" (exact), "sigmoid" or "tanh"."""
     act = _activation(activation)
-    xv, g, u, bg, bu = _gated_inputs(x, w_gate, w_up, b_gate, b_up)
-    rows, inner = xv.shape
-    outer = g.shape[0]
-    ov = _matrix(out, "out", (rows, outer), xv)
-    wptr, wbytes = _workspace(workspace, xv)
-    _lib.call("gpb_gated_unit", xv.device, stream, xv.code, act, rows, inner, outer, ov.ptr, ov.ld,
-              xv.ptr, xv.ld, g.ptr, u.ptr, g.ld, bg, bu, wptr, wbytes)
+    (xp, rows, inner, x_ld, code, dev), g, u, bg, bu = _gated_inputs(x, w_gate, w_up, b_gate, b_up)
+    outer = g[1]
+    op, _, _, out_ld, _, _ = _matrix(out, "out", rows, outer, code, dev)
+    wptr, wbytes = _workspace(workspace, dev)
+    _lib.call("gpb_gated_unit", dev, stream, code, act, rows, inner, outer, op, out_ld, xp, x_ld,
+              g[0], u[0], g[3], bg, bu, wptr, wbytes)
 
 
 def gated_unit_backward(dout, x, w_gate, w_up, b_gate=None, b_up=None, *, dx=None, dw_gate=None,
@@ -240,23 +251,24 @@ def gated_unit_backward(dout, x, w_gate, w_up, b_gate=None, b_up=None, *, dx=Non
     (the projections are recomputed): dx, dw_gate, dw_up, db_gate and db_up are
     written where given, in x's element type."""
     act = _activation(activation)
-    xv, g, u, bg, bu = _gated_inputs(x, w_gate, w_up, b_gate, b_up)
-    rows, inner = xv.shape
-    outer = g.shape[0]
-    dv = _matrix(dout, "dout", (rows, outer), xv)
-    xo = _matrix(dx, "dx", xv.shape, xv) if dx is not None else None
-    go = _matrix(dw_gate, "dw_gate", g.shape, xv) if dw_gate is not None else None
-    uo = _matrix(dw_up, "dw_up", g.shape, xv) if dw_up is not None else None
-    if go and uo and go.ld != uo.ld:
-        raise ValueError(f"dw_gate and dw_up must have one row stride, got {go.ld} and {uo.ld}")
-    wo = go or uo
-    wptr, wbytes = _workspace(workspace, xv)
-    _lib.call("gpb_gated_unit_backward", xv.device, stream, xv.code, act, rows, inner, outer,
-              dv.ptr, dv.ld, xv.ptr, xv.ld, g.ptr, u.ptr, g.ld, bg, bu,
-              xo.ptr if xo else None, xo.ld if xo else 0, go.ptr if go else None,
-              uo.ptr if uo else None, wo.ld if wo else 0,
-              _vector(db_gate, "db_gate", outer, xv, xv.code),
-              _vector(db_up, "db_up", outer, xv, xv.code), wptr, wbytes)
+    (xp, rows, inner, x_ld, code, dev), g, u, bg, bu = _gated_inputs(x, w_gate, w_up, b_gate, b_up)
+    outer = g[1]
+    dp, _, _, dout_ld, _, _ = _matrix(dout, "dout", rows, outer, code, dev)
+    dxp, dx_ld, dgp, dup, dw_ld = None, 0, None, None, 0
+    if dx is not None:
+        dxp, _, _, dx_ld, _, _ = _matrix(dx, "dx", rows, inner, code, dev)
+    if dw_gate is not None:
+        dgp, _, _, dw_ld, _, _ = _matrix(dw_gate, "dw_gate", outer, inner, code, dev)
+    if dw_up is not None:
+        dup, _, _, ld, _, _ = _matrix(dw_up, "dw_up", outer, inner, code, dev)
+        if dgp is not None and ld != dw_ld:
+            raise ValueError(f"dw_gate and dw_up must have one row stride, got {dw_ld} and {ld}")
+        dw_ld = ld
+    wptr, wbytes = _workspace(workspace, dev)
+    _lib.call("gpb_gated_unit_backward", dev, stream, code, act, rows, inner, outer, dp, dout_ld, xp,
+              x_ld, g[0], u[0], g[3], bg, bu, dxp, dx_ld, dgp, dup, dw_ld,
+              _vector(db_gate, "db_gate", outer, code, dev),
+              _vector(db_up, "db_up", outer, code, dev), wptr, wbytes)
 
 
 # ---------------------------------------------------------------- dropout
@@ -266,14 +278,16 @@ def dropout(out, x, p: float, seed: int, *, offset: int = 0, residual=None, stre
     The mask is a function of (seed, offset) and the element's index row *
     columns + column alone (Philox4x32-10), so dropout_backward with the same
     two numbers regenerates it. out may be x or residual themselves."""
-    xv = _View(x, "x", 2)
-    ov = _matrix(out, "out", xv.shape, xv)
-    rv = _matrix(residual, "residual", xv.shape, xv) if residual is not None else None
+    xp, rows, cols, x_ld, code, dev = _matrix(x, "x")
+    op, _, _, out_ld, _, _ = _matrix(out, "out", rows, cols, code, dev)
+    rp, r_ld = None, 0
+    if residual is not None:
+        rp, _, _, r_ld, _, _ = _matrix(residual, "residual", rows, cols, code, dev)
     for name, v in (("seed", seed), ("offset", offset)):
         if not 0 <= v < 1 << 64:
             raise ValueError(f"{name} must be in [0, 2^64), got {v}")
-    _lib.call("gpb_dropout", xv.device, stream, xv.code, xv.shape[0], xv.shape[1], ov.ptr, ov.ld,
-              xv.ptr, xv.ld, rv.ptr if rv else None, rv.ld if rv else 0, p, seed, offset)
+    _lib.call("gpb_dropout", dev, stream, code, rows, cols, op, out_ld, xp, x_ld, rp, r_ld, p, seed,
+              offset)
 
 
 def dropout_backward(dx, dout, p: float, seed: int, *, offset: int = 0, stream=None) -> None:
@@ -284,11 +298,10 @@ def dropout_backward(dx, dout, p: float, seed: int, *, offset: int = 0, stream=N
 
 def cast(out, x, *, stream=None) -> None:
     """out = x in out's element type, rounded to nearest ([rows, columns])."""
-    xv = _View(x, "x", 2)
-    ov = _View(out, "out", 2)
-    if ov.shape != xv.shape:
-        raise ValueError(f"out must have shape {xv.shape}, got {ov.shape}")
-    if ov.device != xv.device:
-        raise ValueError(f"out is on device {ov.device}, expected {xv.device}")
-    _lib.call("gpb_cast", xv.device, stream, ov.code, xv.code, *xv.shape, ov.ptr, ov.ld, xv.ptr,
-              xv.ld)
+    xp, rows, cols, x_ld, code, dev = _matrix(x, "x")
+    op, r, c, out_ld, ocode, odev = _matrix(out, "out")
+    if (r, c) != (rows, cols):
+        raise ValueError(f"out must have shape ({rows}, {cols}), got ({r}, {c})")
+    if odev != dev:
+        raise ValueError(f"out is on device {odev}, expected {dev}")
+    _lib.call("gpb_cast", dev, stream, ocode, code, rows, cols, op, out_ld, xp, x_ld)
