@@ -482,7 +482,9 @@ int gpb_layer_norm_backward(int32_t device, void* stream, int32_t dtype, int32_t
  * activation and the product in one kernel: x [rows][inner], w_gate and w_up
  * [outer][inner] with one leading dimension, biases [outer] or NULL, out
  * [rows][outer], all of one type; `activation` is GPB_ACT_*. out must not
- * overlap an input. */
+ * overlap an input. float32 products are formed from three bfloat16 parts per
+ * value (float32 accuracy): with more than 8 rows, an input beyond 3.3895e38
+ * or not finite makes the outputs that depend on it NaN. */
 int gpb_gated_unit_workspace(int32_t dtype, int64_t rows, int64_t inner, int64_t outer,
                              int32_t backward, int64_t* bytes_out);
 int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activation, int64_t rows,

@@ -210,29 +210,71 @@ __global__ void __launch_bounds__(256) mm_join_kernel(const float* __restrict__ 
   if (c) c[(f / N) * c_ld + f % N] = from_f<T>(s);
 }
 
-// A matrix to tensor-core operands: fp32 to three bf16 planes, or a 16-bit matrix whose rows are not
-// 16-byte aligned to one plane whose are. 8 output columns per thread; columns up to ld are zeros.
+// Matrices to tensor-core operands, one per blockIdx.y: fp32 weights to three bf16 planes, or a matrix
+// whose rows are not 16-byte aligned to a copy whose are (`copy`). 8 output columns per thread;
+// columns up to ld are zeros.
+struct PackArgs {
+  const void* src[3];
+  void* dst[3];
+  int64_t rows[3], src_ld[3];
+  int32_t copy[3];
+  int64_t cols, ld;
+};
 template <typename T, typename D>
-__global__ void __launch_bounds__(256) gated_pack_kernel(const T* __restrict__ src, int64_t src_ld,
-                                                         int64_t rows, int64_t cols, int64_t ld,
-                                                         int64_t plane, D* __restrict__ dst) {
+__global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__ PackArgs A) {
+  const int o = blockIdx.y;
   const int64_t run = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t per = ld / 8;
-  if (run >= rows * per) return;
+  const int64_t per = A.ld / 8;
+  if (run >= A.rows[o] * per) return;
   const int64_t r = run / per, c = (run - r * per) * 8;
+  const T* src = (const T*)A.src[o] + r * A.src_ld[o] + c;
   float v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f(src[r * src_ld + c + i]) : 0.f;
-  if constexpr (sizeof(T) == 4) {
-    float h[8], m[8], l[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) gg_split3(v[i], h[i], m[i], l[i]);
-    store_vec<D, 8>(dst + r * ld + c, h);
-    store_vec<D, 8>(dst + plane + r * ld + c, m);
-    store_vec<D, 8>(dst + 2 * plane + r * ld + c, l);
+  for (int i = 0; i < 8; ++i) v[i] = c + i < A.cols ? to_f(src[i]) : 0.f;
+  if (sizeof(T) == 2 || A.copy[o]) {
+    store_vec<T, 8>((T*)A.dst[o] + r * A.ld + c, v);
   } else {
-    store_vec<D, 8>(dst + r * ld + c, v);
+    D* dst = (D*)A.dst[o] + r * A.ld + c;
+    float2 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = make_float2(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      uint32_t h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = gg_part(x[i]);
+      *reinterpret_cast<uint4*>(dst + k * A.rows[o] * A.ld) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
   }
+}
+
+// The backward pass's joins in one launch: blocks below `dw_blocks` add the ranges of dWg and dWu (in
+// range order), the others the column sums of dgate and dup (32 columns each, 32 threads along the
+// partial rows).
+struct JoinArgs {
+  const float* dw_partial;
+  int64_t ranges, M, N, dw_ld;
+  void* dw[2];
+  const float* col_sums;
+  int64_t sum_rows;
+  void* db[2];
+  int64_t dw_blocks;
+};
+template <typename T>
+__global__ void __launch_bounds__(1024) gated_join_kernel(const __grid_constant__ JoinArgs A) {
+  if (blockIdx.x < A.dw_blocks) {
+    const int64_t e = (int64_t)blockIdx.x * 1024 + threadIdx.x, one = A.M * A.N;
+    if (e >= 2 * one) return;
+    float s = 0.f;
+#pragma unroll 4
+    for (int64_t r = 0; r < A.ranges; ++r) s += A.dw_partial[r * 2 * one + e];
+    const int half = e >= one;
+    T* dst = (T*)A.dw[half];
+    const int64_t f = e - half * one;
+    if (dst) dst[(f / A.N) * A.dw_ld + f % A.N] = from_f<T>(s);
+    return;
+  }
+  column_join<T>(A.col_sums, A.sum_rows, A.M, (T*)A.db[0], (T*)A.db[1], blockIdx.x - A.dw_blocks);
 }
 
 // ------------------------------------------------------------------ host
@@ -255,23 +297,29 @@ static int encode_fn(EncodeTiled* fn) {
   return GPB_OK;
 }
 
-// A 16-bit operand: `planes` matrices [rows][cols] with leading dimension ld (a multiple of 8).
+// An operand as TMA reads it: `planes` matrices [rows][cols] of 16-bit elements, or one of fp32, whose
+// rows are a multiple of 16 bytes apart.
 struct Operand {
   const void* p = nullptr;
+  bool f32 = false;
   int64_t rows = 0, cols = 0, ld = 0, plane = 0;
   int planes = 1;
 };
 
-static int make_map(const Operand& o, int box_rows, CUtensorMap* map) {
+static int make_map(const Operand& o, int box_cols, int box_rows, CUtensorMap* map) {
   EncodeTiled fn;
   GPB_TRY(encode_fn(&fn));
   const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
   const int64_t plane = o.planes > 1 ? o.plane : o.rows * o.ld;
-  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)plane * 2};
-  const cuuint32_t box[3] = {kGgBK, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+  const int es = o.f32 ? 4 : 2;
+  const cuuint64_t strides[2] = {(cuuint64_t)(o.ld * es), (cuuint64_t)(plane * es)};
+  const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
   const CUresult r =
-      fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(o.p), dims, strides, box, step,
-         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      fn(map, o.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
+         const_cast<void*>(o.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         o.f32            ? CU_TENSOR_MAP_SWIZZLE_NONE
+         : box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B
+                          : CU_TENSOR_MAP_SWIZZLE_64B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   GPB_REQUIRE(r == CUDA_SUCCESS, GPB_ERR_CUDA, "tensor map of %lld x %lld (stride %lld): error %d",
               (long long)o.rows, (long long)o.cols, (long long)o.ld, (int)r);
@@ -329,8 +377,8 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
   }
   P.planes = f32 ? 3 : 1;
   P.ldk = round_up(inner, 8);
-  P.ldn = round_up(outer, 8);
-  P.x = take(at, P.planes * rows * P.ldk * 2);
+  P.ldn = round_up(outer, 16);
+  P.x = take(at, rows * P.ldk * dtype_bytes(dtype));
   P.wg = take(at, P.planes * outer * P.ldk * 2);
   P.wu = take(at, P.planes * outer * P.ldk * 2);
   if (backward) {
@@ -340,9 +388,10 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
     P.du = take(at, P.planes_d * P.plane_d * 2);
     P.tile_n = plain_tile(inner, f32);
     const int64_t tiles = (outer <= 64 ? 1 : 2 * ceil_div(outer, kGgBM)) * ceil_div(inner, P.tile_n);
-    const int64_t kb = ceil_div(rows, kGgBK);
-    // At least 8 stages per range; as many ranges as fill the SMs twice.
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * kFeatSMs / tiles, kb / 8));
+    const int bk = f32 ? kGgSplitBK : kGgBK;
+    const int64_t kb = ceil_div(rows, bk);
+    // At least 512 rows per range; as many ranges as fill the SMs twice.
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * kFeatSMs / tiles, kb * bk / 512));
     P.kb_per = (int)ceil_div(kb, want);
     P.splits = (int)ceil_div(kb, P.kb_per);
     P.partial = take(at, P.splits > 1 ? P.splits * 2 * outer * inner * 4 : 0);
@@ -357,36 +406,61 @@ static int gg_launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtenso
                      const CUtensorMap& b1, GgArgs& G, cudaStream_t st) {
   using S = GgShape<MODE, NB, PA, PB>;
   constexpr auto kernel = gated_gemm_kernel<MODE, NB, PA, PB, T, D, PD, BACK>;
-  GPB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  GPB_TRY(allow_smem<kernel>(S::kSmem));
   void* err = nullptr;
   GPB_CHECK_CUDA(cudaGetSymbolAddress(&err, g_feature_err));
   G.err = (int*)err;
   G.idesc = gg_idesc(std::is_same<D, __nv_bfloat16>::value, MODE == GG_DW, MODE != GG_PROJ, NB);
   const int64_t items = (int64_t)G.tiles_m * G.tiles_n * G.splits;
-  kernel<<<(unsigned)std::min<int64_t>(items, kFeatSMs), kGgThreads, S::kSmem, st>>>(a0, a1, b0, b1, G);
+  kernel<<<(unsigned)std::min<int64_t>(items, kFeatSMs), S::kThreads, S::kSmem, st>>>(a0, a1, b0, b1, G);
   GPB_CHECK_CUDA(cudaGetLastError());
   return GPB_OK;
 }
 
-// x and the weights as tensor-core operands: where they lie when they are 16-bit with aligned rows,
-// packed into the workspace otherwise.
+// Alignment of a matrix's rows: 2 = 32 bytes, 1 = 16 bytes, 0 = less.
+static int row_align(const void* p, int64_t row_bytes) {
+  const uint64_t bits = (uint64_t)(uintptr_t)p | (uint64_t)row_bytes;
+  return bits % 32 == 0 ? 2 : bits % 16 == 0 ? 1 : 0;
+}
+
+// x and the weights as TMA reads them: where they lie when their rows are aligned, copied into the
+// workspace otherwise; fp32 weights as planes (fp32 x is split inside the products).
 template <typename T, typename D>
-static int gated_operand(const void* p, int64_t rows, int64_t cols, int64_t ld, const GatedPlan& P,
-                         char* packed, Operand* o, cudaStream_t st) {
-  o->rows = rows;
-  o->cols = cols;
-  if (sizeof(T) == 2 && aligned16(p) && ld % 8 == 0) {
+static int gated_operands(const GatedArgs& A, const GatedPlan& P, char* ws, Operand* x, Operand* wg,
+                          Operand* wu, cudaStream_t st) {
+  PackArgs K{};
+  K.cols = A.inner;
+  K.ld = P.ldk;
+  int count = 0;
+  int64_t most = 0;
+  auto operand = [&](const void* p, int64_t rows, int64_t ld, char* packed, Operand* o, bool planes) {
+    o->rows = rows;
+    o->cols = A.inner;
     o->p = p;
     o->ld = ld;
-    return GPB_OK;
+    o->f32 = sizeof(T) == 4 && !planes;
+    if (!planes && aligned16(p) && ld * sizeof(T) % 16 == 0) return;
+    o->p = packed;
+    o->ld = P.ldk;
+    o->planes = planes ? P.planes : 1;
+    o->plane = rows * P.ldk;
+    K.src[count] = p;
+    K.dst[count] = packed;
+    K.rows[count] = rows;
+    K.src_ld[count] = ld;
+    K.copy[count] = !planes;
+    most = std::max(most, rows);
+    ++count;
+  };
+  constexpr bool kPlanes = sizeof(T) == 4;
+  operand(A.x, A.rows, A.x_ld, ws + P.x, x, false);
+  operand(A.wg, A.outer, A.w_ld, ws + P.wg, wg, kPlanes);
+  operand(A.wu, A.outer, A.w_ld, ws + P.wu, wu, kPlanes);
+  if (count) {
+    gated_pack_kernel<T, D>
+        <<<dim3((unsigned)ceil_div(most * (P.ldk / 8), 256), count), 256, 0, st>>>(K);
+    GPB_CHECK_CUDA(cudaGetLastError());
   }
-  o->p = packed;
-  o->ld = P.ldk;
-  o->planes = P.planes;
-  o->plane = rows * P.ldk;
-  gated_pack_kernel<T, D><<<(unsigned)ceil_div(rows * (P.ldk / 8), 256), 256, 0, st>>>(
-      (const T*)p, ld, rows, cols, P.ldk, o->plane, (D*)packed);
-  GPB_CHECK_CUDA(cudaGetLastError());
   return GPB_OK;
 }
 
@@ -396,14 +470,15 @@ static int gated_project(const GatedArgs& A, const Operand& x, const Operand& wg
   const int nb = proj_tile(A.outer, PL == 3);
   const int bn = nb / 2;
   CUtensorMap mx, mg, mu;
-  GPB_TRY(make_map(x, kGgBM, &mx));
-  GPB_TRY(make_map(wg, bn, &mg));
-  GPB_TRY(make_map(wu, bn, &mu));
+  constexpr int BK = PL == 3 ? kGgSplitBK : kGgBK;
+  GPB_TRY(make_map(wg, BK, bn, &mg));
+  GPB_TRY(make_map(wu, BK, bn, &mu));
+  GPB_TRY(make_map(x, BK, kGgBM, &mx));
   G.M = A.rows;
   G.N = A.outer;
   G.tiles_m = (int32_t)ceil_div(A.rows, kGgBM);
   G.tiles_n = (int32_t)ceil_div(A.outer, bn);
-  G.kblocks = (int32_t)ceil_div(A.inner, kGgBK);
+  G.kblocks = (int32_t)ceil_div(A.inner, BK);
   G.segs = G.splits = 1;
   G.kb_per = G.kblocks;
   G.bg = A.bg;
@@ -425,8 +500,9 @@ template <int MODE, typename T, typename D, int PL, int PD>
 static int gated_plain(const CUtensorMap& a0, const CUtensorMap& a1, const Operand& b0,
                        const Operand& b1, int nb, GgArgs& G, cudaStream_t st) {
   CUtensorMap m0, m1;
-  GPB_TRY(make_map(b0, kGgBK, &m0));
-  GPB_TRY(make_map(b1, kGgBK, &m1));
+  constexpr int BK = gg_splits(MODE, PL) ? kGgSplitBK : kGgBK;
+  GPB_TRY(make_map(b0, 64, BK, &m0));
+  GPB_TRY(make_map(b1, 64, BK, &m1));
   switch (nb) {
     case 64: return gg_launch<MODE, 64, PD, PL, T, D, PD, false>(a0, a1, m0, m1, G, st);
     case 128: return gg_launch<MODE, 128, PD, PL, T, D, PD, false>(a0, a1, m0, m1, G, st);
@@ -505,24 +581,19 @@ static int gated_forward(const GatedArgs& A, char* ws, const GatedPlan& P, cudaS
     return gated_vec<T>(A) ? gated_rows_pick<T, V, false>(A, nullptr, nullptr, st)
                            : gated_rows_pick<T, 1, false>(A, nullptr, nullptr, st);
   Operand x, wg, wu;
-  GPB_TRY((gated_operand<T, D>(A.x, A.rows, A.inner, A.x_ld, P, ws + P.x, &x, st)));
-  GPB_TRY((gated_operand<T, D>(A.wg, A.outer, A.inner, A.w_ld, P, ws + P.wg, &wg, st)));
-  GPB_TRY((gated_operand<T, D>(A.wu, A.outer, A.inner, A.w_ld, P, ws + P.wu, &wu, st)));
+  GPB_TRY((gated_operands<T, D>(A, P, ws, &x, &wg, &wu, st)));
   GgArgs G{};
   G.out[0] = A.out;
   G.out_ld = A.out_ld;
-  G.vec = aligned16(A.out) && A.out_ld % V == 0;
+  G.vec = row_align(A.out, A.out_ld * sizeof(T));
   return gated_project<T, D, PL, PL, false>(A, x, wg, wu, G, st);
 }
 
 template <typename T, typename D, int PL, int PD>
 static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, const GatedPlan& P,
                           cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
   Operand x, wg, wu;
-  GPB_TRY((gated_operand<T, D>(A.x, A.rows, A.inner, A.x_ld, P, ws + P.x, &x, st)));
-  GPB_TRY((gated_operand<T, D>(A.wg, A.outer, A.inner, A.w_ld, P, ws + P.wg, &wg, st)));
-  GPB_TRY((gated_operand<T, D>(A.wu, A.outer, A.inner, A.w_ld, P, ws + P.wu, &wu, st)));
+  GPB_TRY((gated_operands<T, D>(A, P, ws, &x, &wg, &wu, st)));
   float* partial = (float*)(ws + P.partial);
   Operand dg, du;
   dg.p = ws + P.dg;
@@ -538,7 +609,7 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
     G.out[1] = ws + P.du;
     G.out_ld = P.ldn;
     G.plane = P.plane_d;
-    G.vec = aligned16(A.dout) && A.dout_ld % V == 0;
+    G.vec = row_align(A.dout, A.dout_ld * sizeof(T));
     if (R.dbg || R.dbu) G.col_sums = (float*)(ws + P.sums);
     GPB_TRY((gated_project<T, D, PL, PD, true>(A, x, wg, wu, G, st)));
   }
@@ -555,10 +626,10 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
     G.kb_per = 2 * G.kblocks;
     G.out[0] = R.dx;
     G.out_ld = R.dx_ld;
-    G.vec = aligned16(R.dx) && R.dx_ld % V == 0;
+    G.vec = row_align(R.dx, R.dx_ld * sizeof(T));
     CUtensorMap a0, a1;
-    GPB_TRY(make_map(dg, kGgBM, &a0));
-    GPB_TRY(make_map(du, kGgBM, &a1));
+    GPB_TRY(make_map(dg, kGgBK, kGgBM, &a0));
+    GPB_TRY(make_map(du, kGgBK, kGgBM, &a1));
     GPB_TRY((gated_plain<GG_DX, T, D, PL, PD>(a0, a1, wg, wu, nb, G, st)));
   }
   if (R.dwg || R.dwu) {
@@ -569,7 +640,8 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
     G.half_tiles = joined ? 0 : (int32_t)ceil_div(A.outer, kGgBM);
     G.tiles_m = joined ? 1 : 2 * G.half_tiles;
     G.tiles_n = (int32_t)ceil_div(A.inner, P.tile_n);
-    G.kblocks = (int32_t)ceil_div(A.rows, kGgBK);
+    constexpr int BK = PL == 3 ? kGgSplitBK : kGgBK;
+    G.kblocks = (int32_t)ceil_div(A.rows, BK);
     G.segs = 1;
     G.splits = P.splits;
     G.kb_per = P.kb_per;
@@ -577,20 +649,31 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
     G.out[1] = R.dwu;
     G.out_ld = R.dw_ld;
     G.partial = partial;
-    G.vec = aligned16(R.dwg) && aligned16(R.dwu) && R.dw_ld % V == 0;
+    G.vec = std::min(row_align(R.dwg, R.dw_ld * sizeof(T)), row_align(R.dwu, R.dw_ld * sizeof(T)));
     CUtensorMap a0, a1;
-    GPB_TRY(make_map(dg, kGgBK, &a0));
-    GPB_TRY(make_map(du, kGgBK, &a1));
+    GPB_TRY(make_map(dg, 64, BK, &a0));
+    GPB_TRY(make_map(du, 64, BK, &a1));
     GPB_TRY((gated_plain<GG_DW, T, D, PL, PD>(a0, a1, x, x, P.tile_n, G, st)));
-    if (P.splits > 1) {
-      mm_join_kernel<T><<<(unsigned)ceil_div(2 * A.outer * A.inner, 256), 256, 0, st>>>(
-          partial, P.splits, A.outer, A.inner, 2, (T*)R.dwg, (T*)R.dwu, R.dw_ld);
-      GPB_CHECK_CUDA(cudaGetLastError());
-    }
   }
-  if (R.dbg || R.dbu) {
-    column_join_kernel<T><<<(unsigned)ceil_div(2 * A.outer, 32), 1024, 0, st>>>(
-        (const float*)(ws + P.sums), 4 * ceil_div(A.rows, kGgBM), A.outer, (T*)R.dbg, (T*)R.dbu);
+  const bool bias = R.dbg || R.dbu, join_w = P.splits > 1 && (R.dwg || R.dwu);
+  if (bias || join_w) {
+    JoinArgs J{};
+    J.M = A.outer;
+    J.N = A.inner;
+    if (join_w) {
+      J.dw_partial = partial;
+      J.ranges = P.splits;
+      J.dw_ld = R.dw_ld;
+      J.dw[0] = R.dwg;
+      J.dw[1] = R.dwu;
+      J.dw_blocks = ceil_div(2 * A.outer * A.inner, 1024);
+    }
+    J.col_sums = (const float*)(ws + P.sums);
+    J.sum_rows = 4 * ceil_div(A.rows, kGgBM);
+    J.db[0] = R.dbg;
+    J.db[1] = R.dbu;
+    const int64_t grid = J.dw_blocks + (bias ? ceil_div(2 * A.outer, 32) : 0);
+    gated_join_kernel<T><<<(unsigned)grid, 1024, 0, st>>>(J);
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   return GPB_OK;

@@ -514,6 +514,12 @@ __global__ void __launch_bounds__(256) norm_params_wide_kernel(const NormArgs A)
   part[A.cols + c] = db;
 }
 
+template <typename W>
+__global__ void __launch_bounds__(1024) norm_join_kernel(const float* __restrict__ partial,
+                                                         int64_t rows, int64_t cols, W* dw, W* db) {
+  column_join<W>(partial, rows, cols, dw, db, blockIdx.x);
+}
+
 // ------------------------------------------------------------------ host
 // Threads per row and vectors per thread for `nvec` vectors: the widest part of a warp first, then
 // blocks of warps, growing R only once the row has `max_tpr` threads. Returns R, or 0 when the row
@@ -567,9 +573,9 @@ static int norm_backward_run(const NormArgs& A, int grid, int threads, cudaStrea
   if constexpr (VEC > 1) {
     smem = std::max<size_t>(smem, (size_t)(kNormAhead<R> + 1) * R * 2 * threads * 16);
     constexpr auto kernel = norm_backward_kernel<T, W, VEC, R, PARAMS>;
-    if (smem > 40 * 1024)  // with the static part, 48 KB need no opt-in
-      GPB_CHECK_CUDA(
-          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // The ring of the widest block; with the static part, 48 KB need no opt-in.
+    constexpr int kMost = (kNormAhead<R> + 1) * R * 2 * 512 * 16;
+    if (smem > 40 * 1024) GPB_TRY(allow_smem<kernel>(kMost));
     kernel<<<grid, threads, smem, st>>>(A);
   } else {
     norm_backward_scalar_kernel<T, W, R, PARAMS><<<grid, threads, smem, st>>>(A);
@@ -625,7 +631,7 @@ static int norm_backward_launch(NormArgs A, W* dw, W* db, cudaStream_t st) {
     }
   }
   if (params) {
-    column_join_kernel<W><<<(unsigned)ceil_div(2 * (int64_t)A.cols, 32), 1024, 0, st>>>(
+    norm_join_kernel<W><<<(unsigned)ceil_div(2 * (int64_t)A.cols, 32), 1024, 0, st>>>(
         A.partial, blocks, A.cols, dw, db);
     GPB_CHECK_CUDA(cudaGetLastError());
   }

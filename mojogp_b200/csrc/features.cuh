@@ -4,6 +4,8 @@
 // different streams (or in captured graphs) share nothing that the caller did not pass twice.
 #pragma once
 
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -128,29 +130,42 @@ __device__ __forceinline__ uint4 pack16(const float2 (&v)[4], const __half*) {
                     bits32(__float22half2_rn(v[2])), bits32(__float22half2_rn(v[3])));
 }
 
-// Column sums of `blocks` partial rows [2][cols] to two vectors (either may be null): 32 columns per
-// block, 32 threads along the rows of each, in a fixed order.
+// Column sums of `rows` partial rows [2][cols] to two vectors (either may be null): columns
+// [32 chunk, 32 chunk + 32) by a block of 1024 threads, 32 along the rows of each, in a fixed order.
 template <typename W>
-__global__ void __launch_bounds__(1024) column_join_kernel(const float* __restrict__ partial,
-                                                           int64_t blocks, int64_t cols, W* a, W* b) {
+__device__ __forceinline__ void column_join(const float* __restrict__ partial, int64_t rows,
+                                            int64_t cols, W* a, W* b, int64_t chunk) {
   __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t c = chunk * 32 + lane;
   float s = 0.f;
   if (c < 2 * cols) {
 #pragma unroll 8
-    for (int64_t r = part; r < blocks; r += 32) s += partial[r * 2 * cols + c];
+    for (int64_t r = part; r < rows; r += 32) s += partial[r * 2 * cols + c];
   }
   sums[part][lane] = s;
   __syncthreads();
   s = sums[lane][part];  // transposed: warp `part` sums column `part`
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  const int64_t col = (int64_t)blockIdx.x * 32 + part;
+  const int64_t col = chunk * 32 + part;
   if (lane == 0 && col < 2 * cols) {
     W* dst = col < cols ? a : b;
     if (dst) dst[col < cols ? col : col - cols] = from_f<W>(s);
   }
+}
+
+// Opts a kernel into `bytes` of dynamic shared memory, once per kernel and device.
+template <auto kernel>
+int allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  GPB_CHECK_CUDA(cudaGetDevice(&device));
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return GPB_OK;
+  GPB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return GPB_OK;
 }
 
 }  // namespace gpb

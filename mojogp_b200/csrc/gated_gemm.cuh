@@ -10,7 +10,9 @@
 // x and the weights are read where they lie. A product whose reduction index is not the contiguous
 // one takes its operand MN-major: the tensor core transposes, nothing is copied.
 //
-// fp32 inputs are exact sums of three bf16 planes (8 significant bits each), and
+// fp32 inputs are exact sums of three bf16 planes (8 significant bits each; the weights are packed
+// before the call; x comes in as fp32 tiles that four warps split into the planes the MMAs read, 4
+// bytes an element from HBM instead of a pass of 10 and 6 per use), and
 // a product keeps the six plane pairs above 2^-24 of it: hi hi apart from the five small ones, which
 // have their own accumulator. The tensor core truncates where it adds, about 2^-26 of the accumulator
 // per MMA, so after every kGgWindow blocks of the reduction the epilogue warps add both accumulators
@@ -112,9 +114,11 @@ enum GgMode { GG_PROJ = 0, GG_DX = 1, GG_DW = 2 };
 
 constexpr int kGgBM = 128;       // rows of a tile (TMEM lanes)
 constexpr int kGgBK = 64;        // reduction depth of a stage: one 128-byte swizzle row of 16-bit
-constexpr int kGgWindow = 4;     // stages between promotions of the fp32 variant (256 deep)
-constexpr int kGgThreads = 320;
+constexpr int kGgSplitBK = 32;   // the same where x is split: more and smaller stages in flight
+constexpr int kGgWindow = 256;   // depth between promotions of the fp32 variant
 constexpr int kGgEpiWarps = 8;
+constexpr int kGgSplitWarps = 4;
+constexpr int kGgRaw = 4;        // fp32 tiles in flight
 constexpr int kGgGroup = 8;      // row tiles that share a pass over the column tiles (L2 reuse)
 
 struct GgArgs {
@@ -138,19 +142,22 @@ struct GgArgs {
   float* col_sums;     // backward GG_PROJ: [4 tiles_m][2][N] column sums of dgate and dup, or null
   int64_t dout_ld;
   int32_t act;
-  int32_t vec;         // 16-byte stores (and dout loads) are aligned
+  int32_t vec;         // output rows (backward GG_PROJ: dout rows) are 2: 32-byte, 1: 16-byte aligned
   int* err;
 };
 
-// 128-byte-swizzled shared-memory descriptor. K-major: rows of 128 bytes, 8-row atoms `sbo` = 1024
-// bytes apart (lbo unused). MN-major: blocks of [64 reduction rows][64 outputs], 8-row groups 1024
-// bytes apart (sbo), blocks of 64 outputs `lbo` bytes apart.
-__device__ __forceinline__ uint64_t gg_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+// Shared-memory descriptor. K-major: rows of 2 BK bytes, swizzled over their length (128 or 64 bytes),
+// 8-row atoms `sbo` apart (lbo unused). MN-major: 128-byte swizzled blocks of [BK reduction rows][64
+// outputs], 8-row groups 1024 bytes apart (sbo), blocks of 64 outputs `lbo` bytes apart.
+template <bool MN, int BK>
+__device__ __forceinline__ uint64_t gg_desc(uint32_t addr) {
+  constexpr uint32_t lbo = MN ? BK * 128 : 16, sbo = MN ? 1024 : 8 * 2 * BK;
+  constexpr uint64_t swizzle = MN || BK == 64 ? 2 : 4;
   uint64_t d = (uint64_t)((addr >> 4) & 0x3FFFu);
   d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
   d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
   d |= (uint64_t)1 << 46;  // descriptor version for sm_100
-  d |= (uint64_t)2 << 61;  // 128-byte swizzle
+  d |= swizzle << 61;
   return d;
 }
 
@@ -158,6 +165,16 @@ __device__ __forceinline__ uint64_t gg_desc(uint32_t addr, uint32_t lbo, uint32_
 __host__ __device__ constexpr uint32_t gg_idesc(bool bf16, bool a_mn, bool b_mn, int n) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) |
          ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kGgBM >> 4) << 24);
+}
+
+// One lane of a converged warp. A tcgen05.mma under `elect.sync` takes its descriptors from uniform
+// registers; under `lane == 0` the compiler cannot know that one thread runs it.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
 
 __device__ __forceinline__ void gg_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
@@ -179,28 +196,40 @@ __device__ __forceinline__ void gg_tma(uint32_t dst, const CUtensorMap* map, int
       : "memory");
 }
 
-// v = a + b + c exactly, each of 8 significant bits (round to nearest, so the parts shrink by 2^-8
-// and 2^-16 and the dropped products stay below 2^-25). A value that rounds past bf16's range is cut
-// instead; one that is not finite stays whole in the first part.
-__device__ __forceinline__ float gg_bf16_part(float v) {
-  const float r = __bfloat162float(__float2bfloat16_rn(v));
-  return fabsf(r) <= 3.4e38f || v != v ? r : __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
+// The next bf16 part of a pair of fp32 values, which keep their remainders: three parts are the exact
+// value (round to nearest, so they shrink by 2^-8 and 2^-16 and the dropped products stay below
+// 2^-25). A value beyond bf16's largest (3.3895e38) or not finite leaves a NaN remainder, and makes
+// what depends on it NaN; looking for one per pair cost a branch that halted the splitting warps
+// (a stage took 6 us where its MMAs take 0.8).
+__device__ __forceinline__ uint32_t gg_part(float2& x) {
+  const uint32_t h = bits32(__float22bfloat162_rn(x));
+  x.x -= __uint_as_float(h << 16);
+  x.y -= __uint_as_float(h & 0xFFFF0000u);
+  return h;
 }
-__device__ __forceinline__ void gg_split3(float v, float& a, float& b, float& c) {
-  a = gg_bf16_part(v);
-  const float r = v - a;
-  b = r == r ? gg_bf16_part(r) : 0.f;
-  c = r == r ? r - b : 0.f;
-}
+
+// fp32 x is GG_PROJ's A operand and GG_DW's B operand.
+__host__ __device__ constexpr bool gg_splits(int mode, int pb) { return pb == 3 && mode != GG_DX; }
 
 template <int MODE, int NB, int PA, int PB>
 struct GgShape {
-  static constexpr int kABytes = kGgBM * kGgBK * 2;
-  static constexpr int kBBytes = NB * kGgBK * 2;
+  static constexpr bool kSplit = gg_splits(MODE, PB);
+  static constexpr int kBK = kSplit ? kGgSplitBK : kGgBK;
+  static constexpr int kThreads = 32 * (2 + kGgEpiWarps + (kSplit ? kGgSplitWarps : 0));
+  static constexpr int kABytes = kGgBM * kBK * 2;
+  static constexpr int kBBytes = NB * kBK * 2;
   static constexpr int kStage = PA * kABytes + PB * kBBytes;
-  static constexpr int kStages = 200 * 1024 / kStage < 8 ? 200 * 1024 / kStage : 8;
-  static constexpr int kSmem = kStages * kStage + 1024;  // + alignment of the first stage
+  // The part of a stage that TMA writes; the splitting warps write the rest, from a ring of fp32 tiles.
+  static constexpr bool kTmaA = !(kSplit && MODE == GG_PROJ), kTmaB = !(kSplit && MODE == GG_DW);
+  static constexpr int kTmaBytes = (kTmaA ? PA * kABytes : 0) + (kTmaB ? PB * kBBytes : 0);
+  static constexpr int kPlane = kTmaA ? kBBytes : kABytes;  // of the split operand
+  static constexpr int kRaw = kSplit ? 2 * kPlane : 0;
+  static constexpr int kRest = kGgRaw * kRaw;
+  static constexpr int kStages =
+      (208 * 1024 - kRest) / kStage < 8 ? (208 * 1024 - kRest) / kStage : 8;
+  static constexpr int kSmem = kStages * kStage + kRest + 1024;  // + alignment of the first stage
   static constexpr bool kWindowed = PB == 3;             // fp32 inputs
+  static constexpr int kWindow = kGgWindow / kBK;        // stages between promotions
   static constexpr int kAcc = kWindowed ? 2 * NB : NB;   // TMEM columns of one accumulator buffer
   static_assert(2 * kAcc <= 512, "TMEM budget");
   static_assert(kStages >= 2, "shared-memory budget");
@@ -226,21 +255,39 @@ __device__ __forceinline__ GgItem gg_item(const GgArgs& A, int64_t item) {
   return I;
 }
 
-// Four fp32 columns of one row to the output's type.
-template <typename T, int COLS>
-__device__ __forceinline__ void gg_store(T* dst, const float (&v)[COLS], int64_t left, bool vec) {
-  constexpr int V = 16 / sizeof(T);
-  if (vec && left >= COLS) {
+// A whole 32-byte sector in one access (16-byte stores of a thread's own row leave half-written
+// sectors to the L2).
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x),
+               "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
+// 16 columns of one row to the output's type; vec: 2 = 32-byte aligned, 1 = 16-byte, 0 = neither.
+template <typename T>
+__device__ __forceinline__ void gg_store(T* dst, const float (&v)[16], int64_t left, int vec) {
+  constexpr int V = 16 / sizeof(T), Q = 16 / V;
+  if (vec && left >= 16) {
+    uint4 raw[Q];
 #pragma unroll
-    for (int q = 0; q < COLS / V; ++q) {
-      float w[V];
+    for (int q = 0; q < Q; ++q) {
+      float2 w[V / 2];
 #pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = v[q * V + i];
-      store_vec<T, V>(dst + q * V, w);
+      for (int i = 0; i < V / 2; ++i) w[i] = make_float2(v[q * V + 2 * i], v[q * V + 2 * i + 1]);
+      raw[q] = pack16(w, (const T*)nullptr);
+    }
+#pragma unroll
+    for (int q = 0; q < Q; q += 2) {
+      if (vec == 2) {
+        store32(dst + q * V, raw[q], raw[q + 1]);
+      } else {
+        reinterpret_cast<uint4*>(dst)[q] = raw[q];
+        reinterpret_cast<uint4*>(dst)[q + 1] = raw[q + 1];
+      }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < COLS; ++i)
+    for (int i = 0; i < 16; ++i)
       if (i < left) dst[i] = from_f<T>(v[i]);
   }
 }
@@ -306,7 +353,7 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int64_t m, int64_
     if (m >= A.M || left <= 0) return;
 #pragma unroll
     for (int i = 0; i < 16; ++i) g[i] = value[i] * u[i];
-    gg_store<T, 16>((T*)A.out[0] + m * A.out_ld + n, g, left, A.vec);
+    gg_store<T>((T*)A.out[0] + m * A.out_ld + n, g, left, A.vec);
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -322,15 +369,15 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int64_t m, int64_
       }
     }
     if (m >= A.M || left <= 0) return;
-    // The planes' leading dimension is a multiple of 8 columns and their base is aligned, so the
-    // stores are vectors; columns up to the leading dimension past N are never read.
+    // The planes' leading dimension is a multiple of 16 columns and their base is aligned, so the
+    // stores are whole sectors; columns up to the leading dimension past N are never read.
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float(&v)[16] = h == 0 ? g : u;
       D* dst = (D*)A.out[h] + m * A.out_ld + n;
 #pragma unroll
       for (int p = 0; p < PD; ++p) {
-        gg_store<D, 16>(dst + p * A.plane, v, left, true);
+        gg_store<D>(dst + p * A.plane, v, left, 2);
         if (p + 1 < PD) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -363,16 +410,49 @@ __device__ __forceinline__ void gg_plain_store(const GgArgs& A, const GgItem& I,
   if (m >= A.M || n >= A.N) return;
   if (MODE == GG_DW && A.splits > 1) {
     float* dst = A.partial + (((int64_t)I.split * 2 + half) * A.M + m) * A.N + n;
-    gg_store<float, 16>(dst, v, A.N - n, A.N % 4 == 0);
+    gg_store<float>(dst, v, A.N - n, A.N % 8 == 0 ? 2 : 0);
   } else if (A.out[half]) {
-    gg_store<T, 16>((T*)A.out[half] + m * A.out_ld + n, v, A.N - n, A.vec);
+    gg_store<T>((T*)A.out[half] + m * A.out_ld + n, v, A.N - n, A.vec);
+  }
+}
+
+// Splits an fp32 tile into planes: 128 threads, each UNITS runs of 8 elements, 128 runs apart. ROW
+// elements to a row of the tile; planes' rows are swizzled as TMA writes them.
+template <int UNITS, int ROW>
+__device__ __forceinline__ void gg_split_tile(int tid, uint32_t raw, uint32_t tile, uint32_t plane) {
+  float2 v[UNITS][4];
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const uint32_t at = raw + (u * 128 + tid) * 32;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[u][2 * h].x), "=f"(v[u][2 * h].y), "=f"(v[u][2 * h + 1].x),
+                     "=f"(v[u][2 * h + 1].y)
+                   : "r"(at + 16 * h));
+  }
+  constexpr int RUNS = ROW / 8;
+  const int r0 = tid / RUNS, c0 = tid % RUNS;  // 128 runs on: the same swizzle
+  const int c = ROW == 64 ? c0 ^ (r0 & 7) : c0 ^ ((r0 >> 1) & 3);
+  const uint32_t at0 = tile + r0 * (ROW * 2) + c * 16;
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      uint32_t h[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = gg_part(v[u][i]);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at0 + u * 2048 + k * plane),
+                   "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
+                   : "memory");
+    }
   }
 }
 
 // T: the caller's element type; D: the operands' 16-bit type; PA, PB: planes of the two operands;
 // PD: planes of dgate and dup that a backward GG_PROJ writes (their products take PA = PD).
 template <int MODE, int NB, int PA, int PB, typename T, typename D, int PD, bool BACK>
-__global__ void __launch_bounds__(kGgThreads, 1)
+__global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
     gated_gemm_kernel(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
                       const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
                       const __grid_constant__ GgArgs A) {
@@ -382,18 +462,25 @@ __global__ void __launch_bounds__(kGgThreads, 1)
   constexpr int BN = MODE == GG_PROJ ? NB / 2 : NB;  // output columns of a tile
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t raw_full[kGgRaw], raw_empty[kGgRaw];
   __shared__ uint32_t tmem_base;
   __shared__ __align__(16) float bias_tile[kGgEpiWarps][MODE == GG_PROJ ? 2 * (BN / 2) : 4];
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t raw = base + STAGES * S::kStage;
+  constexpr int BK = S::kBK;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 1 + (S::kSplit ? kGgSplitWarps : 0));
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 1);
       mbar_init(&acc_empty[s], kGgEpiWarps);
+    }
+    for (int s = 0; s < kGgRaw; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], kGgSplitWarps);
     }
     fence_barrier_init();
   }
@@ -407,20 +494,35 @@ __global__ void __launch_bounds__(kGgThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
+      int it = 0, raw_it = 0;
       for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
         const GgItem I = gg_item(A, item);
         const int n0 = I.nt * BN;
         for (int kb = I.kb0; kb < I.kb1; ++kb, ++it) {
           const int s = it % STAGES;
+          const int seg = kb >= A.kblocks;
+          const int k0 = (kb - seg * A.kblocks) * BK;
+          if constexpr (S::kSplit) {
+            const int q = it % kGgRaw;
+            if (it >= kGgRaw) ok = mbar_wait_bounded(&raw_empty[q], ((it / kGgRaw) & 1) ^ 1);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&raw_full[q], S::kRaw);
+            const uint32_t dst = raw + q * S::kRaw;
+            if constexpr (MODE == GG_PROJ) {
+              gg_tma(dst, &a0, k0, I.mt * kGgBM, 0, &raw_full[q]);
+            } else {
+#pragma unroll
+              for (int c = 0; c < NB / 64; ++c)
+                gg_tma(dst + c * BK * 64 * 4, &b0, n0 + c * 64, k0, 0, &raw_full[q]);
+            }
+            ++raw_it;
+          }
           if (it >= STAGES) ok = mbar_wait_bounded(&empty[s], ((it / STAGES) & 1) ^ 1);
           if (!ok) break;
-          const int seg = kb >= A.kblocks;
-          const int k0 = (kb - seg * A.kblocks) * kGgBK;
           const uint32_t sa = base + s * S::kStage, sb = sa + PA * S::kABytes;
-          mbar_arrive_expect_tx(&full[s], S::kStage);
+          mbar_arrive_expect_tx(&full[s], S::kTmaBytes);
 #pragma unroll
-          for (int p = 0; p < PA; ++p) {
+          for (int p = 0; p < (S::kTmaA ? PA : 0); ++p) {
             const uint32_t dst = sa + p * S::kABytes;
             if constexpr (MODE == GG_DW) {
 #pragma unroll
@@ -429,22 +531,22 @@ __global__ void __launch_bounds__(kGgThreads, 1)
                 const int m0 = A.half_tiles == 0
                                    ? 0
                                    : (I.mt - half * A.half_tiles) * kGgBM + q * 64;
-                gg_tma(dst + q * 8192, half ? &a1 : &a0, m0, k0, p, &full[s]);
+                gg_tma(dst + q * (BK * 128), half ? &a1 : &a0, m0, k0, p, &full[s]);
               }
             } else {
               gg_tma(dst, MODE == GG_DX && seg ? &a1 : &a0, k0, I.mt * kGgBM, p, &full[s]);
             }
           }
 #pragma unroll
-          for (int p = 0; p < PB; ++p) {
+          for (int p = 0; p < (S::kTmaB ? PB : 0); ++p) {
             const uint32_t dst = sb + p * S::kBBytes;
             if constexpr (MODE == GG_PROJ) {
               gg_tma(dst, &b0, k0, n0, p, &full[s]);
-              gg_tma(dst + BN * 128, &b1, k0, n0, p, &full[s]);
+              gg_tma(dst + BN * (2 * BK), &b1, k0, n0, p, &full[s]);
             } else {
 #pragma unroll
               for (int q = 0; q < NB / 64; ++q)
-                gg_tma(dst + q * 8192, MODE == GG_DX && seg ? &b1 : &b0, n0 + q * 64, k0, p,
+                gg_tma(dst + q * (BK * 128), MODE == GG_DX && seg ? &b1 : &b0, n0 + q * 64, k0, p,
                        &full[s]);
             }
           }
@@ -453,37 +555,40 @@ __global__ void __launch_bounds__(kGgThreads, 1)
       if (!ok) {
         atomicExch(A.err, DEV_WAIT_TIMEOUT);
         drain_ring<STAGES>(full, it);
+        if constexpr (S::kSplit) drain_ring<kGgRaw>(raw_full, raw_it);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t kAdvA = MODE == GG_DW ? 2048 >> 4 : 32 >> 4;
-      constexpr uint32_t kAdvB = MODE == GG_PROJ ? 32 >> 4 : 2048 >> 4;
-      int it = 0, buf_it = 0;
-      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-        const GgItem I = gg_item(A, item);
-        for (int w0 = I.kb0; ok && w0 < I.kb1;) {
-          const int w1 = WIN ? min(I.kb1, w0 + kGgWindow) : I.kb1;
-          const int buf = buf_it & 1;
-          if (buf_it >= 2) ok = mbar_wait_bounded(&acc_empty[buf], ((buf_it >> 1) & 1) ^ 1);
-          if (!ok) break;
+    // The whole warp walks the stages and one elected lane issues: its waits must not part the warp.
+    auto wait = [&](uint64_t* bar, int parity) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
+      return ok;
+    };
+    constexpr uint32_t kAdvA = MODE == GG_DW ? 2048 >> 4 : 32 >> 4;
+    constexpr uint32_t kAdvB = MODE == GG_PROJ ? 32 >> 4 : 2048 >> 4;
+    int it = 0, buf_it = 0;
+    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      const GgItem I = gg_item(A, item);
+      for (int w0 = I.kb0; ok && w0 < I.kb1;) {
+        const int w1 = WIN ? min(I.kb1, w0 + S::kWindow) : I.kb1;
+        const int buf = buf_it & 1;
+        if (buf_it >= 2 && !wait(&acc_empty[buf], ((buf_it >> 1) & 1) ^ 1)) break;
+        const uint32_t d = tmem + buf * S::kAcc;
+        for (int kb = w0; kb < w1; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!wait(&full[s], (it / STAGES) & 1)) break;
           tc_fence_after();
-          const uint32_t d = tmem + buf * S::kAcc;
-          for (int kb = w0; kb < w1; ++kb, ++it) {
-            const int s = it % STAGES;
-            ok = mbar_wait_bounded(&full[s], (it / STAGES) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t sa = base + s * S::kStage, sb = sa + PA * S::kABytes;
+          const uint32_t sa = base + s * S::kStage, sb = sa + PA * S::kABytes;
+          if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < kGgBK / 16; ++ks) {
+            for (int ks = 0; ks < BK / 16; ++ks) {
               uint64_t da[PA], db[PB];
 #pragma unroll
               for (int p = 0; p < PA; ++p)
-                da[p] = gg_desc(sa + p * S::kABytes, MODE == GG_DW ? 8192 : 16, 1024) + ks * kAdvA;
+                da[p] = gg_desc<MODE == GG_DW, BK>(sa + p * S::kABytes) + ks * kAdvA;
 #pragma unroll
               for (int p = 0; p < PB; ++p)
-                db[p] = gg_desc(sb + p * S::kBBytes, MODE == GG_PROJ ? 16 : 8192, 1024) + ks * kAdvB;
+                db[p] = gg_desc<MODE != GG_PROJ, BK>(sb + p * S::kBBytes) + ks * kAdvB;
               const uint32_t first = kb > w0 || ks > 0;
               if constexpr (WIN) {
                 const uint32_t ds = d + NB;
@@ -500,11 +605,35 @@ __global__ void __launch_bounds__(kGgThreads, 1)
               }
             }
             mma_commit(&empty[s]);
+            if (kb + 1 == w1) mma_commit(&acc_full[buf]);
           }
+          __syncwarp();
+        }
+        ++buf_it;
+        w0 = w1;
+      }
+    }
+    if (!ok && lane == 0) atomicExch(A.err, DEV_WAIT_TIMEOUT);
+  } else if (S::kSplit && warp >= 2 + kGgEpiWarps) {
+    if constexpr (S::kSplit) {
+      const int tid = threadIdx.x - 32 * (2 + kGgEpiWarps);
+      int it = 0;
+      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const GgItem I = gg_item(A, item);
+        for (int kb = I.kb0; kb < I.kb1; ++kb, ++it) {
+          const int s = it % STAGES, q = it % kGgRaw;
+          ok = mbar_wait_bounded(&raw_full[q], (it / kGgRaw) & 1);
+          if (ok && it >= STAGES) ok = mbar_wait_bounded(&empty[s], ((it / STAGES) & 1) ^ 1);
           if (!ok) break;
-          mma_commit(&acc_full[buf]);
-          ++buf_it;
-          w0 = w1;
+          const uint32_t tile = base + s * S::kStage + (MODE == GG_PROJ ? 0 : PA * S::kABytes);
+          gg_split_tile<S::kPlane / 2048, MODE == GG_PROJ ? BK : 64>(tid, raw + q * S::kRaw, tile,
+                                                                     S::kPlane);
+          fence_proxy_async_smem();
+          __syncwarp();  // the warp's reads of the fp32 tile are done too
+          if (lane == 0) {
+            mbar_arrive(&raw_empty[q]);
+            mbar_arrive(&full[s]);
+          }
         }
       }
       if (!ok) atomicExch(A.err, DEV_WAIT_TIMEOUT);
@@ -577,7 +706,7 @@ __global__ void __launch_bounds__(kGgThreads, 1)
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int i = 0; i < HC; ++i) acc[r][i] = 0.f;
-        for (int w0 = I.kb0; ok && w0 < I.kb1; w0 += kGgWindow) {
+        for (int w0 = I.kb0; ok && w0 < I.kb1; w0 += S::kWindow) {
           const int buf = buf_it & 1;
           ok = mbar_wait_bounded(&acc_full[buf], (buf_it >> 1) & 1);
           if (!ok) break;

@@ -572,8 +572,7 @@ template <int LEAF, int D>
 static int launch_ig(InputGradArgs& A, cudaStream_t st) {
   if (A.cols > 4) {
     constexpr auto kernel = input_gradient_tc_kernel<LEAF, D>;
-    GPB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        IgcShape<D>::kSmem));
+    GPB_TRY(allow_smem<kernel>(IgcShape<D>::kSmem));
     kernel<<<dim3((unsigned)ceil_div(A.n, 128), kIgCluster), kIgcThreads, IgcShape<D>::kSmem, st>>>(A);
   } else {
     constexpr int R = D <= 16 ? 2 : 1;  // a row's state is 2 D + 8 values
