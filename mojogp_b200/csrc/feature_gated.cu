@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__
     for (int k = 0; k < 3; ++k) {
       uint32_t h[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = gg_part(x[i]);
+      for (int i = 0; i < 4; ++i) h[i] = gg_part<D>(x[i]);
       *reinterpret_cast<uint4*>(dst + k * A.rows[o] * A.ld) = make_uint4(h[0], h[1], h[2], h[3]);
     }
   }

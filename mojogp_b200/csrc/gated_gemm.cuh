@@ -26,6 +26,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "features.cuh"
 #include "tcgen05.cuh"
 
@@ -201,10 +203,19 @@ __device__ __forceinline__ void gg_tma(uint32_t dst, const CUtensorMap* map, int
 // 2^-25). A value beyond bf16's largest (3.3895e38) or not finite leaves a NaN remainder, and makes
 // what depends on it NaN; looking for one per pair cost a branch that halted the splitting warps
 // (a stage took 6 us where its MMAs take 0.8).
+template <typename D>
 __device__ __forceinline__ uint32_t gg_part(float2& x) {
-  const uint32_t h = bits32(__float22bfloat162_rn(x));
-  x.x -= __uint_as_float(h << 16);
-  x.y -= __uint_as_float(h & 0xFFFF0000u);
+  uint32_t h;
+  float2 f;
+  if constexpr (std::is_same<D, __nv_bfloat16>::value) {
+    h = bits32(__float22bfloat162_rn(x));
+    f = make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xFFFF0000u));
+  } else {
+    const __half2 v = __float22half2_rn(x);
+    h = bits32(v);
+    f = __half22float2(v);
+  }
+  x = __ffma2_rn(f, make_float2(-1.f, -1.f), x);
   return h;
 }
 
@@ -373,17 +384,25 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int64_t m, int64_
     // stores are whole sectors; columns up to the leading dimension past N are never read.
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float(&v)[16] = h == 0 ? g : u;
+      const float(&v)[16] = h == 0 ? g : u;
       D* dst = (D*)A.out[h] + m * A.out_ld + n;
+      float2 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = make_float2(v[2 * i], v[2 * i + 1]);
 #pragma unroll
       for (int p = 0; p < PD; ++p) {
-        gg_store<D>(dst + p * A.plane, v, left, 2);
-        if (p + 1 < PD) {
+        uint32_t w[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float r = v[i] - to_f(from_f<D>(v[i]));
-            v[i] = r == r && fabsf(r) < 3.0e38f ? r : 0.f;
-          }
+        for (int i = 0; i < 8; ++i) w[i] = gg_part<D>(x[i]);
+        if (left >= 16) {
+          store32(dst + p * A.plane, make_uint4(w[0], w[1], w[2], w[3]),
+                  make_uint4(w[4], w[5], w[6], w[7]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i < left)
+              reinterpret_cast<uint16_t*>(dst + p * A.plane)[i] =
+                  (uint16_t)(w[i / 2] >> (16 * (i & 1)));
         }
       }
     }
@@ -441,7 +460,7 @@ __device__ __forceinline__ void gg_split_tile(int tid, uint32_t raw, uint32_t ti
     for (int k = 0; k < 3; ++k) {
       uint32_t h[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = gg_part(v[u][i]);
+      for (int i = 0; i < 4; ++i) h[i] = gg_part<__nv_bfloat16>(v[u][i]);
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at0 + u * 2048 + k * plane),
                    "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
                    : "memory");

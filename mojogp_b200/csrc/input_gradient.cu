@@ -254,11 +254,7 @@ __device__ __forceinline__ void igc_split(const InputGradArgs& A, const float* l
   for (int k = 0; k < 3; ++k) {
     uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      h[i] = bits32(__float22bfloat162_rn(x[i]));
-      x[i].x -= __uint_as_float(h[i] << 16);
-      x[i].y -= __uint_as_float(h[i] & 0xFFFF0000u);
-    }
+    for (int i = 0; i < 4; ++i) h[i] = gg_part<__nv_bfloat16>(x[i]);
     *reinterpret_cast<uint4*>(dst + k * kIgcPlane) = make_uint4(h[0], h[1], h[2], h[3]);
   }
 }
