@@ -401,18 +401,26 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
   return P;
 }
 
-template <int MODE, int NB, int PA, int PB, typename T, typename D, int PD, bool BACK>
+template <int MODE, int NB, int PA, int PB, typename T, typename D, int PD, bool BACK, int CTAS = 1>
 static int gg_launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0,
-                     const CUtensorMap& b1, GgArgs& G, cudaStream_t st) {
-  using S = GgShape<MODE, NB, PA, PB>;
-  constexpr auto kernel = gated_gemm_kernel<MODE, NB, PA, PB, T, D, PD, BACK>;
+                     const CUtensorMap& b1, GgArgs G, cudaStream_t st) {
+  using S = GgShape<MODE, NB, PA, PB, CTAS>;
+  // CTA pairs once they still leave an item for every pair of SMs.
+  if constexpr (CTAS == 1 && NB == 256 && PA == 1 && PB == 1) {
+    if (G.tiles_m > 1 && ceil_div(G.tiles_m, 2) * (int64_t)G.tiles_n * G.splits >= kFeatSMs / 2)
+      return gg_launch<MODE, NB, PA, PB, T, D, PD, BACK, 2>(a0, a1, b0, b1, G, st);
+  }
+  constexpr auto kernel = gated_gemm_kernel<MODE, NB, PA, PB, T, D, PD, BACK, CTAS>;
   GPB_TRY(allow_smem<kernel>(S::kSmem));
   void* err = nullptr;
   GPB_CHECK_CUDA(cudaGetSymbolAddress(&err, g_feature_err));
   G.err = (int*)err;
-  G.idesc = gg_idesc(std::is_same<D, __nv_bfloat16>::value, MODE == GG_DW, MODE != GG_PROJ, NB);
+  G.idesc = gg_idesc(std::is_same<D, __nv_bfloat16>::value, MODE == GG_DW, MODE != GG_PROJ, NB,
+                     CTAS * kGgBM);
+  G.tiles_m = (int32_t)ceil_div(G.tiles_m, CTAS);
   const int64_t items = (int64_t)G.tiles_m * G.tiles_n * G.splits;
-  kernel<<<(unsigned)std::min<int64_t>(items, kFeatSMs), S::kThreads, S::kSmem, st>>>(a0, a1, b0, b1, G);
+  const unsigned grid = CTAS * (unsigned)std::min<int64_t>(items, kFeatSMs / CTAS);
+  kernel<<<grid, S::kThreads, S::kSmem, st>>>(a0, a1, b0, b1, G);
   GPB_CHECK_CUDA(cudaGetLastError());
   return GPB_OK;
 }

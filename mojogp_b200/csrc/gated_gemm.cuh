@@ -18,6 +18,12 @@
 // per MMA, so after every kGgWindow blocks of the reduction the epilogue warps add both accumulators
 // to registers in fp32 and the MMAs start again from zero.
 //
+// Wide 16-bit products run on CTA pairs (cta_group::2): one MMA covers 256 rows x 256 columns, each
+// CTA holds its 128 rows of A and half of B's rows, so a stage is 32 KB per CTA where a CTA alone loads
+// 48 KB for the same MMA time: alone, the tile stream ran at 73 bytes per clock and SM, which is what
+// the L2 gives, with the tensor pipe 76 % busy. The pair's even CTA issues the MMAs; both CTAs' loads
+// complete on its barriers, and its commits arrive at both.
+//
 // 10 warps: TMA producer, MMA issuer, 8 epilogue warps (TMEM lane quadrant = warp % 4, two warps
 // share a quadrant's columns). Tiles move by cp.async.bulk.tensor into 128-byte-swizzled stages;
 // accumulators are double-buffered so that a tile's epilogue runs under the next tile's MMAs. Every
@@ -125,7 +131,7 @@ constexpr int kGgGroup = 8;      // row tiles that share a pass over the column 
 
 struct GgArgs {
   int64_t M, N;        // output rows and columns (GG_PROJ: of one projection; GG_DW: of one weight)
-  int32_t tiles_m;     // over all halves
+  int32_t tiles_m;     // row tiles over all halves (pairs of them for CTA pairs)
   int32_t tiles_n;
   int32_t half_tiles;  // GG_DW: row tiles of one weight; 0 = both weights' rows share a tile
   int32_t kblocks;     // stages of one segment
@@ -164,9 +170,10 @@ __device__ __forceinline__ uint64_t gg_desc(uint32_t addr) {
 }
 
 // kind::f16 instruction descriptor: D f32, A and B of one 16-bit type.
-__host__ __device__ constexpr uint32_t gg_idesc(bool bf16, bool a_mn, bool b_mn, int n) {
+__host__ __device__ constexpr uint32_t gg_idesc(bool bf16, bool a_mn, bool b_mn, int n,
+                                                int m = kGgBM) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) |
-         ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kGgBM >> 4) << 24);
+         ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 // One lane of a converged warp. A tcgen05.mma under `elect.sync` takes its descriptors from uniform
@@ -186,6 +193,62 @@ __device__ __forceinline__ void gg_mma(uint32_t d, uint64_t a, uint64_t b, uint3
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The pair's forms.
+__device__ __forceinline__ void gg_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void gg_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], "
+      "%1;" ::"r"(smem_addr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void gg_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   smem_addr(dst_smem)),
+               "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void gg_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
+               : "memory");
+}
+// The same shared-memory object in the pair's even CTA.
+__device__ __forceinline__ uint32_t gg_leader_addr(const void* p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
+  return a;
+}
+__device__ __forceinline__ void gg_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t gg_cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void gg_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// A load of a pair: into this CTA's memory, completing on a barrier of the even CTA.
+__device__ __forceinline__ void gg_tma_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1,
+                                            int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
       : "memory");
 }
 
@@ -222,13 +285,14 @@ __device__ __forceinline__ uint32_t gg_part(float2& x) {
 // fp32 x is GG_PROJ's A operand and GG_DW's B operand.
 __host__ __device__ constexpr bool gg_splits(int mode, int pb) { return pb == 3 && mode != GG_DX; }
 
-template <int MODE, int NB, int PA, int PB>
+template <int MODE, int NB, int PA, int PB, int CTAS>
 struct GgShape {
   static constexpr bool kSplit = gg_splits(MODE, PB);
+  static_assert(CTAS == 1 || (PA == 1 && PB == 1 && NB == 256), "pairs: wide 16-bit products");
   static constexpr int kBK = kSplit ? kGgSplitBK : kGgBK;
   static constexpr int kThreads = 32 * (2 + kGgEpiWarps + (kSplit ? kGgSplitWarps : 0));
   static constexpr int kABytes = kGgBM * kBK * 2;
-  static constexpr int kBBytes = NB * kBK * 2;
+  static constexpr int kBBytes = NB / CTAS * kBK * 2;
   static constexpr int kStage = PA * kABytes + PB * kBBytes;
   // The part of a stage that TMA writes; the splitting warps write the rest, from a ring of fp32 tiles.
   static constexpr bool kTmaA = !(kSplit && MODE == GG_PROJ), kTmaB = !(kSplit && MODE == GG_DW);
@@ -411,7 +475,7 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int64_t m, int64_
 
 // Epilogue of 16 columns of a GG_DX or GG_DW tile.
 template <typename T, int MODE>
-__device__ __forceinline__ void gg_plain_store(const GgArgs& A, const GgItem& I, int lane_row,
+__device__ __forceinline__ void gg_plain_store(const GgArgs& A, int split, int mt, int lane_row,
                                                int64_t n, float (&v)[16]) {
   int half = 0;
   int64_t m;
@@ -420,15 +484,15 @@ __device__ __forceinline__ void gg_plain_store(const GgArgs& A, const GgItem& I,
       half = lane_row >> 6;
       m = lane_row & 63;
     } else {
-      half = I.mt >= A.half_tiles;
-      m = (int64_t)(I.mt - half * A.half_tiles) * kGgBM + lane_row;
+      half = mt >= A.half_tiles;
+      m = (int64_t)(mt - half * A.half_tiles) * kGgBM + lane_row;
     }
   } else {
-    m = (int64_t)I.mt * kGgBM + lane_row;
+    m = (int64_t)mt * kGgBM + lane_row;
   }
   if (m >= A.M || n >= A.N) return;
   if (MODE == GG_DW && A.splits > 1) {
-    float* dst = A.partial + (((int64_t)I.split * 2 + half) * A.M + m) * A.N + n;
+    float* dst = A.partial + (((int64_t)split * 2 + half) * A.M + m) * A.N + n;
     gg_store<float>(dst, v, A.N - n, A.N % 8 == 0 ? 2 : 0);
   } else if (A.out[half]) {
     gg_store<T>((T*)A.out[half] + m * A.out_ld + n, v, A.N - n, A.vec);
@@ -470,12 +534,14 @@ __device__ __forceinline__ void gg_split_tile(int tid, uint32_t raw, uint32_t ti
 
 // T: the caller's element type; D: the operands' 16-bit type; PA, PB: planes of the two operands;
 // PD: planes of dgate and dup that a backward GG_PROJ writes (their products take PA = PD).
-template <int MODE, int NB, int PA, int PB, typename T, typename D, int PD, bool BACK>
-__global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
+template <int MODE, int NB, int PA, int PB, typename T, typename D, int PD, bool BACK, int CTAS>
+__global__ void __cluster_dims__(CTAS, 1, 1)
+    __launch_bounds__((GgShape<MODE, NB, PA, PB, CTAS>::kThreads), 1)
     gated_gemm_kernel(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
                       const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
                       const __grid_constant__ GgArgs A) {
-  using S = GgShape<MODE, NB, PA, PB>;
+  using S = GgShape<MODE, NB, PA, PB, CTAS>;
+  constexpr bool PAIR = CTAS == 2;
   constexpr int STAGES = S::kStages;
   constexpr bool WIN = S::kWindowed;
   constexpr int BN = MODE == GG_PROJ ? NB / 2 : NB;  // output columns of a tile
@@ -495,7 +561,7 @@ __global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], kGgEpiWarps);
+      mbar_init(&acc_empty[s], CTAS * kGgEpiWarps);
     }
     for (int s = 0; s < kGgRaw; ++s) {
       mbar_init(&raw_full[s], 1);
@@ -503,18 +569,29 @@ __global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
     }
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(&tmem_base, 512);
+  const int rank = PAIR ? (int)gg_cluster_rank() : 0;
+  if (warp == 1) {
+    if constexpr (PAIR)
+      gg_alloc_pair(&tmem_base, 512);
+    else
+      tmem_alloc(&tmem_base, 512);
+  }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (PAIR)
+    gg_cluster_sync();  // the other CTA's barriers are initialised, too
+  else
+    __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base;
+  // A pair works on one item: two row tiles of one column tile.
+  const int64_t first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
   const int64_t items = (int64_t)A.tiles_m * A.tiles_n * A.splits;
   bool ok = true;
 
   if (warp == 0) {
     if (lane == 0) {
       int it = 0, raw_it = 0;
-      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      for (int64_t item = first; ok && item < items; item += step) {
         const GgItem I = gg_item(A, item);
         const int n0 = I.nt * BN;
         for (int kb = I.kb0; kb < I.kb1; ++kb, ++it) {
@@ -539,105 +616,128 @@ __global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
           if (it >= STAGES) ok = mbar_wait_bounded(&empty[s], ((it / STAGES) & 1) ^ 1);
           if (!ok) break;
           const uint32_t sa = base + s * S::kStage, sb = sa + PA * S::kABytes;
-          mbar_arrive_expect_tx(&full[s], S::kTmaBytes);
+          const int mt = I.mt * CTAS + rank;
+          // Both CTAs' bytes are expected by the even one (the odd one's may come first).
+          uint32_t pair_bar = 0;
+          if constexpr (PAIR) pair_bar = gg_leader_addr(&full[s]);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * S::kTmaBytes);
+          auto tma = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+            if constexpr (PAIR)
+              gg_tma_pair(dst, map, c0, c1, c2, pair_bar);
+            else
+              gg_tma(dst, map, c0, c1, c2, &full[s]);
+          };
 #pragma unroll
           for (int p = 0; p < (S::kTmaA ? PA : 0); ++p) {
             const uint32_t dst = sa + p * S::kABytes;
             if constexpr (MODE == GG_DW) {
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const int half = A.half_tiles == 0 ? q : I.mt >= A.half_tiles;
-                const int m0 = A.half_tiles == 0
-                                   ? 0
-                                   : (I.mt - half * A.half_tiles) * kGgBM + q * 64;
-                gg_tma(dst + q * (BK * 128), half ? &a1 : &a0, m0, k0, p, &full[s]);
+                const int half = A.half_tiles == 0 ? q : mt >= A.half_tiles;
+                const int m0 =
+                    A.half_tiles == 0 ? 0 : (mt - half * A.half_tiles) * kGgBM + q * 64;
+                tma(dst + q * (BK * 128), half ? &a1 : &a0, m0, k0, p);
               }
             } else {
-              gg_tma(dst, MODE == GG_DX && seg ? &a1 : &a0, k0, I.mt * kGgBM, p, &full[s]);
+              tma(dst, MODE == GG_DX && seg ? &a1 : &a0, k0, mt * kGgBM, p);
             }
           }
 #pragma unroll
           for (int p = 0; p < (S::kTmaB ? PB : 0); ++p) {
             const uint32_t dst = sb + p * S::kBBytes;
             if constexpr (MODE == GG_PROJ) {
-              gg_tma(dst, &b0, k0, n0, p, &full[s]);
-              gg_tma(dst + BN * (2 * BK), &b1, k0, n0, p, &full[s]);
+              if constexpr (PAIR) {  // one projection's rows each
+                tma(dst, rank ? &b1 : &b0, k0, n0, p);
+              } else {
+                tma(dst, &b0, k0, n0, p);
+                tma(dst + BN * (2 * BK), &b1, k0, n0, p);
+              }
             } else {
 #pragma unroll
-              for (int q = 0; q < NB / 64; ++q)
-                gg_tma(dst + q * (BK * 128), MODE == GG_DX && seg ? &b1 : &b0, n0 + q * 64, k0, p,
-                       &full[s]);
+              for (int q = 0; q < NB / CTAS / 64; ++q)
+                tma(dst + q * (BK * 128), MODE == GG_DX && seg ? &b1 : &b0,
+                    n0 + (rank * (NB / CTAS) + q * 64), k0, p);
             }
           }
         }
       }
       if (!ok) {
         atomicExch(A.err, DEV_WAIT_TIMEOUT);
-        drain_ring<STAGES>(full, it);
+        if (rank == 0) drain_ring<STAGES>(full, it);  // a pair's loads complete on the even CTA
         if constexpr (S::kSplit) drain_ring<kGgRaw>(raw_full, raw_it);
       }
     }
   } else if (warp == 1) {
-    // The whole warp walks the stages and one elected lane issues: its waits must not part the warp.
-    auto wait = [&](uint64_t* bar, int parity) {
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
-      return ok;
-    };
-    constexpr uint32_t kAdvA = MODE == GG_DW ? 2048 >> 4 : 32 >> 4;
-    constexpr uint32_t kAdvB = MODE == GG_PROJ ? 32 >> 4 : 2048 >> 4;
-    int it = 0, buf_it = 0;
-    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-      const GgItem I = gg_item(A, item);
-      for (int w0 = I.kb0; ok && w0 < I.kb1;) {
-        const int w1 = WIN ? min(I.kb1, w0 + S::kWindow) : I.kb1;
-        const int buf = buf_it & 1;
-        if (buf_it >= 2 && !wait(&acc_empty[buf], ((buf_it >> 1) & 1) ^ 1)) break;
-        const uint32_t d = tmem + buf * S::kAcc;
-        for (int kb = w0; kb < w1; ++kb, ++it) {
-          const int s = it % STAGES;
-          if (!wait(&full[s], (it / STAGES) & 1)) break;
-          tc_fence_after();
-          const uint32_t sa = base + s * S::kStage, sb = sa + PA * S::kABytes;
-          if (elect_one()) {
+    if (rank == 0) {
+      // The whole warp walks the stages and one elected lane issues: its waits must not part the warp.
+      auto wait = [&](uint64_t* bar, int parity) {
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
+        return ok;
+      };
+      constexpr uint32_t kAdvA = MODE == GG_DW ? 2048 >> 4 : 32 >> 4;
+      constexpr uint32_t kAdvB = MODE == GG_PROJ ? 32 >> 4 : 2048 >> 4;
+      int it = 0, buf_it = 0;
+      for (int64_t item = first; ok && item < items; item += step) {
+        const GgItem I = gg_item(A, item);
+        for (int w0 = I.kb0; ok && w0 < I.kb1;) {
+          const int w1 = WIN ? min(I.kb1, w0 + S::kWindow) : I.kb1;
+          const int buf = buf_it & 1;
+          if (buf_it >= 2 && !wait(&acc_empty[buf], ((buf_it >> 1) & 1) ^ 1)) break;
+          const uint32_t d = tmem + buf * S::kAcc;
+          for (int kb = w0; kb < w1; ++kb, ++it) {
+            const int s = it % STAGES;
+            if (!wait(&full[s], (it / STAGES) & 1)) break;
+            tc_fence_after();
+            const uint32_t sa = base + s * S::kStage, sb = sa + PA * S::kABytes;
+            if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < BK / 16; ++ks) {
-              uint64_t da[PA], db[PB];
+              for (int ks = 0; ks < BK / 16; ++ks) {
+                uint64_t da[PA], db[PB];
 #pragma unroll
-              for (int p = 0; p < PA; ++p)
-                da[p] = gg_desc<MODE == GG_DW, BK>(sa + p * S::kABytes) + ks * kAdvA;
+                for (int p = 0; p < PA; ++p)
+                  da[p] = gg_desc<MODE == GG_DW, BK>(sa + p * S::kABytes) + ks * kAdvA;
 #pragma unroll
-              for (int p = 0; p < PB; ++p)
-                db[p] = gg_desc<MODE != GG_PROJ, BK>(sb + p * S::kBBytes) + ks * kAdvB;
-              const uint32_t first = kb > w0 || ks > 0;
-              if constexpr (WIN) {
-                const uint32_t ds = d + NB;
-                gg_mma(ds, da[2], db[0], A.idesc, first);
-                gg_mma(ds, da[1], db[1], A.idesc, 1);
-                gg_mma(ds, da[0], db[2], A.idesc, 1);
-                gg_mma(ds, da[1], db[0], A.idesc, 1);
-                gg_mma(ds, da[0], db[1], A.idesc, 1);
-                gg_mma(d, da[0], db[0], A.idesc, first);
+                for (int p = 0; p < PB; ++p)
+                  db[p] = gg_desc<MODE != GG_PROJ, BK>(sb + p * S::kBBytes) + ks * kAdvB;
+                const uint32_t first_mma = kb > w0 || ks > 0;
+                if constexpr (WIN) {
+                  const uint32_t ds = d + NB;
+                  gg_mma(ds, da[2], db[0], A.idesc, first_mma);
+                  gg_mma(ds, da[1], db[1], A.idesc, 1);
+                  gg_mma(ds, da[0], db[2], A.idesc, 1);
+                  gg_mma(ds, da[1], db[0], A.idesc, 1);
+                  gg_mma(ds, da[0], db[1], A.idesc, 1);
+                  gg_mma(d, da[0], db[0], A.idesc, first_mma);
+                } else {
+#pragma unroll
+                  for (int p = PA - 1; p >= 0; --p)
+                    if constexpr (PAIR)
+                      gg_mma_pair(d, da[p], db[0], A.idesc, first_mma);
+                    else
+                      gg_mma(d, da[p], db[0], A.idesc, p == PA - 1 ? first_mma : 1);
+                }
+              }
+              if constexpr (PAIR) {
+                gg_commit_pair(&empty[s]);
+                if (kb + 1 == w1) gg_commit_pair(&acc_full[buf]);
               } else {
-#pragma unroll
-                for (int p = PA - 1; p >= 0; --p)
-                  gg_mma(d, da[p], db[0], A.idesc, p == PA - 1 ? first : 1);
+                mma_commit(&empty[s]);
+                if (kb + 1 == w1) mma_commit(&acc_full[buf]);
               }
             }
-            mma_commit(&empty[s]);
-            if (kb + 1 == w1) mma_commit(&acc_full[buf]);
+            __syncwarp();
           }
-          __syncwarp();
+          ++buf_it;
+          w0 = w1;
         }
-        ++buf_it;
-        w0 = w1;
       }
+      if (!ok && lane == 0) atomicExch(A.err, DEV_WAIT_TIMEOUT);
     }
-    if (!ok && lane == 0) atomicExch(A.err, DEV_WAIT_TIMEOUT);
   } else if (S::kSplit && warp >= 2 + kGgEpiWarps) {
     if constexpr (S::kSplit) {
       const int tid = threadIdx.x - 32 * (2 + kGgEpiWarps);
       int it = 0;
-      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+      for (int64_t item = first; ok && item < items; item += step) {
         const GgItem I = gg_item(A, item);
         for (int kb = I.kb0; kb < I.kb1; ++kb, ++it) {
           const int s = it % STAGES, q = it % kGgRaw;
@@ -662,9 +762,10 @@ __global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
     const int lane_row = quad * 32 + lane;
     constexpr int HC = BN / 2;  // output columns of this warp
     int buf_it = 0;
-    for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+    for (int64_t item = first; ok && item < items; item += step) {
       const GgItem I = gg_item(A, item);
-      const int64_t m = (int64_t)I.mt * kGgBM + lane_row;
+      const int mt = I.mt * CTAS + rank;
+      const int64_t m = (int64_t)mt * kGgBM + lane_row;
       const int64_t n = (int64_t)I.nt * BN + half * HC;
       float* bias = bias_tile[warp - 2];
       GgRow<T> dy, dy_next;
@@ -679,7 +780,7 @@ __global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
         __syncwarp();
         if constexpr (BACK) {
           dy_next.load(A, m, n);
-          if (A.col_sums) col_sums = A.col_sums + ((int64_t)I.mt * 4 + quad) * 2 * A.N;
+          if (A.col_sums && (int64_t)mt * kGgBM < A.M) col_sums = A.col_sums + ((int64_t)mt * 4 + quad) * 2 * A.N;
         }
       }
       if constexpr (!WIN) {
@@ -709,12 +810,17 @@ __global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
             } else {
               float v[16];
               tmem_ld16(t + c, v);
-              gg_plain_store<T, MODE>(A, I, lane_row, n + c, v);
+              gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v);
             }
           }
           tc_fence_before();
           __syncwarp();  // also: this tile's biases are read before the next tile's are written
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          if (lane == 0) {
+            if constexpr (PAIR)
+              gg_arrive_cluster(gg_leader_addr(&acc_empty[buf]));
+            else
+              mbar_arrive(&acc_empty[buf]);
+          }
           ++buf_it;
         }
       } else {
@@ -765,7 +871,7 @@ __global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
               gg_proj_store<T, D, PD, BACK>(A, m, n + c, bias + c, HC, dy, col_sums, lane, v[0],
                                             v[R - 1]);
             } else {
-              gg_plain_store<T, MODE>(A, I, lane_row, n + c, v[0]);
+              gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v[0]);
             }
           }
           __syncwarp();
@@ -775,9 +881,17 @@ __global__ void __launch_bounds__((GgShape<MODE, NB, PA, PB>::kThreads), 1)
     if (!ok) atomicExch(A.err, DEV_WAIT_TIMEOUT);
   }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (PAIR)
+    gg_cluster_sync();  // the even CTA's MMAs read the odd one's memory, and its barriers are used
+  else
+    __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 1) {
+    if constexpr (PAIR)
+      gg_dealloc_pair(tmem, 512);
+    else
+      tmem_dealloc(tmem, 512);
+  }
 }
 
 }  // namespace gpb

@@ -264,6 +264,13 @@ def test_gated_unit(ft, rows, inner, outer, dtype):
     gated_case(ft, rows, inner, outer, dtype, act, bias=(rows + outer) % 2 == 0)
 
 
+# Sizes whose products all run on CTA pairs (16-bit), with an odd number of row tiles and ragged edges.
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,inner,outer", [(2660, 1800, 1000), (9500, 264, 1200), (2561, 1928, 1024)])
+def test_gated_unit_large(ft, rows, inner, outer, dtype):
+    gated_case(ft, rows, inner, outer, dtype, "gelu", True)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid", "tanh"])
 @pytest.mark.parametrize("rows", [5, 150])
