@@ -230,8 +230,10 @@ __device__ __forceinline__ uint32_t gg_leader_addr(const void* p) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
   return a;
 }
+// The even CTA's barrier learns that TMEM was read; nothing in memory is handed over (a cluster-wide
+// release would wait for the epilogue's stores).
 __device__ __forceinline__ void gg_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ uint32_t gg_cluster_rank() {
   uint32_t r;
@@ -791,6 +793,18 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
           const uint32_t t = tmem + buf * S::kAcc + ((uint32_t)quad << 21) + half * HC;
 #pragma unroll 1
           for (int c = 0; c < HC; c += 16) {
+            // The accumulator is free once its last columns are in registers, before they are worked on.
+            auto release = [&]() {
+              if (c + 16 < HC) return;
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                if constexpr (PAIR)
+                  gg_arrive_cluster(gg_leader_addr(&acc_empty[buf]));
+                else
+                  mbar_arrive(&acc_empty[buf]);
+              }
+            };
             if constexpr (MODE == GG_PROJ) {
               uint32_t rg[16], ru[16];
               tmem_ld16_async(t + c, rg);
@@ -800,6 +814,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
                 if (c + 16 < HC) dy_next.load(A, m, n + c + 16);
               }
               tmem_wait_ld();
+              release();
               float g[16], u[16];
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
@@ -810,17 +825,11 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
             } else {
               float v[16];
               tmem_ld16(t + c, v);
+              release();
               gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v);
             }
           }
-          tc_fence_before();
-          __syncwarp();  // also: this tile's biases are read before the next tile's are written
-          if (lane == 0) {
-            if constexpr (PAIR)
-              gg_arrive_cluster(gg_leader_addr(&acc_empty[buf]));
-            else
-              mbar_arrive(&acc_empty[buf]);
-          }
+          __syncwarp();  // this tile's biases are read before the next tile's are written
           ++buf_it;
         }
       } else {
