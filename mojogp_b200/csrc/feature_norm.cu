@@ -70,6 +70,24 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Rows in flight per thread in the rings below: what two resident blocks' rings have room for.
+template <int R>
+constexpr int kNormAhead = R >= 4 ? 2 : 4;
+constexpr int kNormScalarAhead = 2;
+
+// Shared memory of one unaligned row: its 16-byte blocks as they lie, the ones it only partly fills
+// included. (A block that holds any of a row's bytes is inside the allocation that holds the row.)
+__host__ __device__ constexpr int norm_slot_bytes(int cols, int es) {
+  return (cols * es + 15 + 15) / 16 * 16;
+}
+template <typename T>
+__device__ __forceinline__ void norm_copy_row(const T* p, int cols, char* slot, int lane, int tpr) {
+  const char* first = reinterpret_cast<const char*>((uintptr_t)p & ~(uintptr_t)15);
+  const int blocks = (int)(((uintptr_t)(p + cols) - (uintptr_t)first + 15) >> 4);
+  const uint32_t dst = smem_addr(slot);
+  for (int v = lane; v < blocks; v += tpr) copy16(dst + 16 * v, first + 16 * v);
+}
+
 // Rows of at most 32 vectors: TPR threads (part of a warp) hold one vector each of RPT rows, so that
 // RPT loads are in flight where one row's would leave HBM idle.
 template <typename T, typename W, int VEC, int RPT>
@@ -135,40 +153,31 @@ __global__ void __launch_bounds__(128) norm_forward_rows_kernel(const NormArgs A
   }
 }
 
-template <typename T, typename W, int VEC, int R>
-__global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs A) {
+// A row per TPR threads, R single elements each (unaligned rows, when they are few).
+template <typename T, typename W, int R>
+__global__ void __launch_bounds__(512) norm_forward_kernel(const NormArgs A) {
   const int tpr = A.tpr;
   const int lane = threadIdx.x & (tpr - 1);
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
   const bool live = row < A.rows;
   const T* x = (const T*)A.x + (live ? row : 0) * A.x_ld;
-  float v[R][VEC];
-  float s[1] = {0.f}, q[1] = {0.f};
+  float v[R], s[1] = {0.f}, q[1] = {0.f};
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int c = (r * tpr + lane) * VEC;
-    if (live && c < A.cols) {
-      load_vec<T, VEC>(x + c, v[r]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[r][i] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) s[0] += v[r][i];
+    const int c = r * tpr + lane;
+    v[r] = live && c < A.cols ? to_f(x[c]) : 0.f;
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r) s[0] += v[r];
   row_sum(s, tpr, 0);
-  const float mean = s[0] / (float)A.cols;
+  const float inv = 1.f / (float)A.cols, mean = s[0] * inv;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const bool in = (r * tpr + lane) * VEC < A.cols;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      v[r][i] -= mean;
-      q[0] = in ? fmaf(v[r][i], v[r][i], q[0]) : q[0];
-    }
+    v[r] -= mean;
+    q[0] = r * tpr + lane < A.cols ? fmaf(v[r], v[r], q[0]) : q[0];
   }
   row_sum(q, tpr, 1);
-  const float rstd = inv_sqrt(q[0] / (float)A.cols + A.eps);
+  const float rstd = inv_sqrt(fmaf(q[0], inv, A.eps));
   if (!live) return;
   if (lane == 0) {
     if (A.mean) A.mean[row] = mean;
@@ -177,19 +186,158 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs A) {
   T* y = (T*)A.out + row * A.out_ld;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int c = (r * tpr + lane) * VEC;
+    const int c = r * tpr + lane;
     if (c >= A.cols) break;
-    float w[VEC], b[VEC], o[VEC];
+    float o = v[r] * rstd;
+    if (A.w) o *= to_f(((const W*)A.w)[c]);
+    if (A.b) o += to_f(((const W*)A.b)[c]);
+    y[c] = from_f<T>(o);
+  }
+}
+
+// A row per TPR threads, R 16-byte vectors each, kept as they came (half the registers of their fp32
+// values, so twice the rows in flight: those loads are what the kernel's rate depends on) and
+// converted in each of the three passes.
+template <typename T, typename W, int VEC, int R>
+__global__ void __launch_bounds__(512) norm_forward_vec_kernel(const NormArgs A) {
+  constexpr int P = VEC / 2;
+  const int tpr = A.tpr;
+  const int lane = threadIdx.x & (tpr - 1);
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+  const bool live = row < A.rows;
+  const int c0 = lane * VEC, dc = tpr * VEC;
+  const T* x = (const T*)A.x + (live ? row : 0) * A.x_ld + c0;
+  const T* tag = nullptr;
+  uint4 raw[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    raw[r] = live && c0 + r * dc < A.cols ? *reinterpret_cast<const uint4*>(x + r * dc)
+                                          : make_uint4(0, 0, 0, 0);
+  const float inv = 1.f / (float)A.cols;
+  float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float2 v[P];
+    unpack16(raw[r], v, tag);
+#pragma unroll
+    for (int i = 0; i < P; ++i) s2 = __fadd2_rn(s2, v[i]);
+  }
+  float s[1] = {s2.x + s2.y};
+  row_sum(s, tpr, 0);
+  const float mean = s[0] * inv;
+  const float2 neg_mean = make_float2(-mean, -mean);
+  float2 q2 = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (c0 + r * dc < A.cols) {
+      float2 v[P];
+      unpack16(raw[r], v, tag);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float2 d = __fadd2_rn(v[i], neg_mean);
+        q2 = __ffma2_rn(d, d, q2);
+      }
+    }
+  }
+  float q[1] = {q2.x + q2.y};
+  row_sum(q, tpr, 1);
+  const float rstd = inv_sqrt(fmaf(q[0], inv, A.eps));
+  if (!live) return;
+  if (lane == 0) {
+    if (A.mean) A.mean[row] = mean;
+    if (A.rstd) A.rstd[row] = rstd;
+  }
+  T* y = (T*)A.out + row * A.out_ld + c0;
+  const float2 scale = make_float2(rstd, rstd);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int c = c0 + r * dc;
+    if (c >= A.cols) break;
+    float2 v[P];
+    unpack16(raw[r], v, tag);
+    float w[VEC], b[VEC];
     if (A.w) load_vec<W, VEC>((const W*)A.w + c, w);
     if (A.b) load_vec<W, VEC>((const W*)A.b + c, b);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      o[i] = v[r][i] * rstd;
-      if (A.w) o[i] *= w[i];
-      if (A.b) o[i] += b[i];
+    for (int i = 0; i < P; ++i) {
+      v[i] = __fmul2_rn(__fadd2_rn(v[i], neg_mean), scale);
+      if (A.w) v[i] = __fmul2_rn(v[i], make_float2(w[2 * i], w[2 * i + 1]));
+      if (A.b) v[i] = __fadd2_rn(v[i], make_float2(b[2 * i], b[2 * i + 1]));
     }
-    store_vec<T, VEC>(y + c, o);
+    *reinterpret_cast<uint4*>(y + r * dc) = pack16(v, tag);
   }
+}
+
+// Many unaligned rows: a fixed number of blocks walks them, copied to shared memory as they lie
+// kNormScalarAhead rows ahead (60000 x 777 bf16: 180 us with single-element loads, 103 us). Aligned
+// rows do not gain from such a ring: its blocks are too few for the two reductions of a row.
+template <typename T, typename W, int R>
+__global__ void __launch_bounds__(512) norm_forward_ring_kernel(const NormArgs A) {
+  extern __shared__ __align__(16) char norm_ring[];
+  constexpr int SLOTS = kNormScalarAhead + 1;
+  const int tpr = A.tpr;
+  const int lane = threadIdx.x & (tpr - 1);
+  const int groups = blockDim.x / tpr, group = threadIdx.x / tpr;
+  const int64_t step = (int64_t)gridDim.x * groups;
+  const int slot_bytes = norm_slot_bytes(A.cols, sizeof(T));
+  char* ring = norm_ring + group * SLOTS * slot_bytes;
+  auto fetch = [&](int64_t row, int s) {
+    if (row < A.rows)
+      norm_copy_row((const T*)A.x + row * A.x_ld, A.cols, ring + s * slot_bytes, lane, tpr);
+    copy_commit();
+  };
+  const int64_t first = (int64_t)blockIdx.x * groups + group;
+#pragma unroll
+  for (int s = 0; s < kNormScalarAhead; ++s) fetch(first + s * step, s);
+  const float inv = 1.f / (float)A.cols;
+  int at = 0;
+  for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows; base += step) {
+    const int64_t row = base + group;
+    const bool live = row < A.rows;
+    copy_wait<kNormScalarAhead - 1>();
+    // Every thread's copies of this row are in, and every thread is done with the row before.
+    if (tpr > 32)
+      __syncthreads();
+    else
+      __syncwarp();
+    fetch(row + kNormScalarAhead * step, at == 0 ? SLOTS - 1 : at - 1);
+    const T* xg = (const T*)A.x + (live ? row : 0) * A.x_ld;
+    const T* x = reinterpret_cast<const T*>(ring + at * slot_bytes + ((uintptr_t)xg & 15));
+    float v[R], s[1] = {0.f}, q[1] = {0.f};
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int c = r * tpr + lane;
+      v[r] = live && c < A.cols ? to_f(x[c]) : 0.f;
+      s[0] += v[r];
+    }
+    row_sum(s, tpr, 0);
+    const float mean = s[0] * inv;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      v[r] -= mean;
+      q[0] = r * tpr + lane < A.cols ? fmaf(v[r], v[r], q[0]) : q[0];
+    }
+    row_sum(q, tpr, 1);
+    const float rstd = inv_sqrt(fmaf(q[0], inv, A.eps));
+    if (live) {
+      if (lane == 0) {
+        if (A.mean) A.mean[row] = mean;
+        if (A.rstd) A.rstd[row] = rstd;
+      }
+      T* y = (T*)A.out + row * A.out_ld;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int c = r * tpr + lane;
+        if (c >= A.cols) break;
+        float o = v[r] * rstd;
+        if (A.w) o *= to_f(((const W*)A.w)[c]);
+        if (A.b) o += to_f(((const W*)A.b)[c]);
+        y[c] = from_f<T>(o);
+      }
+    }
+    at = at + 1 == SLOTS ? 0 : at + 1;
+  }
+  copy_wait<0>();
 }
 
 // Rows too wide for registers: one block per row, x read three times (the second and third from L2).
@@ -277,10 +425,6 @@ __device__ __forceinline__ void norm_store_partial(const NormArgs& A, float* row
 // 125 us, issue-bound at 48 instructions an element; two vectors on pairs, which spread a row's
 // address, reduction and barrier work over twice the columns, 80 us (5.0 TB/s). What is left is the
 // chain of a row's reduction at two blocks per SM (121 registers); a deeper ring changes nothing.
-// Rows in flight per thread: what two resident blocks' rings have room for.
-template <int R>
-constexpr int kNormAhead = R >= 4 ? 2 : 4;
-
 template <typename T, typename W, int VEC, int R, bool PARAMS>
 __global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs A) {
   constexpr int SLOTS = kNormAhead<R> + 1;
@@ -412,25 +556,49 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs A) {
   }
 }
 
-// The same for rows that are not 16-byte aligned: one element at a time.
+// The same for rows that are not 16-byte aligned (an odd width, say): rows are copied to shared memory
+// kNormScalarAhead ahead (norm_copy_row) and their elements read from there, one per lane. Loads of
+// single elements leave too few bytes in flight: 60000 x 777 bf16 took 339 us, now 190 us.
 template <typename T, typename W, int R, bool PARAMS>
 __global__ void __launch_bounds__(512) norm_backward_scalar_kernel(const NormArgs A) {
-  extern __shared__ __align__(16) float row_sums[];  // [slots][2][cols]
+  extern __shared__ __align__(16) float row_sums[];  // the ring, then [slots][2][cols]
+  constexpr int SLOTS = kNormScalarAhead + 1;
   const int tpr = A.tpr;
   const int lane = threadIdx.x & (tpr - 1);
-  const int groups = blockDim.x / tpr;
+  const int groups = blockDim.x / tpr, group = threadIdx.x / tpr;
+  const int slot_bytes = norm_slot_bytes(A.cols, sizeof(T));
+  char* ring = reinterpret_cast<char*>(row_sums) + (int64_t)group * SLOTS * 2 * slot_bytes;
+  const int64_t step = (int64_t)gridDim.x * groups;
+  auto fetch = [&](int64_t row, int s) {
+    if (row < A.rows) {
+      norm_copy_row((const T*)A.x + row * A.x_ld, A.cols, ring + (2 * s) * slot_bytes, lane, tpr);
+      norm_copy_row((const T*)A.dy + row * A.dy_ld, A.cols, ring + (2 * s + 1) * slot_bytes, lane, tpr);
+    }
+    copy_commit();
+  };
   float dw[R][1], db[R][1];
 #pragma unroll
   for (int r = 0; r < R; ++r) dw[r][0] = db[r][0] = 0.f;
-  int flip = 0;
+  const int64_t row_first = (int64_t)blockIdx.x * groups + group;
+#pragma unroll
+  for (int s = 0; s < kNormScalarAhead; ++s) fetch(row_first + s * step, s);
+  int flip = 0, at = 0;
   const float inv = 1.f / (float)A.cols;
-  for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows;
-       base += (int64_t)gridDim.x * groups) {
-    const int64_t row = base + threadIdx.x / tpr;
+  for (int64_t base = (int64_t)blockIdx.x * groups; base < A.rows; base += step) {
+    const int64_t row = base + group;
     const bool live = row < A.rows;
+    copy_wait<kNormScalarAhead - 1>();
+    // Every thread's copies of this row are in, and every thread is done with the row before.
+    if (tpr > 32)
+      __syncthreads();
+    else
+      __syncwarp();
+    fetch(row + kNormScalarAhead * step, at == 0 ? SLOTS - 1 : at - 1);
     const int64_t rr = live ? row : 0;
-    const T* x = (const T*)A.x + rr * A.x_ld;
-    const T* dy = (const T*)A.dy + rr * A.dy_ld;
+    const T* xg = (const T*)A.x + rr * A.x_ld;
+    const T* dg = (const T*)A.dy + rr * A.dy_ld;
+    const T* x = reinterpret_cast<const T*>(ring + (2 * at) * slot_bytes + ((uintptr_t)xg & 15));
+    const T* dy = reinterpret_cast<const T*>(ring + (2 * at + 1) * slot_bytes + ((uintptr_t)dg & 15));
     const float mean = A.mean[rr], rstd = A.rstd[rr];
     float xh[R], g[R], sums[2] = {0.f, 0.f};
 #pragma unroll
@@ -465,7 +633,9 @@ __global__ void __launch_bounds__(512) norm_backward_scalar_kernel(const NormArg
         }
       }
     }
+    at = at + 1 == SLOTS ? 0 : at + 1;
   }
+  copy_wait<0>();
   if constexpr (PARAMS) norm_store_partial<1, R>(A, row_sums, dw, db);
 }
 
@@ -493,25 +663,36 @@ __global__ void __launch_bounds__(1024) norm_backward_wide_kernel(const NormArgs
   }
 }
 
-// dw and db partial sums of wide rows, column by column: blockIdx.x = 256 columns, blockIdx.y = a
-// range of rows.
-template <typename T>
-__global__ void __launch_bounds__(256) norm_params_wide_kernel(const NormArgs A) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+// dw and db partial sums of rows too wide for the above: a thread owns VEC columns and walks a range
+// of rows (blockIdx.y).
+template <typename T, int VEC>
+__global__ void __launch_bounds__(128) norm_params_wide_kernel(const NormArgs A) {
+  const int c = (blockIdx.x * 128 + threadIdx.x) * VEC;
   if (c >= A.cols) return;
   const int64_t per = (A.rows + gridDim.y - 1) / gridDim.y;
   const int64_t r0 = blockIdx.y * per;
   const int64_t r1 = r0 + per < A.rows ? r0 + per : A.rows;
-  float dw = 0.f, db = 0.f;
+  float dw[VEC], db[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) dw[i] = db[i] = 0.f;
+#pragma unroll 4
   for (int64_t r = r0; r < r1; ++r) {
-    const float g = to_f(((const T*)A.dy)[r * A.dy_ld + c]);
-    const float xh = (to_f(((const T*)A.x)[r * A.x_ld + c]) - A.mean[r]) * A.rstd[r];
-    dw = fmaf(g, xh, dw);
-    db += g;
+    float g[VEC], x[VEC];
+    load_vec<T, VEC>((const T*)A.dy + r * A.dy_ld + c, g);
+    load_vec<T, VEC>((const T*)A.x + r * A.x_ld + c, x);
+    const float mean = A.mean[r], rstd = A.rstd[r];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      dw[i] = fmaf(g[i], (x[i] - mean) * rstd, dw[i]);
+      db[i] += g[i];
+    }
   }
-  float* part = A.partial + (int64_t)blockIdx.y * 2 * A.cols;
-  part[c] = dw;
-  part[A.cols + c] = db;
+  float* part = A.partial + (int64_t)blockIdx.y * 2 * A.cols + c;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    part[i] = dw[i];
+    part[A.cols + i] = db[i];
+  }
 }
 
 template <typename W>
@@ -521,16 +702,20 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const float* __restrict
 }
 
 // ------------------------------------------------------------------ host
-// Threads per row and vectors per thread for `nvec` vectors: the widest part of a warp first, then
-// blocks of warps, growing R only once the row has `max_tpr` threads. Returns R, or 0 when the row
-// does not fit max_tpr threads with max_r vectors each.
-static int norm_shape(int64_t nvec, int max_tpr, int max_r, int* tpr) {
-  int t = 1;
-  while (t < max_tpr && t < nvec) t <<= 1;
-  int r = 1;
-  while ((int64_t)t * r < nvec) r <<= 1;
+// Threads per row and vectors per thread for `nvec` vectors. With many rows a row takes as few threads
+// as it can (a warp first, then max_r vectors per thread): its loads are in flight together and
+// fewer barriers join it. With few rows the widest spread answers soonest. Returns the vectors per
+// thread, or 0 when the row does not fit 512 threads with max_r vectors each.
+static int norm_shape(int64_t nvec, int max_r, int64_t rows, int* tpr) {
+  const bool few = rows < 4 * kFeatSMs;
+  int t = 1, r = 1;
+  while (t < 32 && t < nvec) t <<= 1;
+  if (!few)
+    while (r < max_r && (int64_t)t * r < nvec) r <<= 1;
+  while (t < 512 && (int64_t)t * r < nvec) t <<= 1;
+  while (r < max_r && (int64_t)t * r < nvec) r <<= 1;
   *tpr = t;
-  return r <= max_r ? r : 0;
+  return (int64_t)t * r >= nvec ? r : 0;
 }
 
 // Blocks of the backward pass (each writes one partial row of 2 cols sums), a function of the sizes
@@ -540,25 +725,64 @@ static int norm_blocks(int64_t rows, int64_t cols) {
   return (int)(b < rows ? b : (rows > 0 ? rows : 1));
 }
 
+template <typename T, typename W, int R>
+static int norm_forward_ring(const NormArgs& A, cudaStream_t st) {
+  const int threads = A.tpr > 256 ? A.tpr : 256;
+  const int groups = threads / A.tpr;
+  const size_t smem = (size_t)groups * (kNormScalarAhead + 1) * norm_slot_bytes(A.cols, sizeof(T));
+  constexpr auto kernel = norm_forward_ring_kernel<T, W, R>;
+  if (smem > 40 * 1024) GPB_TRY(allow_smem<kernel>(200 * 1024));
+  const int64_t grid = std::min<int64_t>(ceil_div(A.rows, groups), 4 * kFeatSMs);
+  kernel<<<(unsigned)grid, threads, smem, st>>>(A);
+  GPB_CHECK_CUDA(cudaGetLastError());
+  return GPB_OK;
+}
+
+template <typename T, typename W, int VEC, int R>
+static void norm_forward_run(const NormArgs& A, cudaStream_t st) {
+  const int threads = A.tpr > 128 ? A.tpr : 128;
+  const unsigned grid = (unsigned)ceil_div(A.rows, threads / A.tpr);
+  if constexpr (VEC > 1)
+    norm_forward_vec_kernel<T, W, VEC, R><<<grid, threads, 0, st>>>(A);
+  else
+    norm_forward_kernel<T, W, R><<<grid, threads, 0, st>>>(A);
+}
+
 template <typename T, typename W, int VEC>
 static int norm_forward_launch(NormArgs A, cudaStream_t st) {
-  constexpr int kMaxR = VEC == 1 ? 8 : 32 / VEC;
+  constexpr int kMaxR = 32 / VEC;
   int tpr = 1;
-  const int r = norm_shape(ceil_div(A.cols, VEC), 1024, kMaxR, &tpr);
+  const int64_t nvec = ceil_div(A.cols, VEC);
+  const int r = norm_shape(nvec, kMaxR, A.rows, &tpr);
   A.tpr = tpr;
+  if constexpr (VEC == 1) {
+    // The ring: many rows of at most 16 elements per thread.
+    int ring_tpr = 1;
+    const int ring_r = norm_shape(nvec, 16, A.rows, &ring_tpr);
+    if (nvec > 16 && A.rows >= 4 * kFeatSMs && ring_r) {
+      A.tpr = ring_tpr;
+      switch (ring_r) {
+        case 1: return norm_forward_ring<T, W, 1>(A, st);
+        case 2: return norm_forward_ring<T, W, 2>(A, st);
+        case 4: return norm_forward_ring<T, W, 4>(A, st);
+        case 8: return norm_forward_ring<T, W, 8>(A, st);
+        default: return norm_forward_ring<T, W, 16>(A, st);
+      }
+    }
+  }
   if (r == 0) {
     norm_forward_wide_kernel<T, W><<<(unsigned)A.rows, 1024, 0, st>>>(A);
-  } else if (tpr <= 32 && A.rows >= 4096) {
+  } else if (r == 1 && tpr <= 32 && A.rows >= 4096) {
     norm_forward_rows_kernel<T, W, VEC, 4>
         <<<(unsigned)ceil_div(A.rows, 128 / tpr * 4), 128, 0, st>>>(A);
   } else {
-    const int threads = tpr > 128 ? tpr : 128;
-    const unsigned grid = (unsigned)ceil_div(A.rows, threads / tpr);
     switch (r) {
-      case 1: norm_forward_kernel<T, W, VEC, 1><<<grid, threads, 0, st>>>(A); break;
-      case 2: norm_forward_kernel<T, W, VEC, 2><<<grid, threads, 0, st>>>(A); break;
-      case 4: norm_forward_kernel<T, W, VEC, 4><<<grid, threads, 0, st>>>(A); break;
-      default: norm_forward_kernel<T, W, VEC, kMaxR><<<grid, threads, 0, st>>>(A);
+      case 1: norm_forward_run<T, W, VEC, 1>(A, st); break;
+      case 2: norm_forward_run<T, W, VEC, 2>(A, st); break;
+      case 4: norm_forward_run<T, W, VEC, 4>(A, st); break;
+      case 8: norm_forward_run<T, W, VEC, 8 < kMaxR ? 8 : kMaxR>(A, st); break;
+      case 16: norm_forward_run<T, W, VEC, 16 < kMaxR ? 16 : kMaxR>(A, st); break;
+      default: norm_forward_run<T, W, VEC, kMaxR>(A, st);
     }
   }
   GPB_CHECK_CUDA(cudaGetLastError());
@@ -578,7 +802,11 @@ static int norm_backward_run(const NormArgs& A, int grid, int threads, cudaStrea
     if (smem > 40 * 1024) GPB_TRY(allow_smem<kernel>(kMost));
     kernel<<<grid, threads, smem, st>>>(A);
   } else {
-    norm_backward_scalar_kernel<T, W, R, PARAMS><<<grid, threads, smem, st>>>(A);
+    constexpr auto kernel = norm_backward_scalar_kernel<T, W, R, PARAMS>;
+    smem = std::max<size_t>(smem, (size_t)(threads / A.tpr) * (kNormScalarAhead + 1) * 2 *
+                                      norm_slot_bytes(A.cols, sizeof(T)));
+    if (smem > 40 * 1024) GPB_TRY(allow_smem<kernel>(200 * 1024));
+    kernel<<<grid, threads, smem, st>>>(A);
   }
   GPB_CHECK_CUDA(cudaGetLastError());
   return GPB_OK;
@@ -586,9 +814,9 @@ static int norm_backward_run(const NormArgs& A, int grid, int threads, cudaStrea
 
 template <typename T, typename W, int VEC, bool PARAMS>
 static int norm_backward_vec(NormArgs A, int* blocks, cudaStream_t st, bool* done) {
-  // 16 columns per thread in vectors, 8 otherwise (registers). A row takes as few threads as that
-  // allows, but a warp before a second vector.
-  constexpr int kMaxR = VEC == 1 ? 8 : 16 / VEC;
+  // 16 columns per thread, 32 of 16 bits without the weight gradients (registers, and the ring's shared
+  // memory). A row takes as few threads as that allows, but a warp before a second vector.
+  constexpr int kMaxR = (PARAMS || VEC == 1 || sizeof(T) == 4 ? 16 : 32) / VEC;
   const int64_t nvec = ceil_div(A.cols, VEC);
   int tpr = 1, r = 1;
   while (tpr < 32 && tpr < nvec) tpr <<= 1;
@@ -604,6 +832,7 @@ static int norm_backward_vec(NormArgs A, int* blocks, cudaStream_t st, bool* don
     case 1: return norm_backward_run<T, W, VEC, 1, PARAMS>(A, grid, threads, st);
     case 2: return norm_backward_run<T, W, VEC, 2 <= kMaxR ? 2 : kMaxR, PARAMS>(A, grid, threads, st);
     case 4: return norm_backward_run<T, W, VEC, 4 <= kMaxR ? 4 : kMaxR, PARAMS>(A, grid, threads, st);
+    case 8: return norm_backward_run<T, W, VEC, 8 <= kMaxR ? 8 : kMaxR, PARAMS>(A, grid, threads, st);
     default: return norm_backward_run<T, W, VEC, kMaxR, PARAMS>(A, grid, threads, st);
   }
 }
@@ -613,19 +842,18 @@ static int norm_backward_launch(NormArgs A, W* dw, W* db, cudaStream_t st) {
   const bool params = dw || db;
   int blocks = norm_blocks(A.rows, A.cols);
   bool done = false;
-  if (params)
-    GPB_TRY((norm_backward_vec<T, W, VEC, true>(A, &blocks, st, &done)));
-  else
-    GPB_TRY((norm_backward_vec<T, W, VEC, false>(A, &blocks, st, &done)));
+  if (params) GPB_TRY((norm_backward_vec<T, W, VEC, true>(A, &blocks, st, &done)));
   if (!done) {
     // The parameter sums read x and dy before dx may overwrite them in place.
     if (params) {
-      blocks = std::min(blocks, 64);
-      norm_params_wide_kernel<T>
-          <<<dim3((unsigned)ceil_div(A.cols, 256), blocks), 256, 0, st>>>(A);
+      blocks = (int)std::min<int64_t>(blocks, ceil_div(A.rows, 16));
+      norm_params_wide_kernel<T, VEC>
+          <<<dim3((unsigned)ceil_div(A.cols, 128 * VEC), blocks), 128, 0, st>>>(A);
       GPB_CHECK_CUDA(cudaGetLastError());
     }
-    if (A.out) {
+    int unused = norm_blocks(A.rows, A.cols);
+    if (A.out) GPB_TRY((norm_backward_vec<T, W, VEC, false>(A, &unused, st, &done)));
+    if (A.out && !done) {
       norm_backward_wide_kernel<T, W><<<(unsigned)A.rows, 1024, 0, st>>>(A);
       GPB_CHECK_CUDA(cudaGetLastError());
     }
