@@ -211,39 +211,84 @@ __global__ void __launch_bounds__(256) mm_join_kernel(const float* __restrict__ 
 }
 
 // Matrices to tensor-core operands, one per blockIdx.y: fp32 weights to three bf16 planes, or a matrix
-// whose rows are not 16-byte aligned to a copy whose are (`copy`). 8 output columns per thread;
-// columns up to ld are zeros.
+// whose rows are not 16-byte aligned to a copy whose are (`copy`). 8 output columns per step; columns
+// up to ld are zeros.
 struct PackArgs {
   const void* src[3];
   void* dst[3];
   int64_t rows[3], src_ld[3];
   int32_t copy[3];
   int64_t cols, ld;
+  int32_t lanes_log2;
 };
+// Threads: 2^lanes_log2 along a row, the others along rows, kPackRows of them each. 16-bit rows are read
+// as the 4-byte words they touch (5 for 8 elements), in reach of neighbours through L1, and shifted.
+constexpr int kPackRows = 4;
 template <typename T, typename D>
 __global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__ PackArgs A) {
   const int o = blockIdx.y;
-  const int64_t run = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t per = A.ld / 8;
-  if (run >= A.rows[o] * per) return;
-  const int64_t r = run / per, c = (run - r * per) * 8;
-  const T* src = (const T*)A.src[o] + r * A.src_ld[o] + c;
-  float v[8];
+  const int lanes = 1 << A.lanes_log2;
+  const int tx = threadIdx.x & (lanes - 1);
+  const int64_t row_step = 256 >> A.lanes_log2;
+  const int64_t row0 = blockIdx.x * row_step * kPackRows + (threadIdx.x >> A.lanes_log2);
+  if (row0 >= A.rows[o]) return;
+  for (int64_t c = tx * 8; c < A.ld; c += lanes * 8) {
+    uint32_t w[kPackRows][sizeof(T) == 4 ? 8 : 5];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = c + i < A.cols ? to_f(src[i]) : 0.f;
-  if (sizeof(T) == 2 || A.copy[o]) {
-    store_vec<T, 8>((T*)A.dst[o] + r * A.ld + c, v);
-  } else {
-    D* dst = (D*)A.dst[o] + r * A.ld + c;
-    float2 x[4];
+    for (int u = 0; u < kPackRows; ++u) {
+      const int64_t r = row0 + u * row_step;
+      const bool in = r < A.rows[o];
+      const T* src = (const T*)A.src[o] + r * A.src_ld[o] + c;
+      if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = make_float2(v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < 8; ++i)
+          w[u][i] = in && c + i < A.cols ? reinterpret_cast<const uint32_t*>(src)[i] : 0u;
+      } else {
+        const int64_t odd = ((uintptr_t)src >> 1) & 1;
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(src - odd);
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      uint32_t h[4];
+        for (int i = 0; i < 5; ++i) {  // a word is read when it holds an element of the row
+          const int64_t e = c + 2 * i - odd;
+          w[u][i] = in && e < A.cols && (i < 4 || odd) ? p[i] : 0u;
+        }
+      }
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = gg_part<D>(x[i]);
-      *reinterpret_cast<uint4*>(dst + k * A.rows[o] * A.ld) = make_uint4(h[0], h[1], h[2], h[3]);
+    for (int u = 0; u < kPackRows; ++u) {
+      const int64_t r = row0 + u * row_step;
+      if (r >= A.rows[o]) break;
+      if constexpr (sizeof(T) == 4) {
+        if (A.copy[o]) {
+          uint4* dst = reinterpret_cast<uint4*>((T*)A.dst[o] + r * A.ld + c);
+          dst[0] = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+          dst[1] = make_uint4(w[u][4], w[u][5], w[u][6], w[u][7]);
+        } else {
+          D* dst = (D*)A.dst[o] + r * A.ld + c;
+          float2 x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            x[i] = make_float2(__uint_as_float(w[u][2 * i]), __uint_as_float(w[u][2 * i + 1]));
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = gg_part<D>(x[i]);
+            *reinterpret_cast<uint4*>(dst + k * A.rows[o] * A.ld) =
+                make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        }
+      } else {
+        const T* src = (const T*)A.src[o] + r * A.src_ld[o] + c;
+        const uint32_t shift = ((uintptr_t)src & 2) * 8;
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          h[i] = __funnelshift_r(w[u][i], w[u][i + 1], shift);
+          // Columns past the row are zeros.
+          if (c + 2 * i + 1 >= A.cols) h[i] = c + 2 * i < A.cols ? h[i] & 0xFFFFu : 0u;
+        }
+        *reinterpret_cast<uint4*>((T*)A.dst[o] + r * A.ld + c) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
     }
   }
 }
@@ -263,15 +308,18 @@ struct JoinArgs {
 template <typename T>
 __global__ void __launch_bounds__(1024) gated_join_kernel(const __grid_constant__ JoinArgs A) {
   if (blockIdx.x < A.dw_blocks) {
-    const int64_t e = (int64_t)blockIdx.x * 1024 + threadIdx.x, one = A.M * A.N;
+    // The partial sums' rows are padded to a multiple of 16 columns.
+    const int64_t ld = (A.N + 15) / 16 * 16, one = A.M * ld;
+    const int64_t e = (int64_t)blockIdx.x * 1024 + threadIdx.x;
     if (e >= 2 * one) return;
+    const int half = e >= one;
+    const int64_t f = e - half * one, row = f / ld, col = f - row * ld;
+    T* dst = (T*)A.dw[half];
+    if (!dst || col >= A.N) return;
     float s = 0.f;
 #pragma unroll 4
     for (int64_t r = 0; r < A.ranges; ++r) s += A.dw_partial[r * 2 * one + e];
-    const int half = e >= one;
-    T* dst = (T*)A.dw[half];
-    const int64_t f = e - half * one;
-    if (dst) dst[(f / A.N) * A.dw_ld + f % A.N] = from_f<T>(s);
+    dst[row * A.dw_ld + col] = from_f<T>(s);
     return;
   }
   column_join<T>(A.col_sums, A.sum_rows, A.M, (T*)A.db[0], (T*)A.db[1], blockIdx.x - A.dw_blocks);
@@ -394,7 +442,7 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * kFeatSMs / tiles, kb * bk / 512));
     P.kb_per = (int)ceil_div(kb, want);
     P.splits = (int)ceil_div(kb, P.kb_per);
-    P.partial = take(at, P.splits > 1 ? P.splits * 2 * outer * inner * 4 : 0);
+    P.partial = take(at, P.splits > 1 ? P.splits * 2 * outer * round_up(inner, 16) * 4 : 0);
     P.sums = take(at, 4 * ceil_div(rows, kGgBM) * 2 * outer * 4);
   }
   P.total = at;
@@ -465,8 +513,10 @@ static int gated_operands(const GatedArgs& A, const GatedPlan& P, char* ws, Oper
   operand(A.wg, A.outer, A.w_ld, ws + P.wg, wg, kPlanes);
   operand(A.wu, A.outer, A.w_ld, ws + P.wu, wu, kPlanes);
   if (count) {
+    while (K.lanes_log2 < 8 && (8 << K.lanes_log2) < P.ldk) ++K.lanes_log2;
+    const int64_t per_block = (256 >> K.lanes_log2) * kPackRows;
     gated_pack_kernel<T, D>
-        <<<dim3((unsigned)ceil_div(most * (P.ldk / 8), 256), count), 256, 0, st>>>(K);
+        <<<dim3((unsigned)ceil_div(most, per_block), count), 256, 0, st>>>(K);
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   return GPB_OK;
@@ -674,7 +724,7 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
       J.dw_ld = R.dw_ld;
       J.dw[0] = R.dwg;
       J.dw[1] = R.dwu;
-      J.dw_blocks = ceil_div(2 * A.outer * A.inner, 1024);
+      J.dw_blocks = ceil_div(2 * A.outer * round_up(A.inner, 16), 1024);
     }
     J.col_sums = (const float*)(ws + P.sums);
     J.sum_rows = 4 * ceil_div(A.rows, kGgBM);

@@ -126,7 +126,7 @@ constexpr int kGgSplitBK = 32;   // the same where x is split: more and smaller 
 constexpr int kGgWindow = 256;   // depth between promotions of the fp32 variant
 constexpr int kGgEpiWarps = 8;
 constexpr int kGgSplitWarps = 4;
-constexpr int kGgRaw = 4;        // fp32 tiles in flight
+constexpr int kGgRaw = 3;        // fp32 tiles in flight (a fourth's memory is the rows' transpose)
 constexpr int kGgGroup = 8;      // row tiles that share a pass over the column tiles (L2 reuse)
 
 struct GgArgs {
@@ -303,7 +303,7 @@ struct GgShape {
   static constexpr int kRaw = kSplit ? 2 * kPlane : 0;
   static constexpr int kRest = kGgRaw * kRaw;
   static constexpr int kStages =
-      (208 * 1024 - kRest) / kStage < 8 ? (208 * 1024 - kRest) / kStage : 8;
+      (200 * 1024 - kRest) / kStage < 8 ? (200 * 1024 - kRest) / kStage : 8;
   static constexpr int kSmem = kStages * kStage + kRest + 1024;  // + alignment of the first stage
   static constexpr bool kWindowed = PB == 3;             // fp32 inputs
   static constexpr int kWindow = kGgWindow / kBK;        // stages between promotions
@@ -340,11 +340,39 @@ __device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b)
                : "memory");
 }
 
-// 16 columns of one row to the output's type; vec: 2 = 32-byte aligned, 1 = 16-byte, 0 = neither.
+// Unaligned rows go through a warp's own 32 x 16 tile of shared memory, so that 16 lanes share a row:
+// a lane's own row, element by element, makes every access 32 sectors of one element each.
+constexpr int kGgTileLd = 17;  // words per row of the tile
+constexpr int kGgTile = 32 * kGgTileLd;
+
+// 16 columns of the warp's 32 rows, of which lane holds its own row; rows start at `row0` (lane 0's).
 template <typename T>
-__device__ __forceinline__ void gg_store(T* dst, const float (&v)[16], int64_t left, int vec) {
+__device__ __forceinline__ void gg_store_rows(T* out, int64_t ld, int64_t row0, int64_t rows, int64_t n,
+                                              const float (&v)[16], int64_t left, float* tile,
+                                              int lane) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) tile[lane * kGgTileLd + i] = v[i];
+  __syncwarp();
+  const int c = lane & 15;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = 2 * i + (lane >> 4);
+    if (row0 + r < rows && c < left) out[(row0 + r) * ld + n + c] = from_f<T>(tile[r * kGgTileLd + c]);
+  }
+  __syncwarp();
+}
+
+// 16 columns of the lane's row m to the output's type; vec: 2 = 32-byte aligned rows, 1 = 16-byte, 0 =
+// neither. The whole warp takes part.
+template <typename T>
+__device__ __forceinline__ void gg_store(T* out, int64_t ld, int64_t m, int64_t rows, int64_t n,
+                                         const float (&v)[16], int64_t left, int vec, float* tile,
+                                         int lane) {
   constexpr int V = 16 / sizeof(T), Q = 16 / V;
+  if (left <= 0) return;
   if (vec && left >= 16) {
+    if (m >= rows) return;
+    T* dst = out + m * ld + n;
     uint4 raw[Q];
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
@@ -363,9 +391,7 @@ __device__ __forceinline__ void gg_store(T* dst, const float (&v)[16], int64_t l
       }
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < left) dst[i] = from_f<T>(v[i]);
+    gg_store_rows<T>(out, ld, m - lane, rows, n, v, left, tile, lane);
   }
 }
 
@@ -392,16 +418,29 @@ template <typename T>
 struct GgRow {
   static constexpr int kVecs = sizeof(T);  // 16 columns are 2 or 4 16-byte vectors
   uint4 raw[kVecs];
-  __device__ __forceinline__ void load(const GgArgs& A, int64_t m, int64_t n) {
+  __device__ __forceinline__ void load(const GgArgs& A, int64_t m, int64_t n, float* tile, int lane) {
     const T* src = (const T*)A.dout + m * A.dout_ld + n;
-    const int64_t left = m < A.M ? A.N - n : 0;
+    const int64_t left = A.N - n;
     if (A.vec && left >= 16) {
 #pragma unroll
-      for (int q = 0; q < kVecs; ++q) raw[q] = reinterpret_cast<const uint4*>(src)[q];
+      for (int q = 0; q < kVecs; ++q)
+        raw[q] = m < A.M ? reinterpret_cast<const uint4*>(src)[q] : make_uint4(0, 0, 0, 0);
     } else {
+      const int c = lane & 15;
+      const int64_t row0 = m - lane;
+      T* t = reinterpret_cast<T*>(tile);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = 2 * i + (lane >> 4);
+        t[r * kGgTileLd + c] = row0 + r < A.M && c < left
+                                   ? ((const T*)A.dout)[(row0 + r) * A.dout_ld + n + c]
+                                   : from_f<T>(0.f);
+      }
+      __syncwarp();
       T* e = reinterpret_cast<T*>(raw);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) e[i] = i < left ? src[i] : from_f<T>(0.f);
+      for (int i = 0; i < 16; ++i) e[i] = t[lane * kGgTileLd + i];
+      __syncwarp();
     }
   }
   __device__ __forceinline__ float get(int i) const {
@@ -414,7 +453,7 @@ struct GgRow {
 template <typename T, typename D, int PD, bool BACK>
 __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int64_t m, int64_t n,
                                               const float* bias, int step, const GgRow<T>& dy,
-                                              float* col_sums, int lane, float (&g)[16],
+                                              float* col_sums, float* tile, int lane, float (&g)[16],
                                               float (&u)[16]) {
   const int64_t left = A.N - n;
 #pragma unroll
@@ -427,10 +466,9 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int64_t m, int64_
   float value[16], slope[16];
   gated_act<BACK>(A.act, g, value, slope);
   if constexpr (!BACK) {
-    if (m >= A.M || left <= 0) return;
 #pragma unroll
     for (int i = 0; i < 16; ++i) g[i] = value[i] * u[i];
-    gg_store<T>((T*)A.out[0] + m * A.out_ld + n, g, left, A.vec);
+    gg_store<T>((T*)A.out[0], A.out_ld, m, A.M, n, g, left, A.vec, tile, lane);
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -460,25 +498,18 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int64_t m, int64_
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = gg_part<D>(x[i]);
-        if (left >= 16) {
-          store32(dst + p * A.plane, make_uint4(w[0], w[1], w[2], w[3]),
-                  make_uint4(w[4], w[5], w[6], w[7]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (i < left)
-              reinterpret_cast<uint16_t*>(dst + p * A.plane)[i] =
-                  (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-        }
+        store32(dst + p * A.plane, make_uint4(w[0], w[1], w[2], w[3]),
+                make_uint4(w[4], w[5], w[6], w[7]));
       }
     }
   }
 }
 
-// Epilogue of 16 columns of a GG_DX or GG_DW tile.
+// Epilogue of 16 columns of a GG_DX or GG_DW tile. The warp's 32 rows belong to one weight (halves of a
+// shared tile are 64 rows).
 template <typename T, int MODE>
 __device__ __forceinline__ void gg_plain_store(const GgArgs& A, int split, int mt, int lane_row,
-                                               int64_t n, float (&v)[16]) {
+                                               int64_t n, float (&v)[16], float* tile, int lane) {
   int half = 0;
   int64_t m;
   if constexpr (MODE == GG_DW) {
@@ -492,12 +523,22 @@ __device__ __forceinline__ void gg_plain_store(const GgArgs& A, int split, int m
   } else {
     m = (int64_t)mt * kGgBM + lane_row;
   }
-  if (m >= A.M || n >= A.N) return;
+  const int64_t left = A.N - n;
   if (MODE == GG_DW && A.splits > 1) {
-    float* dst = A.partial + (((int64_t)split * 2 + half) * A.M + m) * A.N + n;
-    gg_store<float>(dst, v, A.N - n, A.N % 8 == 0 ? 2 : 0);
+    // Rows padded to a multiple of 16: whole sectors, columns past N unread.
+    const int64_t ld = (A.N + 15) / 16 * 16;
+    if (m < A.M && left > 0) {
+      float* dst = A.partial + (((int64_t)split * 2 + half) * A.M + m) * ld + n;
+#pragma unroll
+      for (int q = 0; q < 16; q += 8)
+        store32(dst + q,
+                make_uint4(__float_as_uint(v[q]), __float_as_uint(v[q + 1]),
+                           __float_as_uint(v[q + 2]), __float_as_uint(v[q + 3])),
+                make_uint4(__float_as_uint(v[q + 4]), __float_as_uint(v[q + 5]),
+                           __float_as_uint(v[q + 6]), __float_as_uint(v[q + 7])));
+    }
   } else if (A.out[half]) {
-    gg_store<T>((T*)A.out[half] + m * A.out_ld + n, v, A.N - n, A.vec);
+    gg_store<T>((T*)A.out[half], A.out_ld, m, A.M, n, v, left, A.vec, tile, lane);
   }
 }
 
@@ -552,6 +593,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
   __shared__ __align__(8) uint64_t raw_full[kGgRaw], raw_empty[kGgRaw];
   __shared__ uint32_t tmem_base;
   __shared__ __align__(16) float bias_tile[kGgEpiWarps][MODE == GG_PROJ ? 2 * (BN / 2) : 4];
+  __shared__ float row_tile[kGgEpiWarps][kGgTile];
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t raw = base + STAGES * S::kStage;
   constexpr int BK = S::kBK;
@@ -770,6 +812,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
       const int64_t m = (int64_t)mt * kGgBM + lane_row;
       const int64_t n = (int64_t)I.nt * BN + half * HC;
       float* bias = bias_tile[warp - 2];
+      float* tile = row_tile[warp - 2];
       GgRow<T> dy, dy_next;
       float* col_sums = nullptr;
       if constexpr (MODE == GG_PROJ) {
@@ -781,7 +824,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
         }
         __syncwarp();
         if constexpr (BACK) {
-          dy_next.load(A, m, n);
+          dy_next.load(A, m, n, tile, lane);
           if (A.col_sums && (int64_t)mt * kGgBM < A.M) col_sums = A.col_sums + ((int64_t)mt * 4 + quad) * 2 * A.N;
         }
       }
@@ -811,7 +854,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
               tmem_ld16_async(t + BN + c, ru);
               if constexpr (BACK) {
                 dy = dy_next;
-                if (c + 16 < HC) dy_next.load(A, m, n + c + 16);
+                if (c + 16 < HC) dy_next.load(A, m, n + c + 16, tile, lane);
               }
               tmem_wait_ld();
               release();
@@ -821,12 +864,12 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
                 g[i] = __uint_as_float(rg[i]);
                 u[i] = __uint_as_float(ru[i]);
               }
-              gg_proj_store<T, D, PD, BACK>(A, m, n + c, bias + c, HC, dy, col_sums, lane, g, u);
+              gg_proj_store<T, D, PD, BACK>(A, m, n + c, bias + c, HC, dy, col_sums, tile, lane, g, u);
             } else {
               float v[16];
               tmem_ld16(t + c, v);
               release();
-              gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v);
+              gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v, tile, lane);
             }
           }
           __syncwarp();  // this tile's biases are read before the next tile's are written
@@ -875,12 +918,12 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
             if constexpr (MODE == GG_PROJ) {
               if constexpr (BACK) {
                 dy = dy_next;
-                if (c + 16 < HC) dy_next.load(A, m, n + c + 16);
+                if (c + 16 < HC) dy_next.load(A, m, n + c + 16, tile, lane);
               }
-              gg_proj_store<T, D, PD, BACK>(A, m, n + c, bias + c, HC, dy, col_sums, lane, v[0],
+              gg_proj_store<T, D, PD, BACK>(A, m, n + c, bias + c, HC, dy, col_sums, tile, lane, v[0],
                                             v[R - 1]);
             } else {
-              gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v[0]);
+              gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v[0], tile, lane);
             }
           }
           __syncwarp();
