@@ -435,7 +435,8 @@ int gpb_forward_matvec_noalloc(gpb_provider* p, float* out_dev, const float* v_d
  * provider (the input gradient aside): each call names its device and CUDA
  * stream (NULL = the legacy default stream), allocates nothing, never
  * synchronises, leaves the caller's current device as it was and can be
- * captured into a CUDA graph. Blocks are row-major with a leading dimension
+ * captured into a CUDA graph (after a first call on the device outside of any
+ * capture, which loads the kernel). Blocks are row-major with a leading dimension
  * (>= the column count, in elements) and unit column stride. Types are
  * GPB_DTYPE_*; statistics and sums are float32. A workspace is scratch of the
  * size the matching *_workspace call gives for the same sizes (it depends on

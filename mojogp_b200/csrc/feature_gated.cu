@@ -332,16 +332,17 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 static int encode_fn(EncodeTiled* fn) {
-  static EncodeTiled cached = nullptr;  // the same pointer whichever thread writes it
-  if (!cached) {
+  static std::atomic<EncodeTiled> cached{nullptr};
+  *fn = cached.load(std::memory_order_acquire);
+  if (!*fn) {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
     GPB_CHECK_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q));
     GPB_REQUIRE(p && q == cudaDriverEntryPointSuccess, GPB_ERR_CUDA,
                 "cuTensorMapEncodeTiled is not available");
-    cached = (EncodeTiled)p;
+    *fn = (EncodeTiled)p;
+    cached.store(*fn, std::memory_order_release);
   }
-  *fn = cached;
   return GPB_OK;
 }
 
@@ -513,7 +514,12 @@ static int gated_operands(const GatedArgs& A, const GatedPlan& P, char* ws, Oper
   operand(A.wg, A.outer, A.w_ld, ws + P.wg, wg, kPlanes);
   operand(A.wu, A.outer, A.w_ld, ws + P.wu, wu, kPlanes);
   if (count) {
-    while (K.lanes_log2 < 8 && (8 << K.lanes_log2) < P.ldk) ++K.lanes_log2;
+    // Lanes along a row: at least 8 (or the row), and as few idle ones in its last step as that allows.
+    const int64_t per = P.ldk / 8;
+    while (K.lanes_log2 < 3 && (1 << K.lanes_log2) < per) ++K.lanes_log2;
+    for (int l = K.lanes_log2 + 1; l <= 8; ++l)
+      if (round_up(per, (int64_t)1 << l) <= round_up(per, (int64_t)1 << K.lanes_log2))
+        K.lanes_log2 = l;
     const int64_t per_block = (256 >> K.lanes_log2) * kPackRows;
     gated_pack_kernel<T, D>
         <<<dim3((unsigned)ceil_div(most, per_block), count), 256, 0, st>>>(K);
@@ -757,8 +763,8 @@ static int gated_check(int32_t dtype, int64_t rows, int64_t inner, int64_t outer
   GPB_REQUIRE(rows >= 0 && inner >= 1 && outer >= 1, GPB_ERR_INVALID,
               "gated unit needs rows >= 0, inner >= 1 and outer >= 1, got %lld, %lld, %lld",
               (long long)rows, (long long)inner, (long long)outer);
-  GPB_REQUIRE(rows < ((int64_t)1 << 31) && inner <= (1 << 20) && outer <= (1 << 20),
-              GPB_ERR_INVALID, "gated unit sizes %lld, %lld, %lld are too large (2^31, 2^20, 2^20)",
+  GPB_REQUIRE(rows <= ((int64_t)1 << 30) && inner <= (1 << 20) && outer <= (1 << 20),
+              GPB_ERR_INVALID, "gated unit sizes %lld, %lld, %lld are too large (2^30, 2^20, 2^20)",
               (long long)rows, (long long)inner, (long long)outer);
   GPB_REQUIRE(rows * std::max(inner, outer) <= ((int64_t)1 << 40), GPB_ERR_INVALID,
               "gated unit of %lld rows is too large", (long long)rows);
@@ -867,8 +873,6 @@ int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t
   GPB_TRY(gated_check(dtype, rows, inner, outer));
   GPB_REQUIRE(activation >= GPB_ACT_SILU && activation <= GPB_ACT_TANH, GPB_ERR_INVALID,
               "unknown activation %d", activation);
-  GPB_REQUIRE(dx_dev || dw_gate_dev || dw_up_dev || db_gate_dev || db_up_dev, GPB_ERR_INVALID,
-              "no output was asked for");
   const int es = dtype_bytes(dtype);
   GPB_REQUIRE((!dx_dev || dx_ld >= inner) && (!(dw_gate_dev || dw_up_dev) || dw_ld >= inner),
               GPB_ERR_INVALID, "leading dimension below the column count");
@@ -885,6 +889,8 @@ int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t
       if (b) GPB_CHECK_CUDA(cudaMemsetAsync(b, 0, outer * es, st));
     return GPB_OK;
   }
+  GPB_REQUIRE(dx_dev || dw_gate_dev || dw_up_dev || db_gate_dev || db_up_dev, GPB_ERR_INVALID,
+              "no output was asked for");
   GPB_REQUIRE(dout_dev && x_dev && w_gate_dev && w_up_dev, GPB_ERR_INVALID, "null argument");
   GPB_REQUIRE(x_ld >= inner && w_ld >= inner && dout_ld >= outer, GPB_ERR_INVALID,
               "leading dimension below the column count");

@@ -921,6 +921,20 @@ int gpb_layer_norm(int32_t device, void* stream, int32_t dtype, int32_t param_dt
                   !overlaps(out_dev, span_bytes(rows, cols, out_ld, es), x_dev,
                             span_bytes(rows, cols, x_ld, es)),
               GPB_ERR_INVALID, "out overlaps x (in place needs the same pointer and stride)");
+  {
+    // The statistics are written while rows, weight and bias are still read.
+    const struct { const void* p; int64_t n; } used[] = {
+        {out_dev, span_bytes(rows, cols, out_ld, es)}, {x_dev, span_bytes(rows, cols, x_ld, es)},
+        {weight_dev, cols * ps}, {bias_dev, cols * ps}};
+    for (const auto& u : used)
+      GPB_REQUIRE(!overlaps(mean_dev, rows * 4, u.p, u.n) && !overlaps(rstd_dev, rows * 4, u.p, u.n),
+                  GPB_ERR_INVALID, "mean or rstd overlaps another argument");
+    GPB_REQUIRE(!overlaps(mean_dev, rows * 4, rstd_dev, rows * 4), GPB_ERR_INVALID,
+                "mean and rstd overlap");
+    for (int i = 2; i < 4; ++i)
+      GPB_REQUIRE(!overlaps(out_dev, used[0].n, used[i].p, used[i].n), GPB_ERR_INVALID,
+                  "out overlaps weight or bias");
+  }
   GPB_DEVICE_SCOPE(device);
   NormArgs A{};
   A.x = x_dev;
@@ -965,7 +979,6 @@ int gpb_layer_norm_backward(int32_t device, void* stream, int32_t dtype, int32_t
   GPB_TRY(norm_check(dtype, param_dtype, rows, cols));
   const bool params = dweight_dev || dbias_dev;
   const int es = dtype_bytes(dtype), ps = dtype_bytes(param_dtype);
-  GPB_REQUIRE(dx_dev || params, GPB_ERR_INVALID, "no output was asked for");
   GPB_REQUIRE(elem_aligned(dweight_dev, ps) && elem_aligned(dbias_dev, ps), GPB_ERR_INVALID,
               "pointer is not aligned to its element type");
   if (rows == 0) {
@@ -974,6 +987,7 @@ int gpb_layer_norm_backward(int32_t device, void* stream, int32_t dtype, int32_t
     if (dbias_dev) GPB_CHECK_CUDA(cudaMemsetAsync(dbias_dev, 0, cols * ps, (cudaStream_t)stream));
     return GPB_OK;
   }
+  GPB_REQUIRE(dx_dev || params, GPB_ERR_INVALID, "no output was asked for");
   GPB_REQUIRE(dout_dev && x_dev && mean_dev && rstd_dev, GPB_ERR_INVALID, "null argument");
   GPB_REQUIRE(dout_ld >= cols && x_ld >= cols && (!dx_dev || dx_ld >= cols), GPB_ERR_INVALID,
               "leading dimension below the %lld columns", (long long)cols);
@@ -994,6 +1008,20 @@ int gpb_layer_norm_backward(int32_t device, void* stream, int32_t dtype, int32_t
                 "the weight gradients need a workspace of %lld bytes, got %lld", (long long)need,
                 (long long)(workspace_dev ? workspace_bytes : 0));
     GPB_REQUIRE(aligned16(workspace_dev), GPB_ERR_INVALID, "workspace is not 16-byte aligned");
+    const int64_t pb = cols * ps;
+    const struct { const void* p; int64_t n; } in[] = {
+        {dout_dev, span_bytes(rows, cols, dout_ld, es)}, {x_dev, span_bytes(rows, cols, x_ld, es)},
+        {weight_dev, pb}, {mean_dev, rows * 4}, {rstd_dev, rows * 4}};
+    const struct { const void* p; int64_t n; } out[] = {
+        {dx_dev, dxb}, {dweight_dev, pb}, {dbias_dev, pb}, {workspace_dev, need}};
+    for (int o = 1; o < 4; ++o) {
+      for (const auto& i : in)
+        GPB_REQUIRE(!overlaps(out[o].p, out[o].n, i.p, i.n), GPB_ERR_INVALID,
+                    "dweight, dbias or the workspace overlaps an input");
+      for (int q = 0; q < o; ++q)
+        GPB_REQUIRE(!overlaps(out[o].p, out[o].n, out[q].p, out[q].n), GPB_ERR_INVALID,
+                    "two outputs (or an output and the workspace) overlap");
+    }
   }
   GPB_DEVICE_SCOPE(device);
   NormArgs A{};

@@ -476,6 +476,11 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int64_t m, int64_
       g[i] = d * u[i] * slope[i];
       u[i] = d * value[i];
     }
+    if (m >= A.M) {
+      // Past the last row x and dout are zeros, but a weight or bias that is not finite is not.
+#pragma unroll
+      for (int i = 0; i < 16; ++i) g[i] = u[i] = 0.f;
+    }
     if (col_sums && left > 0) {  // uniform over the warp
 #pragma unroll
       for (int h = 0; h < 2; ++h) {

@@ -87,12 +87,19 @@ def test_layer_norm_refusals(ft):
     refuse("overlaps", ft.layer_norm, FakeArray((4, 8), ptr=MB + 32), FakeArray((4, 8), ptr=MB))
     refuse("device array", ft.layer_norm, y, np.zeros((4, 8), np.float32))
     refuse("columns", ft.layer_norm, arr((4, 0), 2), arr((4, 0)))
+    refuse("mean or rstd overlaps", ft.layer_norm, y, x, mean=FakeArray((4,), ptr=y.data_ptr()))
+    refuse("overlap", ft.layer_norm, y, x, mean=arr((4,), 9), rstd=arr((4,), 9))
+    refuse("weight or bias", ft.layer_norm, y, x, FakeArray((8,), ptr=y.data_ptr()))
     m, r = arr((4,), 5), arr((4,), 6)
     d, dx = arr((4, 8), 7), arr((4, 8), 8)
     refuse("no output", ft.layer_norm_backward, None, d, x, m, r)
     refuse("workspace", ft.layer_norm_backward, dx, d, x, m, r, v, dweight=arr((8,), 9))
     refuse("workspace", ft.layer_norm_backward, dx, d, x, m, r, v, dweight=arr((8,), 9),
            workspace=arr((16,), 10, dtype="uint8"))
+    ws = arr((1 << 20,), 10, dtype="uint8")
+    refuse("two outputs", ft.layer_norm_backward, dx, d, x, m, r, v, dweight=arr((8,), 9),
+           dbias=arr((8,), 9), workspace=ws)
+    refuse("overlaps an input", ft.layer_norm_backward, dx, d, x, m, r, v, dweight=v, workspace=ws)
     refuse("overlaps", ft.layer_norm_backward, FakeArray((4, 8), ptr=MB + 32),
            FakeArray((4, 8), ptr=MB), x, m, r)
 
@@ -170,8 +177,8 @@ def test_workspace_sizes_follow_the_sizes_alone(gpb_lib):
     assert ft.layer_norm_workspace(100, 64) == ft.layer_norm_workspace(100, 64)
     assert ft.gated_unit_workspace(1, 64, 64, "bfloat16") == 0
     assert ft.gated_unit_workspace(100, 64, 64, "bfloat16", backward=True) >= 2 * 100 * 64 * 2
-    # float32 operands are three 16-bit planes
-    assert ft.gated_unit_workspace(100, 64, 64, "float32") >= 3 * 2 * (100 * 64 + 2 * 64 * 64)
+    # float32 weights are three 16-bit planes; x has room for an aligned copy
+    assert ft.gated_unit_workspace(100, 64, 64, "float32") >= 3 * 2 * 2 * 64 * 64 + 4 * 100 * 64
 
 
 def test_feature_map_refusals_and_shapes():

@@ -164,6 +164,7 @@ def test_layer_norm_options_and_repeats(ft):
     ft.layer_norm(e, e.clone(), one, zero)
     ft.layer_norm_backward(e, e, e, e[:, 0], e[:, 0], one, dweight=dw, dbias=db, workspace=ws)
     assert (dw == 0).all() and (db == 0).all()
+    ft.layer_norm_backward(e, e, e, e[:, 0], e[:, 0], one)  # and nothing else to do
     # A constant row has variance 0: rstd = 1 / sqrt(eps), y = bias.
     c = torch.full((2, 96), 3.25, device="cuda")
     ft.layer_norm(y[:2], c, one, zero, eps=1e-4, rstd=rstd[:2])
@@ -318,6 +319,43 @@ def test_gated_unit_no_rows(ft):
     ft.gated_unit_backward(o, e, w, w2, dw_gate=dw, dw_up=dw2, db_gate=db, db_up=db2)
     for v in (dw, dw2, db, db2):
         assert (v == 0).all()
+    ft.gated_unit_backward(o, e, w, w2, dx=e)
+
+
+def test_gated_unit_padding_stays_out_of_the_sums(ft):
+    """A bias that is not finite makes the outputs of its own column what the formula says; the rows
+    that pad the last tile add nothing to the bias gradients."""
+    for t in (torch.bfloat16, torch.float32):
+        x, wg, wu = randn(1, 70, 32, dtype=t), randn(2, 40, 32, dtype=t), randn(3, 40, 32, dtype=t)
+        bg, bu = torch.zeros(40, dtype=t, device="cuda"), torch.zeros(40, dtype=t, device="cuda")
+        bg[7] = float("inf")  # sigmoid 1, slope 0
+        dy = randn(4, 70, 40, dtype=t)
+        ws = torch.empty(ft.gated_unit_workspace(70, 32, 40, t, backward=True), dtype=torch.uint8,
+                         device="cuda")
+        out = torch.empty_like(dy)
+        ft.gated_unit(out, x, wg, wu, bg, bu, activation="sigmoid", workspace=ws)
+        dbg, dbu = torch.empty_like(bg), torch.empty_like(bu)
+        ft.gated_unit_backward(dy, x, wg, wu, bg, bu, db_gate=dbg, db_up=dbu, activation="sigmoid",
+                               workspace=ws)
+        assert torch.isfinite(out).all() and torch.isfinite(dbu).all() and dbg[7] == 0
+
+
+def test_non_finite_rows_stay_their_own(ft):
+    """A row with NaN or infinity leaves every other row's results as they were."""
+    for t in (torch.bfloat16, torch.float32):
+        x, wg, wu = randn(1, 300, 64, dtype=t), randn(2, 48, 64, dtype=t), randn(3, 48, 64, dtype=t)
+        ws = torch.empty(ft.gated_unit_workspace(300, 64, 48, t), dtype=torch.uint8, device="cuda")
+        a, b = (torch.empty((300, 48), dtype=t, device="cuda") for _ in range(2))
+        ft.gated_unit(a, x, wg, wu, workspace=ws)
+        na, nb = torch.empty_like(x), torch.empty_like(x)
+        ft.layer_norm(na, x)
+        x[17, 3], x[130, 63] = float("nan"), float("inf")
+        ft.gated_unit(b, x, wg, wu, workspace=ws)
+        ft.layer_norm(nb, x)
+        rest = torch.ones(300, dtype=torch.bool, device="cuda")
+        rest[17] = rest[130] = False
+        assert torch.equal(a[rest], b[rest]) and torch.equal(na[rest], nb[rest])
+        assert not torch.isfinite(b[17]).any() and not torch.isfinite(nb[17]).any()
 
 
 def test_gated_unit_gradient_against_differences(ft):
