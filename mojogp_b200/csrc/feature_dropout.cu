@@ -6,6 +6,9 @@
 // with key = seed and counter = (block, offset). It is kept iff its word >= floor(p 2^32), and a
 // kept element is x / (1 - p): out = kept ? x * (1 / (1 - p)) : 0, plus residual where given. A
 // dropped element is 0 whatever x holds (NaN and infinity included).
+//
+// HBM bound once the generator is out of the way: 16384 x 4096 bf16 with a residual (403 MB) 75 us,
+// 5.4 TB/s; with the round keys added up per thread and one run per thread it took 91 us.
 #include <cmath>
 
 #include "features.cuh"

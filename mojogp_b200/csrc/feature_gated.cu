@@ -399,7 +399,9 @@ static int64_t take(int64_t& at, int64_t bytes) {
 // 16-bit dgate and dup are kept as two planes (16 and more significant bits) up to this many
 // multiply-adds per product, as one above. One plane's rounding adds to the outputs' own: 1.4 times
 // their error, and more where few terms or few outputs average it. The second plane doubles the MMAs
-// of three of the four products: KTWO_NOTE
+// of three of the four products (backward, bf16 silu with bias: 2048 x 256 -> 512 49 us against 48 with
+// one plane, 4096 x 512 -> 512 55 against 47, 8192 x 512 -> 512 76 against 62). Above the bound it would
+// cost half the call's time or more, and the outputs' sums are long enough to average the rounding.
 constexpr int64_t kTwoPlanes = (int64_t)1 << 31;
 
 // Column tile of a GG_DX / GG_DW product with n output columns.

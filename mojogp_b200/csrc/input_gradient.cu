@@ -10,7 +10,8 @@
 //   few columns (up to 4): G_ij on the CUDA cores, two rows per thread;
 //   more: G = [a | b]' [b | a] is a product of depth 32, formed on the tensor cores (bf16 planes, six
 //     products, fp32-accurate) into TMEM while the CUDA cores run psi and the sums over j. On the CUDA
-//     cores G was 32 of the 74 FMAs of a pair: 2.0 ms at 20000 points in 8 dimensions.
+//     cores G was 32 of the 74 FMAs of a pair: 2.0 ms at 20000 points in 8 dimensions with 16 columns,
+//     0.71 ms here (Matern-5/2; the FP32 pipe alone would take 0.61).
 // Both work on fp32 pairs (FFMA2), split the columns of a row tile over a cluster of 8 blocks and
 // join through distributed shared memory, in block order: no workspace (a captured graph owns
 // nothing) and no atomics.
