@@ -44,44 +44,87 @@ struct GatedGrads {
 };
 
 // ------------------------------------------------------------- few rows
+// A weight vector, read once: past L1, which keeps x.
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 q;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+               : "l"(p));
+  return q;
+}
+template <typename T>
+__device__ __forceinline__ T load_once(const T* p) {
+  return *p;
+}
+// A vector's elements as pairs: 16 bytes, or one element and a zero.
+template <typename T, int P>
+__device__ __forceinline__ void to_pairs(const uint4& q, float2 (&o)[P]) {
+  unpack16(q, o, (const T*)nullptr);
+}
+template <typename T, int P>
+__device__ __forceinline__ void to_pairs(const T& q, float2 (&o)[P]) {
+  o[0] = make_float2(to_f(q), 0.f);
+}
+
 // One warp (WPO = 1) or one block (WPO = 8) per output column; lanes run along the weight row. BACK
-// writes dgate and dup [rows][outer] in fp32.
+// writes dgate and dup [rows][outer] in fp32. HBM bound: a lane issues U vectors of each weight row
+// before it uses the first.
 template <typename T, int ROWS, int VEC, int WPO, bool BACK>
 __global__ void __launch_bounds__(256) gated_rows_kernel(const GatedArgs A, float* dg, float* du) {
+  using Raw = typename std::conditional<VEC == 1, T, uint4>::type;
+  constexpr int P = VEC == 1 ? 1 : VEC / 2, U = 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t n = WPO == 1 ? (int64_t)blockIdx.x * 8 + warp : (int64_t)blockIdx.x;
-  float g[ROWS], u[ROWS];
+  float2 g2[ROWS], u2[ROWS];
 #pragma unroll
-  for (int m = 0; m < ROWS; ++m) g[m] = u[m] = 0.f;
+  for (int m = 0; m < ROWS; ++m) g2[m] = u2[m] = make_float2(0.f, 0.f);
   if (n < A.outer) {
     const T* wg = (const T*)A.wg + n * A.w_ld;
     const T* wu = (const T*)A.wu + n * A.w_ld;
     constexpr int kStep = (WPO == 1 ? 32 : 256) * VEC;
-#pragma unroll 4
-    for (int64_t k = (WPO == 1 ? lane : (int)threadIdx.x) * VEC; k < A.inner; k += kStep) {
-      float a[VEC], b[VEC];
-      load_vec<T, VEC>(wg + k, a);
-      load_vec<T, VEC>(wu + k, b);
+    for (int k0 = (WPO == 1 ? lane : (int)threadIdx.x) * VEC; k0 < A.inner; k0 += U * kStep) {
+      Raw a[U], b[U];
 #pragma unroll
-      for (int m = 0; m < ROWS; ++m) {
-        if (m < A.rows) {
-          float x[VEC];
-          load_vec<T, VEC>((const T*)A.x + m * A.x_ld + k, x);
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * kStep;
+        if (k < A.inner) {
+          a[u] = load_once((const Raw*)(wg + k));
+          b[u] = load_once((const Raw*)(wu + k));
+        }
+      }
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            g[m] = fmaf(x[i], a[i], g[m]);
-            u[m] = fmaf(x[i], b[i], u[m]);
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * kStep;
+        if (k < A.inner) {
+          float2 p[P], q[P];
+          to_pairs<T>(a[u], p);
+          to_pairs<T>(b[u], q);
+#pragma unroll
+          for (int m = 0; m < ROWS; ++m) {
+            if (m < A.rows) {
+              float2 x[P];
+              to_pairs<T>(*(const Raw*)((const T*)A.x + m * A.x_ld + k), x);
+#pragma unroll
+              for (int i = 0; i < P; ++i) {
+                g2[m] = __ffma2_rn(x[i], p[i], g2[m]);
+                u2[m] = __ffma2_rn(x[i], q[i], u2[m]);
+              }
+            }
           }
         }
       }
     }
   }
+  float g[ROWS], u[ROWS];
 #pragma unroll
-  for (int m = 0; m < ROWS; ++m)
+  for (int m = 0; m < ROWS; ++m) {
+    g[m] = g2[m].x + g2[m].y;
+    u[m] = u2[m].x + u2[m].y;
     for (int o = 16; o > 0; o >>= 1) {
       g[m] += __shfl_xor_sync(0xffffffffu, g[m], o);
       u[m] += __shfl_xor_sync(0xffffffffu, u[m], o);
     }
+  }
   if constexpr (WPO == 8) {
     __shared__ float sums[8][2][ROWS];
     if (lane == 0)
@@ -101,27 +144,31 @@ __global__ void __launch_bounds__(256) gated_rows_kernel(const GatedArgs A, floa
     }
   }
   if (n >= A.outer || (WPO == 8 && warp > 0)) return;
+  float gate = g[0], up = u[0];  // lane m finishes row m
 #pragma unroll
-  for (int m = 0; m < ROWS; ++m) {
-    if (lane == m && m < A.rows) {
-      const float gate = g[m] + (A.bg ? to_f(((const T*)A.bg)[n]) : 0.f);
-      const float up = u[m] + (A.bu ? to_f(((const T*)A.bu)[n]) : 0.f);
-      const float z[1] = {gate};
-      float value[1], slope[1];
-      gated_act<BACK>(A.act, z, value, slope);
-      if constexpr (BACK) {
-        const float dy = to_f(((const T*)A.dout)[m * A.dout_ld + n]);
-        dg[m * A.outer + n] = dy * up * slope[0];
-        du[m * A.outer + n] = dy * value[0];
-      } else {
-        ((T*)A.out)[m * A.out_ld + n] = from_f<T>(value[0] * up);
-      }
+  for (int m = 1; m < ROWS; ++m)
+    if (lane == m) {
+      gate = g[m];
+      up = u[m];
+    }
+  if (lane < ROWS && lane < A.rows) {
+    if (A.bg) gate += to_f(((const T*)A.bg)[n]);
+    if (A.bu) up += to_f(((const T*)A.bu)[n]);
+    const float z[1] = {gate};
+    float value[1], slope[1];
+    gated_act<BACK>(A.act, z, value, slope);
+    if constexpr (BACK) {
+      const float dy = to_f(((const T*)A.dout)[lane * A.dout_ld + n]);
+      dg[lane * A.outer + n] = dy * up * slope[0];
+      du[lane * A.outer + n] = dy * value[0];
+    } else {
+      ((T*)A.out)[lane * A.out_ld + n] = from_f<T>(value[0] * up);
     }
   }
 }
 
 // dx of few rows: a thread owns VEC columns of the weights and walks a range of their rows
-// (blockIdx.y); the ranges' sums are joined by mm_join_kernel.
+// (blockIdx.y); the ranges' sums are joined by gated_rows_join_kernel.
 template <typename T, int ROWS, int VEC>
 __global__ void __launch_bounds__(128) gated_rows_dx_kernel(const GatedArgs A, const float* dg,
                                                             const float* du, int64_t per,
@@ -195,19 +242,25 @@ __global__ void __launch_bounds__(128) gated_rows_dw_kernel(const GatedArgs A, c
 }
 
 // ------------------------------------------------------------- helpers
-// C = sum of the ranges' partial sums [range][halves][M][N], in range order.
+// dx of few rows: the sum of the ranges' partial sums [range][M][N], 32 elements per block, 32 threads
+// along the ranges of each.
 template <typename T>
-__global__ void __launch_bounds__(256) mm_join_kernel(const float* __restrict__ partial, int ranges,
-                                                      int64_t M, int64_t N, int halves, T* c0, T* c1,
-                                                      int64_t c_ld) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= halves * M * N) return;
+__global__ void __launch_bounds__(1024) gated_rows_join_kernel(const float* __restrict__ partial,
+                                                               int ranges, int64_t M, int64_t N, T* c,
+                                                               int64_t c_ld) {
+  __shared__ float sums[32][33];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int64_t e = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.f;
-  for (int r = 0; r < ranges; ++r) s += partial[r * halves * M * N + e];
-  const int half = e >= M * N;
-  T* c = half ? c1 : c0;
-  const int64_t f = e - half * M * N;
-  if (c) c[(f / N) * c_ld + f % N] = from_f<T>(s);
+  if (e < M * N)
+#pragma unroll 4
+    for (int r = part; r < ranges; r += 32) s += partial[r * M * N + e];
+  sums[part][lane] = s;
+  __syncthreads();
+  float v = sums[lane][part];  // warp: element, lane: ranges
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int64_t out = (int64_t)blockIdx.x * 32 + part;
+  if (lane == 0 && out < M * N) c[(out / N) * c_ld + out % N] = from_f<T>(v);
 }
 
 // Matrices to tensor-core operands, one per blockIdx.y: fp32 weights to three bf16 planes, or a matrix
@@ -293,36 +346,44 @@ __global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__
   }
 }
 
-// The backward pass's joins in one launch: blocks below `dw_blocks` add the ranges of dWg and dWu (in
-// range order), the others the column sums of dgate and dup (32 columns each, 32 threads along the
-// partial rows).
+// The backward pass's joins in one launch: the ranges of dWg and dWu, then those of dx (in range order),
+// then the column sums of dgate and dup (32 columns to a block, 32 threads along the partial rows).
+struct RangeSums {
+  const float* partial;  // [ranges][halves][M][N rounded up to 16]
+  int64_t ranges, M, N, ld;
+  int32_t halves;
+  void* out[2];
+  int64_t blocks;        // of 1024 elements
+};
 struct JoinArgs {
-  const float* dw_partial;
-  int64_t ranges, M, N, dw_ld;
-  void* dw[2];
+  RangeSums dw, dx;
   const float* col_sums;
-  int64_t sum_rows;
+  int64_t sum_rows, outer;
   void* db[2];
-  int64_t dw_blocks;
 };
 template <typename T>
-__global__ void __launch_bounds__(1024) gated_join_kernel(const __grid_constant__ JoinArgs A) {
-  if (blockIdx.x < A.dw_blocks) {
-    // The partial sums' rows are padded to a multiple of 16 columns.
-    const int64_t ld = (A.N + 15) / 16 * 16, one = A.M * ld;
-    const int64_t e = (int64_t)blockIdx.x * 1024 + threadIdx.x;
-    if (e >= 2 * one) return;
-    const int half = e >= one;
-    const int64_t f = e - half * one, row = f / ld, col = f - row * ld;
-    T* dst = (T*)A.dw[half];
-    if (!dst || col >= A.N) return;
-    float s = 0.f;
+__device__ __forceinline__ void range_join(const RangeSums& A, int64_t block) {
+  const int64_t ld = (A.N + 15) / 16 * 16, one = A.M * ld;
+  const int64_t e = block * 1024 + threadIdx.x;
+  if (e >= A.halves * one) return;
+  const int half = e >= one;
+  const int64_t f = e - half * one, row = f / ld, col = f - row * ld;
+  T* dst = (T*)A.out[half];
+  if (!dst || col >= A.N) return;
+  float s = 0.f;
 #pragma unroll 4
-    for (int64_t r = 0; r < A.ranges; ++r) s += A.dw_partial[r * 2 * one + e];
-    dst[row * A.dw_ld + col] = from_f<T>(s);
-    return;
-  }
-  column_join<T>(A.col_sums, A.sum_rows, A.M, (T*)A.db[0], (T*)A.db[1], blockIdx.x - A.dw_blocks);
+  for (int64_t r = 0; r < A.ranges; ++r) s += A.partial[r * A.halves * one + e];
+  dst[row * A.ld + col] = from_f<T>(s);
+}
+template <typename T>
+__global__ void __launch_bounds__(1024) gated_join_kernel(const __grid_constant__ JoinArgs A) {
+  if (blockIdx.x < A.dw.blocks)
+    range_join<T>(A.dw, blockIdx.x);
+  else if (blockIdx.x < A.dw.blocks + A.dx.blocks)
+    range_join<T>(A.dx, blockIdx.x - A.dw.blocks);
+  else
+    column_join<T>(A.col_sums, A.sum_rows, A.outer, (T*)A.db[0], (T*)A.db[1],
+                   blockIdx.x - A.dw.blocks - A.dx.blocks);
 }
 
 // ------------------------------------------------------------------ host
@@ -386,6 +447,8 @@ struct GatedPlan {
   int64_t partial = 0, total = 0;
   int tile_n = 0;                      // GG_DW column tile
   int splits = 1, kb_per = 1;          // GG_DW
+  int splits_x = 1, kb_per_x = 1;      // GG_DX
+  int64_t partial_x = 0;
   int64_t sums = 0;                    // column sums of dgate and dup
   int ranges_x = 1;                    // dx of few rows
 };
@@ -406,8 +469,22 @@ constexpr int64_t kTwoPlanes = (int64_t)1 << 31;
 
 // Column tile of a GG_DX / GG_DW product with n output columns.
 static int plain_tile(int64_t n, bool f32) { return n <= 64 ? 64 : n <= 128 || f32 ? 128 : 256; }
-// MMA width of GG_PROJ: gate and up columns of one tile.
-static int proj_tile(int64_t outer, bool f32) { return outer <= 32 ? 64 : outer <= 64 || f32 ? 128 : 256; }
+// MMA width of GG_PROJ: gate and up columns of one tile. The widest tile that its columns fill, or a
+// narrower one where that finds more SMs: a tile's time goes with the 128 + nb rows that a stage loads
+// (bf16, 16 rows, 2048 -> 8192: 64 tiles of 256 26 us, 128 tiles of 128 TILE_NOTE us).
+static int proj_tile(int64_t rows, int64_t outer, bool f32) {
+  int best = 64;
+  int64_t least = INT64_MAX;
+  for (int nb = outer <= 32 ? 64 : outer <= 64 || f32 ? 128 : 256; nb >= 64; nb /= 2) {
+    const int64_t tiles = ceil_div(rows, kGgBM) * ceil_div(outer, nb / 2);
+    const int64_t time = ceil_div(tiles, kFeatSMs) * (kGgBM + nb);
+    if (time < least) {
+      least = time;
+      best = nb;
+    }
+  }
+  return best;
+}
 
 static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t dtype, bool backward) {
   GatedPlan P;
@@ -446,6 +523,14 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
     P.kb_per = (int)ceil_div(kb, want);
     P.splits = (int)ceil_div(kb, P.kb_per);
     P.partial = take(at, P.splits > 1 ? P.splits * 2 * outer * round_up(inner, 16) * 4 : 0);
+    // dx: the reduction is 2 outer long; ranges of at least 8 stages while they find idle SMs (bf16,
+    // 16 rows, 2048 -> 8192: 8 tiles, 159 us in one range).
+    const int64_t kbx = 2 * ceil_div(outer, kGgBK);
+    const int64_t tiles_x = ceil_div(rows, kGgBM) * ceil_div(inner, P.tile_n);
+    const int64_t want_x = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles_x, kbx / 8));
+    P.kb_per_x = (int)ceil_div(kbx, want_x);
+    P.splits_x = (int)ceil_div(kbx, P.kb_per_x);
+    P.partial_x = take(at, P.splits_x > 1 ? P.splits_x * rows * round_up(inner, 16) * 4 : 0);
     P.sums = take(at, 4 * ceil_div(rows, kGgBM) * 2 * outer * 4);
   }
   P.total = at;
@@ -533,7 +618,7 @@ static int gated_operands(const GatedArgs& A, const GatedPlan& P, char* ws, Oper
 template <typename T, typename D, int PL, int PD, bool BACK>
 static int gated_project(const GatedArgs& A, const Operand& x, const Operand& wg, const Operand& wu,
                          GgArgs G, cudaStream_t st) {
-  const int nb = proj_tile(A.outer, PL == 3);
+  const int nb = proj_tile(A.rows, A.outer, PL == 3);
   const int bn = nb / 2;
   CUtensorMap mx, mg, mu;
   constexpr int BK = PL == 3 ? kGgSplitBK : kGgBK;
@@ -609,8 +694,8 @@ static int gated_rows_grads(const GatedArgs& A, const GatedGrads& G, const Gated
     gated_rows_dx_kernel<T, ROWS, VEC>
         <<<dim3((unsigned)cols, ranges), 128, 0, st>>>(A, dg, du, per, partial);
     GPB_CHECK_CUDA(cudaGetLastError());
-    mm_join_kernel<T><<<(unsigned)ceil_div(A.rows * A.inner, 256), 256, 0, st>>>(
-        partial, ranges, A.rows, A.inner, 1, (T*)G.dx, nullptr, G.dx_ld);
+    gated_rows_join_kernel<T><<<(unsigned)ceil_div(A.rows * A.inner, 32), 1024, 0, st>>>(
+        partial, ranges, A.rows, A.inner, (T*)G.dx, G.dx_ld);
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   if (G.dwg || G.dwu || G.dbg || G.dbu) {
@@ -688,8 +773,9 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
     G.tiles_n = (int32_t)ceil_div(A.inner, nb);
     G.kblocks = (int32_t)ceil_div(A.outer, kGgBK);
     G.segs = 2;
-    G.splits = 1;
-    G.kb_per = 2 * G.kblocks;
+    G.splits = P.splits_x;
+    G.kb_per = P.kb_per_x;
+    G.partial = (float*)(ws + P.partial_x);
     G.out[0] = R.dx;
     G.out_ld = R.dx_ld;
     G.vec = row_align(R.dx, R.dx_ld * sizeof(T));
@@ -721,24 +807,21 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
     GPB_TRY(make_map(du, 64, BK, &a1));
     GPB_TRY((gated_plain<GG_DW, T, D, PL, PD>(a0, a1, x, x, P.tile_n, G, st)));
   }
-  const bool bias = R.dbg || R.dbu, join_w = P.splits > 1 && (R.dwg || R.dwu);
-  if (bias || join_w) {
-    JoinArgs J{};
-    J.M = A.outer;
-    J.N = A.inner;
-    if (join_w) {
-      J.dw_partial = partial;
-      J.ranges = P.splits;
-      J.dw_ld = R.dw_ld;
-      J.dw[0] = R.dwg;
-      J.dw[1] = R.dwu;
-      J.dw_blocks = ceil_div(2 * A.outer * round_up(A.inner, 16), 1024);
-    }
-    J.col_sums = (const float*)(ws + P.sums);
-    J.sum_rows = 4 * ceil_div(A.rows, kGgBM);
-    J.db[0] = R.dbg;
-    J.db[1] = R.dbu;
-    const int64_t grid = J.dw_blocks + (bias ? ceil_div(2 * A.outer, 32) : 0);
+  const bool bias = R.dbg || R.dbu;
+  JoinArgs J{};
+  if (P.splits > 1 && (R.dwg || R.dwu))
+    J.dw = {partial, P.splits, A.outer, A.inner, R.dw_ld, 2, {R.dwg, R.dwu},
+            ceil_div(2 * A.outer * round_up(A.inner, 16), 1024)};
+  if (P.splits_x > 1 && R.dx)
+    J.dx = {(float*)(ws + P.partial_x), P.splits_x, A.rows, A.inner, R.dx_ld, 1, {R.dx, nullptr},
+            ceil_div(A.rows * round_up(A.inner, 16), 1024)};
+  J.col_sums = (const float*)(ws + P.sums);
+  J.sum_rows = 4 * ceil_div(A.rows, kGgBM);
+  J.outer = A.outer;
+  J.db[0] = R.dbg;
+  J.db[1] = R.dbu;
+  const int64_t grid = J.dw.blocks + J.dx.blocks + (bias ? ceil_div(2 * A.outer, 32) : 0);
+  if (grid > 0) {
     gated_join_kernel<T><<<(unsigned)grid, 1024, 0, st>>>(J);
     GPB_CHECK_CUDA(cudaGetLastError());
   }

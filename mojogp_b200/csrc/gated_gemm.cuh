@@ -5,8 +5,9 @@
 //            of the same outputs share the x tile and one MMA, and the epilogue applies the
 //            activation and the product (or, for the backward pass, forms dgate and dup);
 //   GG_DX    dx = dgate Wg + dup Wu      one accumulation over two segments;
-//   GG_DW    dWg = dgate' x, dWu = dup' x   the reduction runs over rows, which are split over CTAs
-//            when the weight has few tiles (fp32 partial sums, joined in split order).
+//   GG_DW    dWg = dgate' x, dWu = dup' x   the reduction runs over rows.
+// GG_DX and GG_DW with too few tiles for the SMs split the reduction over CTAs (fp32 partial sums, joined
+// in split order).
 // x and the weights are read where they lie. A product whose reduction index is not the contiguous
 // one takes its operand MN-major: the tensor core transposes, nothing is copied.
 //
@@ -139,14 +140,14 @@ struct GgArgs {
   int32_t half_tiles;  // GG_DW: row tiles of one weight; 0 = both weights' rows share a tile
   int32_t kblocks;     // stages of one segment
   int32_t segs;        // segments of the reduction
-  int32_t splits;      // GG_DW: ranges of the reduction
+  int32_t splits;      // GG_DX, GG_DW: ranges of the reduction
   int32_t kb_per;      // stages per range
   uint32_t idesc;
   // epilogue
   void* out[2];        // GG_PROJ: out, or the dgate / dup planes; GG_DX: dx; GG_DW: dWg, dWu
   int64_t out_ld;
   int64_t plane;       // elements between planes of dgate / dup
-  float* partial;      // GG_DW with splits > 1: [split][2][M][N]
+  float* partial;      // with splits > 1: [split][2 (GG_DW), 1 (GG_DX)][M][N rounded up to 16]
   const void* bg;
   const void* bu;
   const void* dout;
@@ -532,11 +533,12 @@ __device__ __forceinline__ void gg_plain_store(const GgArgs& A, int split, int m
     m = (int64_t)mt * kGgBM + lane_row;
   }
   const int64_t left = A.N - n;
-  if (MODE == GG_DW && A.splits > 1) {
+  if (A.splits > 1) {
+    constexpr int HALVES = MODE == GG_DW ? 2 : 1;
     // Rows padded to a multiple of 16: whole sectors, columns past N unread.
     const int64_t ld = (A.N + 15) / 16 * 16;
     if (m < A.M && left > 0) {
-      float* dst = A.partial + (((int64_t)split * 2 + half) * A.M + m) * ld + n;
+      float* dst = A.partial + (((int64_t)split * HALVES + half) * A.M + m) * ld + n;
 #pragma unroll
       for (int q = 0; q < 16; q += 8)
         store32(dst + q,
