@@ -467,6 +467,10 @@ static int64_t take(int64_t& at, int64_t bytes) {
 // cost half the call's time or more, and the outputs' sums are long enough to average the rounding.
 constexpr int64_t kTwoPlanes = (int64_t)1 << 31;
 
+// Rows of an A tile that a single row tile loads: whole groups of 8 (the swizzle's unit).
+static int tile_rows(int64_t rows) {
+  return rows < kGgBM ? (int)round_up(rows, 8) : kGgBM;
+}
 // Column tile of a GG_DX / GG_DW product with n output columns.
 static int plain_tile(int64_t n, bool f32) { return n <= 64 ? 64 : n <= 128 || f32 ? 128 : 256; }
 // MMA width of GG_PROJ: gate and up columns of one tile. The widest tile that its columns fill, or a
@@ -624,7 +628,8 @@ static int gated_project(const GatedArgs& A, const Operand& x, const Operand& wg
   constexpr int BK = PL == 3 ? kGgSplitBK : kGgBK;
   GPB_TRY(make_map(wg, BK, bn, &mg));
   GPB_TRY(make_map(wu, BK, bn, &mu));
-  GPB_TRY(make_map(x, BK, kGgBM, &mx));
+  G.a_rows = tile_rows(A.rows);
+  GPB_TRY(make_map(x, BK, G.a_rows, &mx));
   G.M = A.rows;
   G.N = A.outer;
   G.tiles_m = (int32_t)ceil_div(A.rows, kGgBM);
@@ -780,8 +785,9 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
     G.out_ld = R.dx_ld;
     G.vec = row_align(R.dx, R.dx_ld * sizeof(T));
     CUtensorMap a0, a1;
-    GPB_TRY(make_map(dg, kGgBK, kGgBM, &a0));
-    GPB_TRY(make_map(du, kGgBK, kGgBM, &a1));
+    G.a_rows = tile_rows(A.rows);
+    GPB_TRY(make_map(dg, kGgBK, G.a_rows, &a0));
+    GPB_TRY(make_map(du, kGgBK, G.a_rows, &a1));
     GPB_TRY((gated_plain<GG_DX, T, D, PL, PD>(a0, a1, wg, wu, nb, G, st)));
   }
   if (R.dwg || R.dwu) {

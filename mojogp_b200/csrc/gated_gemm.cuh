@@ -142,6 +142,7 @@ struct GgArgs {
   int32_t segs;        // segments of the reduction
   int32_t splits;      // GG_DX, GG_DW: ranges of the reduction
   int32_t kb_per;      // stages per range
+  int32_t a_rows;      // GG_PROJ, GG_DX: rows of an A tile that are loaded (the rest feeds unused rows)
   uint32_t idesc;
   // epilogue
   void* out[2];        // GG_PROJ: out, or the dgate / dup planes; GG_DX: dx; GG_DW: dWg, dWu
@@ -656,7 +657,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
             const int q = it % kGgRaw;
             if (it >= kGgRaw) ok = mbar_wait_bounded(&raw_empty[q], ((it / kGgRaw) & 1) ^ 1);
             if (!ok) break;
-            mbar_arrive_expect_tx(&raw_full[q], S::kRaw);
+            mbar_arrive_expect_tx(&raw_full[q], MODE == GG_PROJ ? A.a_rows * (BK * 4) : S::kRaw);
             const uint32_t dst = raw + q * S::kRaw;
             if constexpr (MODE == GG_PROJ) {
               gg_tma(dst, &a0, k0, I.mt * kGgBM, 0, &raw_full[q]);
@@ -674,7 +675,12 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
           // Both CTAs' bytes are expected by the even one (the odd one's may come first).
           uint32_t pair_bar = 0;
           if constexpr (PAIR) pair_bar = gg_leader_addr(&full[s]);
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * S::kTmaBytes);
+          if (rank == 0) {
+            int bytes = CTAS * S::kTmaBytes;
+            if constexpr (CTAS == 1 && S::kTmaA && MODE != GG_DW)
+              bytes -= PA * (kGgBM - A.a_rows) * (2 * BK);
+            mbar_arrive_expect_tx(&full[s], bytes);
+          }
           auto tma = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
             if constexpr (PAIR)
               gg_tma_pair(dst, map, c0, c1, c2, pair_bar);
