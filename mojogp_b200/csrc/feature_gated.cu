@@ -5,8 +5,9 @@
 //   dgate = dout up act'(gate),  dup = dout act(gate)
 //   dx = dgate Wg + dup Wu,  dWg = dgate' x,  dWu = dup' x,  dbg, dbu = column sums
 //
-// Up to kFewRows rows read every weight once for a handful of multiply-adds: HBM bound, on the CUDA
-// cores in fp32 (gated_rows_*). More rows run on the tensor cores (gated_gemm.cuh).
+// A few rows (few_rows) read every weight once for a handful of multiply-adds: HBM bound, on the CUDA
+// cores in fp32 (gated_rows_*; 1 row, 2048 -> 8192 bf16, 67 MB: 16 us). More rows run on the tensor cores
+// (gated_gemm.cuh), up to some 200 of them for the time of the weights' reading.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -346,6 +347,64 @@ __global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__
   }
 }
 
+// Joins a projection's ranges and runs its epilogue: 32 rows x 32 columns to a block, a warp to a row.
+template <typename T, typename D, int PD, bool BACK>
+__global__ void __launch_bounds__(256) gated_finish_kernel(const __grid_constant__ GgArgs A) {
+  __shared__ float sums[8][2][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n = (int64_t)blockIdx.x * 32 + lane, ld = (A.N + 15) / 16 * 16;
+  const bool in = n < A.N;
+  const float bg = in && A.bg ? to_f(((const T*)A.bg)[n]) : 0.f;
+  const float bu = in && A.bu ? to_f(((const T*)A.bu)[n]) : 0.f;
+  float sg = 0.f, su = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = (int64_t)blockIdx.y * 32 + i * 8 + warp;
+    if (m >= A.M || !in) continue;
+    const float* src = A.partial + m * ld + n;
+    float gate = 0.f, up = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < A.splits; ++s) {
+      gate += src[(2 * s) * A.M * ld];
+      up += src[(2 * s + 1) * A.M * ld];
+    }
+    up += bu;
+    const float z[1] = {gate + bg};
+    float value[1], slope[1];
+    gated_act<BACK>(A.act, z, value, slope);
+    if constexpr (BACK) {
+      const float dy = to_f(((const T*)A.dout)[m * A.dout_ld + n]);
+      const float d[2] = {dy * up * slope[0], dy * value[0]};
+      sg += d[0];
+      su += d[1];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float rest = d[h];
+#pragma unroll
+        for (int p = 0; p < PD; ++p) {
+          const D part = from_f<D>(rest);
+          ((D*)A.out[h])[p * A.plane + m * A.out_ld + n] = part;
+          rest -= to_f(part);
+        }
+      }
+    } else {
+      ((T*)A.out[0])[m * A.out_ld + n] = from_f<T>(value[0] * up);
+    }
+  }
+  if constexpr (BACK) {
+    if (!A.col_sums) return;
+    sums[warp][0][lane] = sg;
+    sums[warp][1][lane] = su;
+    __syncthreads();
+    if (warp < 2 && in) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s += sums[w][warp][lane];
+      A.col_sums[((int64_t)blockIdx.y * 2 + warp) * A.N + n] = s;
+    }
+  }
+}
+
 // The backward pass's joins in one launch: the ranges of dWg and dWu, then those of dx (in range order),
 // then the column sums of dgate and dup (32 columns to a block, 32 threads along the partial rows).
 struct RangeSums {
@@ -447,6 +506,8 @@ struct GatedPlan {
   int64_t partial = 0, total = 0;
   int tile_n = 0;                      // GG_DW column tile
   int splits = 1, kb_per = 1;          // GG_DW
+  int splits_p = 1, kb_per_p = 1;      // GG_PROJ
+  int64_t partial_p = 0;
   int splits_x = 1, kb_per_x = 1;      // GG_DX
   int64_t partial_x = 0;
   int64_t sums = 0;                    // column sums of dgate and dup
@@ -475,7 +536,7 @@ static int tile_rows(int64_t rows) {
 static int plain_tile(int64_t n, bool f32) { return n <= 64 ? 64 : n <= 128 || f32 ? 128 : 256; }
 // MMA width of GG_PROJ: gate and up columns of one tile. The widest tile that its columns fill, or a
 // narrower one where that finds more SMs: a tile's time goes with the 128 + nb rows that a stage loads
-// (bf16, 16 rows, 2048 -> 8192: 64 tiles of 256 26 us, 128 tiles of 128 TILE_NOTE us).
+// (bf16, 16 rows, 2048 -> 8192: 64 tiles of 256 26 us, 128 tiles of 128 20 us).
 static int proj_tile(int64_t rows, int64_t outer, bool f32) {
   int best = 64;
   int64_t least = INT64_MAX;
@@ -490,11 +551,27 @@ static int proj_tile(int64_t rows, int64_t outer, bool f32) {
   return best;
 }
 
+// Rows up to which a call runs on the CUDA cores. Weights of a quarter million elements on: 16-bit, 2
+// (2048 -> 8192 bf16 forward at 4 rows 39 us against 23.5 on the tensor cores, backward 105 against 75; at
+// 2 rows 26.6 against 23.4, 72.6 against 74.5); fp32, whose tensor-core path packs the weights into
+// planes first, all of kFewRows (57 us against 114, 181 against 212), but 4 where rows cannot be read as
+// vectors (2047 -> 8191 at 8 rows 225 against 118, 427 against 247; at 4 rows 84 against 118). Smaller
+// weights: launches decide, and this path has the fewer (501 -> 333 bf16 at 8 rows 11 us against 15,
+// backward 28 against 48).
+static int few_rows(int64_t inner, int64_t outer, bool f32) {
+  if (inner * outer < (1 << 18)) return kFewRows;
+  return !f32 ? 2 : inner % 4 ? 4 : kFewRows;
+}
+
+// Depth of a projection's range when few tiles split their reduction (a range costs its partial sums
+// and the call another launch): 8192 -> 1024 bf16 at 16 rows 44 us in one range, 23.5 in four.
+constexpr int kProjDepth = 1024;
+
 static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t dtype, bool backward) {
   GatedPlan P;
   const bool f32 = dtype == GPB_DTYPE_F32;
   int64_t at = 0;
-  if (rows <= kFewRows) {
+  if (rows <= few_rows(inner, outer, f32)) {
     P.few = true;
     if (!backward) return P;
     P.dg = take(at, rows * outer * 4);
@@ -513,6 +590,14 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
   P.x = take(at, rows * P.ldk * dtype_bytes(dtype));
   P.wg = take(at, P.planes * outer * P.ldk * 2);
   P.wu = take(at, P.planes * outer * P.ldk * 2);
+  {
+    const int64_t kb = ceil_div(inner, f32 ? kGgSplitBK : kGgBK);
+    const int64_t tiles = ceil_div(rows, kGgBM) * ceil_div(outer, proj_tile(rows, outer, f32) / 2);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles, inner / kProjDepth));
+    P.kb_per_p = (int)ceil_div(kb, want);
+    P.splits_p = (int)ceil_div(kb, P.kb_per_p);
+    P.partial_p = take(at, P.splits_p > 1 ? P.splits_p * 2 * rows * round_up(outer, 16) * 4 : 0);
+  }
   if (backward) {
     P.planes_d = f32 ? 3 : rows * inner * outer <= kTwoPlanes ? 2 : 1;
     P.plane_d = rows * P.ldn;
@@ -620,8 +705,8 @@ static int gated_operands(const GatedArgs& A, const GatedPlan& P, char* ws, Oper
 }
 
 template <typename T, typename D, int PL, int PD, bool BACK>
-static int gated_project(const GatedArgs& A, const Operand& x, const Operand& wg, const Operand& wu,
-                         GgArgs G, cudaStream_t st) {
+static int gated_project(const GatedArgs& A, const GatedPlan& P, char* ws, const Operand& x,
+                         const Operand& wg, const Operand& wu, GgArgs G, cudaStream_t st) {
   const int nb = proj_tile(A.rows, A.outer, PL == 3);
   const int bn = nb / 2;
   CUtensorMap mx, mg, mu;
@@ -635,21 +720,32 @@ static int gated_project(const GatedArgs& A, const Operand& x, const Operand& wg
   G.tiles_m = (int32_t)ceil_div(A.rows, kGgBM);
   G.tiles_n = (int32_t)ceil_div(A.outer, bn);
   G.kblocks = (int32_t)ceil_div(A.inner, BK);
-  G.segs = G.splits = 1;
-  G.kb_per = G.kblocks;
+  G.segs = 1;
+  G.splits = P.splits_p;
+  G.kb_per = P.kb_per_p;
+  G.partial = (float*)(ws + P.partial_p);
   G.bg = A.bg;
   G.bu = A.bu;
   G.act = A.act;
   G.dout = A.dout;
   G.dout_ld = A.dout_ld;
-  switch (nb) {
-    case 64: return gg_launch<GG_PROJ, 64, PL, PL, T, D, PD, BACK>(mx, mx, mg, mu, G, st);
-    case 128: return gg_launch<GG_PROJ, 128, PL, PL, T, D, PD, BACK>(mx, mx, mg, mu, G, st);
-    default:
-      if constexpr (PL == 1)
-        return gg_launch<GG_PROJ, 256, PL, PL, T, D, PD, BACK>(mx, mx, mg, mu, G, st);
-      return GPB_ERR_UNSUPPORTED;
+  auto run = [&]() {
+    switch (nb) {
+      case 64: return gg_launch<GG_PROJ, 64, PL, PL, T, D, PD, BACK>(mx, mx, mg, mu, G, st);
+      case 128: return gg_launch<GG_PROJ, 128, PL, PL, T, D, PD, BACK>(mx, mx, mg, mu, G, st);
+      default:
+        if constexpr (PL == 1)
+          return gg_launch<GG_PROJ, 256, PL, PL, T, D, PD, BACK>(mx, mx, mg, mu, G, st);
+        return (int)GPB_ERR_UNSUPPORTED;
+    }
+  };
+  GPB_TRY(run());
+  if (G.splits > 1) {
+    const dim3 grid((unsigned)ceil_div(A.outer, 32), (unsigned)(4 * ceil_div(A.rows, kGgBM)));
+    gated_finish_kernel<T, D, PD, BACK><<<grid, 256, 0, st>>>(G);
+    GPB_CHECK_CUDA(cudaGetLastError());
   }
+  return GPB_OK;
 }
 
 template <int MODE, typename T, typename D, int PL, int PD>
@@ -742,7 +838,7 @@ static int gated_forward(const GatedArgs& A, char* ws, const GatedPlan& P, cudaS
   G.out[0] = A.out;
   G.out_ld = A.out_ld;
   G.vec = row_align(A.out, A.out_ld * sizeof(T));
-  return gated_project<T, D, PL, PL, false>(A, x, wg, wu, G, st);
+  return gated_project<T, D, PL, PL, false>(A, P, ws, x, wg, wu, G, st);
 }
 
 template <typename T, typename D, int PL, int PD>
@@ -767,7 +863,7 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
     G.plane = P.plane_d;
     G.vec = row_align(A.dout, A.dout_ld * sizeof(T));
     if (R.dbg || R.dbu) G.col_sums = (float*)(ws + P.sums);
-    GPB_TRY((gated_project<T, D, PL, PD, true>(A, x, wg, wu, G, st)));
+    GPB_TRY((gated_project<T, D, PL, PD, true>(A, P, ws, x, wg, wu, G, st)));
   }
   if (R.dx) {
     GgArgs G{};

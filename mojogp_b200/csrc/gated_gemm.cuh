@@ -6,8 +6,8 @@
 //            activation and the product (or, for the backward pass, forms dgate and dup);
 //   GG_DX    dx = dgate Wg + dup Wu      one accumulation over two segments;
 //   GG_DW    dWg = dgate' x, dWu = dup' x   the reduction runs over rows.
-// GG_DX and GG_DW with too few tiles for the SMs split the reduction over CTAs (fp32 partial sums, joined
-// in split order).
+// A product with too few tiles for the SMs splits its reduction over CTAs (fp32 partial sums, joined in
+// split order; GG_PROJ's epilogue then runs in the join).
 // x and the weights are read where they lie. A product whose reduction index is not the contiguous
 // one takes its operand MN-major: the tensor core transposes, nothing is copied.
 //
@@ -140,7 +140,7 @@ struct GgArgs {
   int32_t half_tiles;  // GG_DW: row tiles of one weight; 0 = both weights' rows share a tile
   int32_t kblocks;     // stages of one segment
   int32_t segs;        // segments of the reduction
-  int32_t splits;      // GG_DX, GG_DW: ranges of the reduction
+  int32_t splits;      // ranges of the reduction
   int32_t kb_per;      // stages per range
   int32_t a_rows;      // GG_PROJ, GG_DX: rows of an A tile that are loaded (the rest feeds unused rows)
   uint32_t idesc;
@@ -148,7 +148,7 @@ struct GgArgs {
   void* out[2];        // GG_PROJ: out, or the dgate / dup planes; GG_DX: dx; GG_DW: dWg, dWu
   int64_t out_ld;
   int64_t plane;       // elements between planes of dgate / dup
-  float* partial;      // with splits > 1: [split][2 (GG_DW), 1 (GG_DX)][M][N rounded up to 16]
+  float* partial;      // with splits > 1: [split][2, GG_DX 1][M][N rounded up to 16]
   const void* bg;
   const void* bu;
   const void* dout;
@@ -426,6 +426,7 @@ struct GgRow {
   __device__ __forceinline__ void load(const GgArgs& A, int64_t m, int64_t n, float* tile, int lane) {
     const T* src = (const T*)A.dout + m * A.dout_ld + n;
     const int64_t left = A.N - n;
+    if (A.splits > 1) return;  // the join reads dout
     if (A.vec && left >= 16) {
 #pragma unroll
       for (int q = 0; q < kVecs; ++q)
@@ -453,14 +454,33 @@ struct GgRow {
   }
 };
 
+// 16 fp32 partial sums of a row: whole sectors (rows are padded to a multiple of 16 columns).
+__device__ __forceinline__ void gg_store_partial(float* dst, const float (&v)[16]) {
+#pragma unroll
+  for (int q = 0; q < 16; q += 8)
+    store32(dst + q,
+            make_uint4(__float_as_uint(v[q]), __float_as_uint(v[q + 1]), __float_as_uint(v[q + 2]),
+                       __float_as_uint(v[q + 3])),
+            make_uint4(__float_as_uint(v[q + 4]), __float_as_uint(v[q + 5]),
+                       __float_as_uint(v[q + 6]), __float_as_uint(v[q + 7])));
+}
+
 // Epilogue of 16 columns of one output row; `bias` holds the columns' gate biases, then `step` floats
 // on their up biases. BACK: PD planes of dgate and dup, 16-bit type D, and their column sums.
 template <typename T, typename D, int PD, bool BACK>
-__device__ __forceinline__ void gg_proj_store(const GgArgs& A, int64_t m, int64_t n,
+__device__ __forceinline__ void gg_proj_store(const GgArgs& A, int split, int64_t m, int64_t n,
                                               const float* bias, int step, const GgRow<T>& dy,
                                               float* col_sums, float* tile, int lane, float (&g)[16],
                                               float (&u)[16]) {
   const int64_t left = A.N - n;
+  if (A.splits > 1) {
+    const int64_t ld = (A.N + 15) / 16 * 16;
+    if (m < A.M && left > 0) {
+      gg_store_partial(A.partial + ((int64_t)split * 2 * A.M + m) * ld + n, g);
+      gg_store_partial(A.partial + (((int64_t)split * 2 + 1) * A.M + m) * ld + n, u);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 16; i += 4) {
     const float4 b = *reinterpret_cast<const float4*>(bias + i);
@@ -536,18 +556,9 @@ __device__ __forceinline__ void gg_plain_store(const GgArgs& A, int split, int m
   const int64_t left = A.N - n;
   if (A.splits > 1) {
     constexpr int HALVES = MODE == GG_DW ? 2 : 1;
-    // Rows padded to a multiple of 16: whole sectors, columns past N unread.
     const int64_t ld = (A.N + 15) / 16 * 16;
-    if (m < A.M && left > 0) {
-      float* dst = A.partial + (((int64_t)split * HALVES + half) * A.M + m) * ld + n;
-#pragma unroll
-      for (int q = 0; q < 16; q += 8)
-        store32(dst + q,
-                make_uint4(__float_as_uint(v[q]), __float_as_uint(v[q + 1]),
-                           __float_as_uint(v[q + 2]), __float_as_uint(v[q + 3])),
-                make_uint4(__float_as_uint(v[q + 4]), __float_as_uint(v[q + 5]),
-                           __float_as_uint(v[q + 6]), __float_as_uint(v[q + 7])));
-    }
+    if (m < A.M && left > 0)
+      gg_store_partial(A.partial + (((int64_t)split * HALVES + half) * A.M + m) * ld + n, v);
   } else if (A.out[half]) {
     gg_store<T>((T*)A.out[half], A.out_ld, m, A.M, n, v, left, A.vec, tile, lane);
   }
@@ -880,7 +891,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
                 g[i] = __uint_as_float(rg[i]);
                 u[i] = __uint_as_float(ru[i]);
               }
-              gg_proj_store<T, D, PD, BACK>(A, m, n + c, bias + c, HC, dy, col_sums, tile, lane, g, u);
+              gg_proj_store<T, D, PD, BACK>(A, I.split, m, n + c, bias + c, HC, dy, col_sums, tile, lane, g, u);
             } else {
               float v[16];
               tmem_ld16(t + c, v);
@@ -936,7 +947,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
                 dy = dy_next;
                 if (c + 16 < HC) dy_next.load(A, m, n + c + 16, tile, lane);
               }
-              gg_proj_store<T, D, PD, BACK>(A, m, n + c, bias + c, HC, dy, col_sums, tile, lane, v[0],
+              gg_proj_store<T, D, PD, BACK>(A, I.split, m, n + c, bias + c, HC, dy, col_sums, tile, lane, v[0],
                                             v[R - 1]);
             } else {
               gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v[0], tile, lane);

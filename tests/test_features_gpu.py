@@ -272,6 +272,33 @@ def test_gated_unit_large(ft, rows, inner, outer, dtype):
     gated_case(ft, rows, inner, outer, dtype, "gelu", True)
 
 
+# Few tiles: a long reduction is split (projections from 2048 columns, dx from 512 outputs) and the ranges
+# end unevenly; a few rows on either side of the CUDA-core path's bound, rows that a 16-byte vector cannot
+# read among them.
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,inner,outer", [
+    (2, 520, 520), (3, 520, 520), (3, 517, 523), (5, 517, 523), (8, 520, 520), (9, 520, 520),
+    (3, 2100, 130), (11, 2048, 7), (16, 4104, 72), (40, 5000, 33), (100, 2050, 40), (130, 3100, 200),
+    (290, 2048, 64), (20, 40, 1030), (129, 8, 2100), (260, 264, 800)])
+def test_gated_unit_few_tiles(ft, rows, inner, outer, dtype):
+    act = ["silu", "gelu", "sigmoid", "tanh"][(rows + inner + outer) % 4]
+    gated_case(ft, rows, inner, outer, dtype, act, bias=(rows + outer) % 3 > 0)
+
+
+def test_gated_unit_split_repeats(ft):
+    """Split reductions join in a fixed order: results repeat bit for bit."""
+    full = gated_case(ft, 50, 4096, 96, "bf16", "silu", True)
+    again = gated_case(ft, 50, 4096, 96, "bf16", "silu", True)
+    for a, b in zip(full, again):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [3, 140])
+@pytest.mark.parametrize("pad,offset", [(8, 0), (3, 0), (0, 1), (5, 3)])
+def test_gated_unit_split_strides(ft, rows, pad, offset):
+    gated_case(ft, rows, 2304, 144, "bf16", "gelu", True, transform=lambda v: strided(v, pad, offset))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid", "tanh"])
 @pytest.mark.parametrize("rows", [5, 150])
