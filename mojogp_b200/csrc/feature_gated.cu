@@ -275,7 +275,8 @@ struct PackArgs {
   int64_t cols, ld;
   int32_t lanes_log2;
 };
-// Threads: 2^lanes_log2 along a row, the others along rows, kPackRows of them each. 16-bit rows are read
+// Threads: 2^lanes_log2 along a row, the others along rows, kPackRows of them each; blockIdx.z: column steps
+// of few rows (195 x 6669 fp32 in 2 blocks: 140 us). 16-bit rows are read
 // as the 4-byte words they touch (5 for 8 elements), in reach of neighbours through L1, and shifted.
 constexpr int kPackRows = 4;
 template <typename T, typename D>
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__
   const int64_t row_step = 256 >> A.lanes_log2;
   const int64_t row0 = blockIdx.x * row_step * kPackRows + (threadIdx.x >> A.lanes_log2);
   if (row0 >= A.rows[o]) return;
-  for (int64_t c = tx * 8; c < A.ld; c += lanes * 8) {
+  for (int64_t c = (blockIdx.z * lanes + tx) * 8; c < A.ld; c += (int64_t)gridDim.z * lanes * 8) {
     uint32_t w[kPackRows][sizeof(T) == 4 ? 8 : 5];
 #pragma unroll
     for (int u = 0; u < kPackRows; ++u) {
@@ -349,18 +350,16 @@ __global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__
 
 // Joins a projection's ranges and runs its epilogue: 32 rows x 32 columns to a block, a warp to a row.
 template <typename T, typename D, int PD, bool BACK>
-__global__ void __launch_bounds__(256) gated_finish_kernel(const __grid_constant__ GgArgs A) {
-  __shared__ float sums[8][2][32];
+__global__ void __launch_bounds__(1024) gated_finish_kernel(const __grid_constant__ GgArgs A) {
+  __shared__ float sums[32][2][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t n = (int64_t)blockIdx.x * 32 + lane, ld = (A.N + 15) / 16 * 16;
   const bool in = n < A.N;
   const float bg = in && A.bg ? to_f(((const T*)A.bg)[n]) : 0.f;
   const float bu = in && A.bu ? to_f(((const T*)A.bu)[n]) : 0.f;
   float sg = 0.f, su = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = (int64_t)blockIdx.y * 32 + i * 8 + warp;
-    if (m >= A.M || !in) continue;
+  const int64_t m = (int64_t)blockIdx.y * 32 + warp;
+  if (m < A.M && in) {
     const float* src = A.partial + m * ld + n;
     float gate = 0.f, up = 0.f;
 #pragma unroll 4
@@ -375,8 +374,8 @@ __global__ void __launch_bounds__(256) gated_finish_kernel(const __grid_constant
     if constexpr (BACK) {
       const float dy = to_f(((const T*)A.dout)[m * A.dout_ld + n]);
       const float d[2] = {dy * up * slope[0], dy * value[0]};
-      sg += d[0];
-      su += d[1];
+      sg = d[0];
+      su = d[1];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float rest = d[h];
@@ -396,11 +395,13 @@ __global__ void __launch_bounds__(256) gated_finish_kernel(const __grid_constant
     sums[warp][0][lane] = sg;
     sums[warp][1][lane] = su;
     __syncthreads();
-    if (warp < 2 && in) {
-      float s = 0.f;
+    // Warp w adds column w's rows, one per lane.
+    const int64_t c = (int64_t)blockIdx.x * 32 + warp;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) s += sums[w][warp][lane];
-      A.col_sums[((int64_t)blockIdx.y * 2 + warp) * A.N + n] = s;
+    for (int h = 0; h < 2; ++h) {
+      float s = sums[lane][h][warp];
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0 && c < A.N) A.col_sums[((int64_t)blockIdx.y * 2 + h) * A.N + c] = s;
     }
   }
 }
@@ -563,10 +564,6 @@ static int few_rows(int64_t inner, int64_t outer, bool f32) {
   return !f32 ? 2 : inner % 4 ? 4 : kFewRows;
 }
 
-// Depth of a projection's range when few tiles split their reduction (a range costs its partial sums
-// and the call another launch): 8192 -> 1024 bf16 at 16 rows 44 us in one range, 23.5 in four.
-constexpr int kProjDepth = 1024;
-
 static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t dtype, bool backward) {
   GatedPlan P;
   const bool f32 = dtype == GPB_DTYPE_F32;
@@ -591,9 +588,11 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
   P.wg = take(at, P.planes * outer * P.ldk * 2);
   P.wu = take(at, P.planes * outer * P.ldk * 2);
   {
+    // Few tiles split a projection's reduction, into ranges that outlast the further launch: 1024 deep,
+    // 256 for fp32 (8192 -> 1024 bf16 at 16 rows: 44 us in one range, 23.5 in four).
     const int64_t kb = ceil_div(inner, f32 ? kGgSplitBK : kGgBK);
     const int64_t tiles = ceil_div(rows, kGgBM) * ceil_div(outer, proj_tile(rows, outer, f32) / 2);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles, inner / kProjDepth));
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles, inner / (f32 ? 256 : 1024)));
     P.kb_per_p = (int)ceil_div(kb, want);
     P.splits_p = (int)ceil_div(kb, P.kb_per_p);
     P.partial_p = take(at, P.splits_p > 1 ? P.splits_p * 2 * rows * round_up(outer, 16) * 4 : 0);
@@ -607,16 +606,17 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
     const int64_t tiles = (outer <= 64 ? 1 : 2 * ceil_div(outer, kGgBM)) * ceil_div(inner, P.tile_n);
     const int bk = f32 ? kGgSplitBK : kGgBK;
     const int64_t kb = ceil_div(rows, bk);
-    // At least 512 rows per range; as many ranges as fill the SMs twice.
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * kFeatSMs / tiles, kb * bk / 512));
+    // At least 8 stages per range; as many ranges as fill the SMs twice.
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * kFeatSMs / tiles, kb / 8));
     P.kb_per = (int)ceil_div(kb, want);
     P.splits = (int)ceil_div(kb, P.kb_per);
     P.partial = take(at, P.splits > 1 ? P.splits * 2 * outer * round_up(inner, 16) * 4 : 0);
-    // dx: the reduction is 2 outer long; ranges of at least 8 stages while they find idle SMs (bf16,
+    // dx: the reduction is 2 outer long; ranges of at least 8 stages (4 of fp32's longer ones)
+    // while they find idle SMs (bf16,
     // 16 rows, 2048 -> 8192: 8 tiles, 159 us in one range).
     const int64_t kbx = 2 * ceil_div(outer, kGgBK);
     const int64_t tiles_x = ceil_div(rows, kGgBM) * ceil_div(inner, P.tile_n);
-    const int64_t want_x = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles_x, kbx / 8));
+    const int64_t want_x = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles_x, kbx / (f32 ? 4 : 8)));
     P.kb_per_x = (int)ceil_div(kbx, want_x);
     P.splits_x = (int)ceil_div(kbx, P.kb_per_x);
     P.partial_x = take(at, P.splits_x > 1 ? P.splits_x * rows * round_up(inner, 16) * 4 : 0);
@@ -697,8 +697,10 @@ static int gated_operands(const GatedArgs& A, const GatedPlan& P, char* ws, Oper
       if (round_up(per, (int64_t)1 << l) <= round_up(per, (int64_t)1 << K.lanes_log2))
         K.lanes_log2 = l;
     const int64_t per_block = (256 >> K.lanes_log2) * kPackRows;
-    gated_pack_kernel<T, D>
-        <<<dim3((unsigned)ceil_div(most, per_block), count), 256, 0, st>>>(K);
+    const int64_t blocks = ceil_div(most, per_block);
+    const int64_t steps = ceil_div(per, (int64_t)1 << K.lanes_log2);
+    const int64_t split = std::min(steps, ceil_div(8 * kFeatSMs, blocks));
+    gated_pack_kernel<T, D><<<dim3((unsigned)blocks, count, (unsigned)split), 256, 0, st>>>(K);
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   return GPB_OK;
@@ -742,7 +744,7 @@ static int gated_project(const GatedArgs& A, const GatedPlan& P, char* ws, const
   GPB_TRY(run());
   if (G.splits > 1) {
     const dim3 grid((unsigned)ceil_div(A.outer, 32), (unsigned)(4 * ceil_div(A.rows, kGgBM)));
-    gated_finish_kernel<T, D, PD, BACK><<<grid, 256, 0, st>>>(G);
+    gated_finish_kernel<T, D, PD, BACK><<<grid, 1024, 0, st>>>(G);
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   return GPB_OK;
