@@ -484,8 +484,9 @@ int gpb_layer_norm_backward(int32_t device, void* stream, int32_t dtype, int32_t
  * [outer][inner] with one leading dimension, biases [outer] or NULL, out
  * [rows][outer], all of one type; `activation` is GPB_ACT_*. out must not
  * overlap an input. float32 products are formed from three bfloat16 parts per
- * value (float32 accuracy): with more than 8 rows, an input beyond 3.3895e38
- * or not finite makes the outputs that depend on it NaN. */
+ * value (float32 accuracy): with more than 4 rows, an input beyond 3.3895e38
+ * or not finite makes the outputs that depend on it NaN. (Up to 8 rows may be
+ * computed without the tensor cores, depending on the sizes.) */
 int gpb_gated_unit_workspace(int32_t dtype, int64_t rows, int64_t inner, int64_t outer,
                              int32_t backward, int64_t* bytes_out);
 int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activation, int64_t rows,
@@ -497,7 +498,9 @@ int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activati
  * (the projections are recomputed, nothing is kept from the forward call):
  * dx [rows][inner], dw_gate and dw_up [outer][inner], db_gate and db_up
  * [outer], each optional (NULL). Outputs overlap neither inputs nor one
- * another. rows = 0 writes zero weight and bias gradients. */
+ * another. rows = 0 writes zero weight and bias gradients. Where out's own
+ * factors (dout up act', dout act) are not finite, the gradients that depend
+ * on them are infinite or NaN. */
 int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t activation,
                             int64_t rows, int64_t inner, int64_t outer, const void* dout_dev,
                             int64_t dout_ld, const void* x_dev, int64_t x_ld,
