@@ -265,85 +265,104 @@ __global__ void __launch_bounds__(1024) gated_rows_join_kernel(const float* __re
 }
 
 // Matrices to tensor-core operands, one per blockIdx.y: fp32 weights to three bf16 planes, or a matrix
-// whose rows are not 16-byte aligned to a copy whose are (`copy`). 8 output columns per step; columns
-// up to ld are zeros.
+// whose rows are not 16-byte aligned to a copy whose are (`copy`). Columns up to ld are zeros.
 struct PackArgs {
   const void* src[3];
   void* dst[3];
   int64_t rows[3], src_ld[3];
   int32_t copy[3];
   int64_t cols, ld;
-  int32_t lanes_log2;
 };
-// Threads: 2^lanes_log2 along a row, the others along rows, kPackRows of them each; blockIdx.z: column steps
-// of few rows (195 x 6669 fp32 in 2 blocks: 140 us). 16-bit rows are read
-// as the 4-byte words they touch (5 for 8 elements), in reach of neighbours through L1, and shifted.
-constexpr int kPackRows = 4;
+// 16 bytes from an address that is only 2-byte aligned, of which the first `bytes` are asked for: the one or
+// two aligned blocks that hold them, shifted.
+__device__ __forceinline__ void load_blocks(const void* p, int64_t bytes, uint4& a, uint4& b) {
+  const int off = (int)((uintptr_t)p & 15);
+  const uint4* q = reinterpret_cast<const uint4*>((const char*)p - off);
+  a = b = make_uint4(0, 0, 0, 0);
+  if (bytes > 0) a = q[0];
+  if (off + (bytes < 16 ? bytes : 16) > 16) b = q[1];
+}
+__device__ __forceinline__ uint4 shift_blocks(const void* p, const uint4& a, const uint4& b) {
+  const int off = (int)((uintptr_t)p & 15);
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t h[6], o[5];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) h[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) o[i] = off & 4 ? h[i + 1] : h[i];
+  const int bits = (off & 2) * 8;
+  return make_uint4(__funnelshift_r(o[0], o[1], bits), __funnelshift_r(o[1], o[2], bits),
+                    __funnelshift_r(o[2], o[3], bits), __funnelshift_r(o[3], o[4], bits));
+}
+
+// HBM bound. A thread takes a few columns at a time (16 bits: eight, read as the aligned 16-byte blocks that
+// hold them; fp32: two), and a block consecutive ones, rows end to end: whole lines whatever the rows' width
+// and alignment, and no idle lanes at a row's end. Lanes assigned to rows, and unaligned words 16 or 32
+// bytes apart, went through L1 several times: forward 94812 x 519 -> 51 bf16 126 us in all, 85 this way;
+// 21764 x 3975 fp16 99 us of packing, now 62 (5.6 TB/s).
+template <typename T>
+struct PackShape {
+  static constexpr int kCols = sizeof(T) == 4 ? 2 : 8;
+  static constexpr int kItems = sizeof(T) == 4 ? 8 : 4;  // per thread
+};
 template <typename T, typename D>
 __global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__ PackArgs A) {
+  constexpr int COLS = PackShape<T>::kCols, ITEMS = PackShape<T>::kItems;
   const int o = blockIdx.y;
-  const int lanes = 1 << A.lanes_log2;
-  const int tx = threadIdx.x & (lanes - 1);
-  const int64_t row_step = 256 >> A.lanes_log2;
-  const int64_t row0 = blockIdx.x * row_step * kPackRows + (threadIdx.x >> A.lanes_log2);
-  if (row0 >= A.rows[o]) return;
-  for (int64_t c = (blockIdx.z * lanes + tx) * 8; c < A.ld; c += (int64_t)gridDim.z * lanes * 8) {
-    uint32_t w[kPackRows][sizeof(T) == 4 ? 8 : 5];
+  const int64_t rows = A.rows[o], first = (int64_t)blockIdx.x * (256 * ITEMS);
+  const uint32_t per = (uint32_t)(A.ld / COLS);
+  const int64_t row0 = first / per;
+  if (row0 >= rows) return;
+  const uint32_t at0 = (uint32_t)(first - row0 * per) + threadIdx.x;
+  const int left_rows = (int)(rows - row0 < (1 << 30) ? rows - row0 : 1 << 30);
+  const T* src0 = (const T*)A.src[o] + row0 * A.src_ld[o];
+  int r[ITEMS], c[ITEMS];
 #pragma unroll
-    for (int u = 0; u < kPackRows; ++u) {
-      const int64_t r = row0 + u * row_step;
-      const bool in = r < A.rows[o];
-      const T* src = (const T*)A.src[o] + r * A.src_ld[o] + c;
-      if constexpr (sizeof(T) == 4) {
+  for (int u = 0; u < ITEMS; ++u) {
+    const uint32_t at = at0 + u * 256;
+    r[u] = (int)(at / per);
+    c[u] = (int)(at - r[u] * per) * COLS;
+  }
+  if constexpr (sizeof(T) == 4) {
+    float2 w[ITEMS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          w[u][i] = in && c + i < A.cols ? reinterpret_cast<const uint32_t*>(src)[i] : 0u;
-      } else {
-        const int64_t odd = ((uintptr_t)src >> 1) & 1;
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(src - odd);
-#pragma unroll
-        for (int i = 0; i < 5; ++i) {  // a word is read when it holds an element of the row
-          const int64_t e = c + 2 * i - odd;
-          w[u][i] = in && e < A.cols && (i < 4 || odd) ? p[i] : 0u;
-        }
-      }
+    for (int u = 0; u < ITEMS; ++u) {
+      const T* src = src0 + r[u] * A.src_ld[o] + c[u];
+      const bool in = r[u] < left_rows;
+      w[u].x = in && c[u] < A.cols ? src[0] : 0.f;
+      w[u].y = in && c[u] + 1 < A.cols ? src[1] : 0.f;
     }
 #pragma unroll
-    for (int u = 0; u < kPackRows; ++u) {
-      const int64_t r = row0 + u * row_step;
-      if (r >= A.rows[o]) break;
-      if constexpr (sizeof(T) == 4) {
-        if (A.copy[o]) {
-          uint4* dst = reinterpret_cast<uint4*>((T*)A.dst[o] + r * A.ld + c);
-          dst[0] = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
-          dst[1] = make_uint4(w[u][4], w[u][5], w[u][6], w[u][7]);
-        } else {
-          D* dst = (D*)A.dst[o] + r * A.ld + c;
-          float2 x[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x[i] = make_float2(__uint_as_float(w[u][2 * i]), __uint_as_float(w[u][2 * i + 1]));
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            uint32_t h[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = gg_part<D>(x[i]);
-            *reinterpret_cast<uint4*>(dst + k * A.rows[o] * A.ld) =
-                make_uint4(h[0], h[1], h[2], h[3]);
-          }
-        }
+    for (int u = 0; u < ITEMS; ++u) {
+      if (r[u] >= left_rows) break;
+      const int64_t at = (row0 + r[u]) * A.ld + c[u];
+      if (A.copy[o]) {
+        *reinterpret_cast<float2*>((T*)A.dst[o] + at) = w[u];
       } else {
-        const T* src = (const T*)A.src[o] + r * A.src_ld[o] + c;
-        const uint32_t shift = ((uintptr_t)src & 2) * 8;
-        uint32_t h[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          h[i] = __funnelshift_r(w[u][i], w[u][i + 1], shift);
-          // Columns past the row are zeros.
-          if (c + 2 * i + 1 >= A.cols) h[i] = c + 2 * i < A.cols ? h[i] & 0xFFFFu : 0u;
-        }
-        *reinterpret_cast<uint4*>((T*)A.dst[o] + r * A.ld + c) = make_uint4(h[0], h[1], h[2], h[3]);
+        for (int k = 0; k < 3; ++k)
+          *reinterpret_cast<uint32_t*>((D*)A.dst[o] + k * rows * A.ld + at) = gg_part<D>(w[u]);
       }
+    }
+  } else {
+    uint4 a[ITEMS], b[ITEMS];
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u)
+      load_blocks(src0 + r[u] * A.src_ld[o] + c[u], r[u] < left_rows ? 2 * (A.cols - c[u]) : 0, a[u],
+                  b[u]);
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      if (r[u] >= left_rows) break;
+      const uint4 q = shift_blocks(src0 + r[u] * A.src_ld[o] + c[u], a[u], b[u]);
+      uint32_t h[4] = {q.x, q.y, q.z, q.w};
+      const int64_t left = A.cols - c[u];
+      if (left < COLS) {  // columns past the row are zeros
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (2 * i + 1 >= left) h[i] = 2 * i < left ? h[i] & 0xFFFFu : 0u;
+      }
+      *reinterpret_cast<uint4*>((T*)A.dst[o] + (row0 + r[u]) * A.ld + c[u]) =
+          make_uint4(h[0], h[1], h[2], h[3]);
     }
   }
 }
@@ -690,17 +709,9 @@ static int gated_operands(const GatedArgs& A, const GatedPlan& P, char* ws, Oper
   operand(A.wg, A.outer, A.w_ld, ws + P.wg, wg, kPlanes);
   operand(A.wu, A.outer, A.w_ld, ws + P.wu, wu, kPlanes);
   if (count) {
-    // Lanes along a row: at least 8 (or the row), and as few idle ones in its last step as that allows.
-    const int64_t per = P.ldk / 8;
-    while (K.lanes_log2 < 3 && (1 << K.lanes_log2) < per) ++K.lanes_log2;
-    for (int l = K.lanes_log2 + 1; l <= 8; ++l)
-      if (round_up(per, (int64_t)1 << l) <= round_up(per, (int64_t)1 << K.lanes_log2))
-        K.lanes_log2 = l;
-    const int64_t per_block = (256 >> K.lanes_log2) * kPackRows;
-    const int64_t blocks = ceil_div(most, per_block);
-    const int64_t steps = ceil_div(per, (int64_t)1 << K.lanes_log2);
-    const int64_t split = std::min(steps, ceil_div(8 * kFeatSMs, blocks));
-    gated_pack_kernel<T, D><<<dim3((unsigned)blocks, count, (unsigned)split), 256, 0, st>>>(K);
+    using S = PackShape<T>;
+    const int64_t blocks = ceil_div(most * P.ldk, (int64_t)S::kCols * 256 * S::kItems);
+    gated_pack_kernel<T, D><<<dim3((unsigned)blocks, count), 256, 0, st>>>(K);
     GPB_CHECK_CUDA(cudaGetLastError());
   }
   return GPB_OK;
