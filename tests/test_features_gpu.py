@@ -293,6 +293,59 @@ def test_gated_unit_split_repeats(ft):
         assert torch.equal(a, b)
 
 
+def test_gated_unit_split_outputs_alone_and_in_a_graph(ft):
+    rows, inner, outer, t = 50, 4096, 530, torch.bfloat16
+    full = gated_case(ft, rows, inner, outer, "bf16", "silu", True)
+    x, dy = randn(11, rows, inner, dtype=t), randn(16, rows, outer, dtype=t)
+    wg = randn(12, outer, inner, dtype=t, scale=inner ** -0.5)
+    wu = randn(13, outer, inner, dtype=t, scale=inner ** -0.5)
+    bg, bu = randn(14, outer, dtype=t, scale=0.3), randn(15, outer, dtype=t, scale=0.3)
+    ws = torch.empty(ft.gated_unit_workspace(rows, inner, outer, t, backward=True), dtype=torch.uint8,
+                     device="cuda")
+    names = ["dx", "dw_gate", "dw_up", "db_gate", "db_up"]
+    for name, want in zip(names, full[1:]):
+        got = torch.empty_like(want)
+        ft.gated_unit_backward(dy, x, wg, wu, bg, bu, workspace=ws, **{name: got})
+        assert torch.equal(got, want), name
+    got = [torch.zeros_like(v) for v in full]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stream = torch.cuda.current_stream().cuda_stream
+        ft.gated_unit(got[0], x, wg, wu, bg, bu, workspace=ws, stream=stream)
+        ft.gated_unit_backward(dy, x, wg, wu, bg, bu, workspace=ws, stream=stream,
+                               **dict(zip(names, got[1:])))
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for g, w in zip(got, full):
+        assert torch.equal(g, w)
+
+
+def test_gated_unit_split_padding_stays_out_of_the_sums(ft):
+    """The rows of a split product's last tile past the caller's add nothing to any gradient, whatever a
+    bias holds."""
+    rows, inner, outer, t = 33, 2048, 70, torch.bfloat16
+    x, dy = randn(1, rows, inner, dtype=t), randn(2, rows, outer, dtype=t)
+    wg, wu = randn(3, outer, inner, dtype=t, scale=0.02), randn(4, outer, inner, dtype=t, scale=0.02)
+    bg, bu = torch.zeros(outer, dtype=t, device="cuda"), torch.zeros(outer, dtype=t, device="cuda")
+    bu[5] = float("inf")
+    ws = torch.full((ft.gated_unit_workspace(rows, inner, outer, t, backward=True),), 0xFF,
+                    dtype=torch.uint8, device="cuda")
+    dbg, dbu = torch.zeros_like(bg), torch.zeros_like(bg)
+    ft.gated_unit_backward(dy, x, wg, wu, bg, bu, db_gate=dbg, db_up=dbu, workspace=ws)
+    gate = x.double() @ wg.double().T
+    val, _ = act_ref("silu", gate)
+    want = (dy.double() * val).sum(0)
+    eg = sum_error(inner, False) * (x.double().abs() @ wg.double().abs().T)
+    ev = 1.13 * eg + 2.0 ** -22 * (4 + gate * gate) * val.abs()
+    term = dy.double().abs() * ev
+    bound = term.sum(0) + (rows + 20) * E24 * ((dy.double() * val).abs() + term).sum(0)
+    check(dbu, want, bound + half_step(t) * (want.abs() + bound))
+    keep = torch.arange(outer, device="cuda") != 5
+    assert torch.isfinite(dbg[keep]).all() and not torch.isfinite(dbg[5])
+
+
 @pytest.mark.parametrize("rows", [3, 140])
 @pytest.mark.parametrize("pad,offset", [(8, 0), (3, 0), (0, 1), (5, 3)])
 def test_gated_unit_split_strides(ft, rows, pad, offset):
