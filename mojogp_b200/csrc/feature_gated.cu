@@ -515,7 +515,7 @@ static int make_map(const Operand& o, int box_cols, int box_rows, CUtensorMap* m
   return GPB_OK;
 }
 
-// Workspace of a call; every offset is a multiple of 256 bytes.
+// Workspace of a call; every offset from its 32-byte aligned base is a multiple of 256 bytes.
 struct GatedPlan {
   bool few = false;                    // CUDA-core path
   int planes = 1;                      // of packed x and weights
@@ -533,6 +533,11 @@ struct GatedPlan {
   int64_t sums = 0;                    // column sums of dgate and dup
   int ranges_x = 1;                    // dx of few rows
 };
+
+// The kernels store whole 32-byte sectors into the workspace (st.global.v8), while a caller's is 16-byte
+// aligned: its base is rounded up, into 16 bytes that the size asked for has to spare.
+static int64_t workspace_need(const GatedPlan& P) { return P.total > 0 ? P.total + 16 : 0; }
+static char* workspace_base(void* p) { return (char*)(((uintptr_t)p + 31) & ~(uintptr_t)31); }
 
 static int64_t take(int64_t& at, int64_t bytes) {
   const int64_t o = at;
@@ -996,7 +1001,7 @@ int gpb_gated_unit_workspace(int32_t dtype, int64_t rows, int64_t inner, int64_t
   clear_error();
   GPB_REQUIRE(bytes_out, GPB_ERR_INVALID, "null output");
   GPB_TRY(gated_check(dtype, rows, inner, outer));
-  *bytes_out = gated_plan(rows, inner, outer, dtype, backward != 0).total;
+  *bytes_out = workspace_need(gated_plan(rows, inner, outer, dtype, backward != 0));
   return GPB_OK;
 }
 
@@ -1025,16 +1030,17 @@ int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activati
                   !overlaps(out_dev, ob, b_up_dev, outer * es),
               GPB_ERR_INVALID, "out overlaps an input");
   const GatedPlan P = gated_plan(rows, inner, outer, dtype, false);
-  GPB_REQUIRE(P.total == 0 || (workspace_dev && workspace_bytes >= P.total), GPB_ERR_INVALID,
-              "gated unit needs a workspace of %lld bytes, got %lld", (long long)P.total,
+  const int64_t need = workspace_need(P);
+  GPB_REQUIRE(need == 0 || (workspace_dev && workspace_bytes >= need), GPB_ERR_INVALID,
+              "gated unit needs a workspace of %lld bytes, got %lld", (long long)need,
               (long long)(workspace_dev ? workspace_bytes : 0));
   GPB_REQUIRE(aligned16(workspace_dev), GPB_ERR_INVALID, "workspace is not 16-byte aligned");
-  GPB_REQUIRE(!overlaps(workspace_dev, P.total, out_dev, ob) &&
-                  !overlaps(workspace_dev, P.total, x_dev, span_bytes(rows, inner, x_ld, es)) &&
-                  !overlaps(workspace_dev, P.total, w_gate_dev, wb) &&
-                  !overlaps(workspace_dev, P.total, w_up_dev, wb) &&
-                  !overlaps(workspace_dev, P.total, b_gate_dev, outer * es) &&
-                  !overlaps(workspace_dev, P.total, b_up_dev, outer * es),
+  GPB_REQUIRE(!overlaps(workspace_dev, need, out_dev, ob) &&
+                  !overlaps(workspace_dev, need, x_dev, span_bytes(rows, inner, x_ld, es)) &&
+                  !overlaps(workspace_dev, need, w_gate_dev, wb) &&
+                  !overlaps(workspace_dev, need, w_up_dev, wb) &&
+                  !overlaps(workspace_dev, need, b_gate_dev, outer * es) &&
+                  !overlaps(workspace_dev, need, b_up_dev, outer * es),
               GPB_ERR_INVALID, "the workspace overlaps an input or out");
   GPB_DEVICE_SCOPE(device);
   GatedArgs A{};
@@ -1052,12 +1058,13 @@ int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activati
   A.outer = outer;
   A.act = activation;
   cudaStream_t st = (cudaStream_t)stream;
+  char* ws = workspace_base(workspace_dev);
   switch (dtype) {
     case GPB_DTYPE_F32:
-      return gated_forward<float, __nv_bfloat16, 3>(A, (char*)workspace_dev, P, st);
-    case GPB_DTYPE_F16: return gated_forward<__half, __half, 1>(A, (char*)workspace_dev, P, st);
+      return gated_forward<float, __nv_bfloat16, 3>(A, ws, P, st);
+    case GPB_DTYPE_F16: return gated_forward<__half, __half, 1>(A, ws, P, st);
     default:
-      return gated_forward<__nv_bfloat16, __nv_bfloat16, 1>(A, (char*)workspace_dev, P, st);
+      return gated_forward<__nv_bfloat16, __nv_bfloat16, 1>(A, ws, P, st);
   }
 }
 
@@ -1099,8 +1106,9 @@ int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t
                   elem_aligned(b_gate_dev, es) && elem_aligned(b_up_dev, es),
               GPB_ERR_INVALID, "pointer is not aligned to its element type");
   const GatedPlan P = gated_plan(rows, inner, outer, dtype, true);
-  GPB_REQUIRE(workspace_dev && workspace_bytes >= P.total, GPB_ERR_INVALID,
-              "the backward pass needs a workspace of %lld bytes, got %lld", (long long)P.total,
+  const int64_t need = workspace_need(P);
+  GPB_REQUIRE(workspace_dev && workspace_bytes >= need, GPB_ERR_INVALID,
+              "the backward pass needs a workspace of %lld bytes, got %lld", (long long)need,
               (long long)(workspace_dev ? workspace_bytes : 0));
   GPB_REQUIRE(aligned16(workspace_dev), GPB_ERR_INVALID, "workspace is not 16-byte aligned");
   {
@@ -1112,7 +1120,7 @@ int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t
     const int64_t dwb = span_bytes(outer, inner, dw_ld, es);
     const struct { const void* p; int64_t n; } out[] = {
         {dx_dev, span_bytes(rows, inner, dx_ld, es)}, {dw_gate_dev, dwb}, {dw_up_dev, dwb},
-        {db_gate_dev, bb}, {db_up_dev, bb}, {workspace_dev, P.total}};
+        {db_gate_dev, bb}, {db_up_dev, bb}, {workspace_dev, need}};
     for (int o = 0; o < 6; ++o) {
       for (const auto& i : in)
         GPB_REQUIRE(!overlaps(out[o].p, out[o].n, i.p, i.n), GPB_ERR_INVALID,
@@ -1138,12 +1146,13 @@ int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t
   A.outer = outer;
   A.act = activation;
   GatedGrads G{dx_dev, dx_ld, dw_gate_dev, dw_up_dev, dw_ld, db_gate_dev, db_up_dev};
+  char* ws = workspace_base(workspace_dev);
   switch (dtype) {
     case GPB_DTYPE_F32:
-      return gated_backward<float, __nv_bfloat16, 3>(A, G, (char*)workspace_dev, P, st);
-    case GPB_DTYPE_F16: return gated_backward<__half, __half, 1>(A, G, (char*)workspace_dev, P, st);
+      return gated_backward<float, __nv_bfloat16, 3>(A, G, ws, P, st);
+    case GPB_DTYPE_F16: return gated_backward<__half, __half, 1>(A, G, ws, P, st);
     default:
-      return gated_backward<__nv_bfloat16, __nv_bfloat16, 1>(A, G, (char*)workspace_dev, P, st);
+      return gated_backward<__nv_bfloat16, __nv_bfloat16, 1>(A, G, ws, P, st);
   }
 }
 

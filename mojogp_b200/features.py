@@ -12,9 +12,9 @@ biases and statistics.
 Calls are asynchronous on `stream` (an integer CUDA stream handle; None or 0
 is the legacy default stream), allocate nothing, and can be captured into a
 CUDA graph (after a first call on the device outside of any capture); where one
-takes a workspace, it is any array of at least the bytes the matching
-*_workspace function returns, not shared by calls that may run at the same
-time. Argument errors raise ValueError before any device work.
+takes a workspace, it is any 16-byte aligned array of at least the bytes the
+matching *_workspace function returns, not shared by calls that may run at the
+same time. Argument errors raise ValueError before any device work.
 """
 from __future__ import annotations
 

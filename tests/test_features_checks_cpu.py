@@ -1,0 +1,51 @@
+"""Argument checks and size queries of the feature-map operators, without a GPU."""
+import pytest
+
+from mojogp_b200 import _lib
+from test_features_cpu import MB, FakeArray, arr, refuse
+
+
+@pytest.fixture()
+def ft(gpb_lib):
+    from mojogp_b200 import features
+    return features
+
+
+def no_device(fn, *a, **kw):
+    """The call passes its checks: it ends where it looks for its device (64, which no machine here has)."""
+    with pytest.raises(_lib.GPBError) as e:
+        fn(*a, **kw)
+    assert not isinstance(e.value, ValueError) and "device 64" in str(e.value)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("rows,inner,outer", [(1, 64, 48), (4, 600, 500), (16, 4104, 72), (100, 64, 64),
+                                              (300, 517, 33), (3000, 1024, 2048)])
+@pytest.mark.parametrize("backward", [False, True])
+def test_gated_workspace_base_is_rounded_up(gpb_lib, rows, inner, outer, dtype, backward):
+    """The kernels store 32-byte sectors into the workspace, whose base need only be 16-byte aligned: the
+    parts, 256-byte multiples from the rounded base, still end inside the size asked for."""
+    from mojogp_b200 import features as ft
+    need = ft.gated_unit_workspace(rows, inner, outer, dtype, backward=backward)
+    if need == 0:
+        assert not backward and rows <= 8  # the CUDA cores' forward pass has none
+        return
+    parts = need // 256 * 256
+    for base in (1 << 20, (1 << 20) + 16, (1 << 20) + 32, (1 << 20) + 48):
+        rounded = -(-base // 32) * 32
+        assert rounded + parts <= base + need
+
+
+def test_gated_workspace_of_any_allowed_alignment_is_taken(ft):
+    n = dict(device=64)
+    x, w, u, y = arr((64, 8), **n), arr((6, 8), 2, **n), arr((6, 8), 3, **n), arr((64, 6), 4, **n)
+    need = ft.gated_unit_workspace(64, 8, 6, "float32", backward=True)
+    for off in (0, 16, 32):
+        ws = FakeArray((need,), dtype="uint8", ptr=512 * MB + off, **n)
+        no_device(ft.gated_unit, y, x, w, u, workspace=ws)
+        no_device(ft.gated_unit_backward, y, x, w, u, dx=arr((64, 8), 5, **n), workspace=ws)
+    for off in (4, 8, 24):
+        ws = FakeArray((need,), dtype="uint8", ptr=512 * MB + off, **n)
+        refuse("aligned", ft.gated_unit_backward, y, x, w, u, dx=arr((64, 8), 5, **n), workspace=ws)
+    short = FakeArray((need - 1,), dtype="uint8", ptr=512 * MB, **n)
+    refuse("workspace", ft.gated_unit_backward, y, x, w, u, dx=arr((64, 8), 5, **n), workspace=short)
