@@ -573,9 +573,13 @@ static int launch_ig(InputGradArgs& A, cudaStream_t st) {
     kernel<<<dim3((unsigned)ceil_div(A.n, 128), kIgCluster), kIgcThreads, IgcShape<D>::kSmem, st>>>(A);
   } else {
     constexpr int R = D <= 16 ? 2 : 1;  // a row's state is 2 D + 8 values
-    const size_t smem = (size_t)R * kIgThreads * D * sizeof(float);
-    input_gradient_kernel<LEAF, D, R>
-        <<<dim3((unsigned)ceil_div(A.n, R * kIgThreads), kIgCluster), kIgThreads, smem, st>>>(A);
+    constexpr int smem = R * kIgThreads * D * (int)sizeof(float);
+    // The column tiles are static shared memory beside it: 50 KB in all at 64 dimensions.
+    constexpr int tiles = 2 * kIgTile * (D + 8) * (int)sizeof(float);
+    static_assert(smem + tiles <= 227 * 1024, "shared memory of a block");
+    constexpr auto kernel = input_gradient_kernel<LEAF, D, R>;
+    if constexpr (smem + tiles > 47 * 1024) GPB_TRY(allow_smem<kernel>(smem));
+    kernel<<<dim3((unsigned)ceil_div(A.n, R * kIgThreads), kIgCluster), kIgThreads, smem, st>>>(A);
   }
   GPB_CHECK_CUDA(cudaGetLastError());
   return GPB_OK;
