@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs A) {
   for (int k = 0; k < loops; ++k) {
     copy_wait<kNormAhead<R> - 1>();
     fetch();  // into the slot of the row before this one, whose values are long used
-    const float scale = rstd, shift = -mean * rstd;
+    const float scale = rstd, shift = -mean;
     if (k + 1 < mine) {
       mp += step;
       rp += step;
@@ -513,7 +513,8 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(const NormArgs A) {
       unpack16(dr, g[r], (const T*)nullptr);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        xh[r][i] = __ffma2_rn(xh[r][i], scale2, shift2);
+        // Subtracted first: x rstd - mean rstd would lose |mean| rstd 2^-24 in rows far from zero.
+        xh[r][i] = __fmul2_rn(__fadd2_rn(xh[r][i], shift2), scale2);
         if constexpr (PARAMS) {
           dw[r][i] = __ffma2_rn(g[r][i], xh[r][i], dw[r][i]);
           db[r][i] = __fadd2_rn(g[r][i], db[r][i]);
