@@ -462,7 +462,8 @@ int gpb_feature_status(int32_t device, int32_t* status_out);
  * rstd = 1 / sqrt(mean((x - mean)^2) + eps). weight and bias [cols] may be
  * NULL (1 and 0) and are param_dtype: float32 or x's type. mean_dev and
  * rstd_dev [rows] float32 are written where not NULL. out may be x itself
- * (same pointer and leading dimension). */
+ * (same pointer and leading dimension). A variance beyond float32's largest
+ * counts as infinite: rstd = 0, out = bias. */
 int gpb_layer_norm(int32_t device, void* stream, int32_t dtype, int32_t param_dtype, int64_t rows,
                    int64_t cols, void* out_dev, int64_t out_ld, const void* x_dev, int64_t x_ld,
                    const void* weight_dev, const void* bias_dev, float eps, float* mean_dev,

@@ -57,10 +57,11 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, int flip) {
 }
 
 // 1 / sqrt(v), v >= 0: the hardware's estimate and one Newton step (about 1 ulp; a division and a
-// square root cost 30 instructions a row).
+// square root cost 30 instructions a row). The estimate of 0 is infinity and that of infinity 0: they
+// are the results, and a step from them would be NaN.
 __device__ __forceinline__ float inv_sqrt(float v) {
   const float r = rsqrtf(v);
-  return v > 0.f ? fmaf(fmaf(-0.5f * v * r, r, 0.5f), r, r) : r;
+  return v > 0.f && r > 0.f ? fmaf(fmaf(-0.5f * v * r, r, 0.5f), r, r) : r;
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {

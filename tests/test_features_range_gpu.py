@@ -53,3 +53,20 @@ def test_layer_norm_backward_far_from_zero(ft, rows, cols, dtype, mean):
     ref, mag = (D * xh).sum(0), (D * xh).abs().sum(0)
     bound = k * mag + (D.abs() * e_x).sum(0)
     check(dw, ref, bound + E24 * (ref.abs() + bound))
+
+
+# One vector per thread of few and many rows, several vectors, unaligned rows of few and many, wide rows.
+@pytest.mark.parametrize("rows,cols", [(3, 16), (5000, 64), (40, 1000), (40, 999), (700, 999), (700, 4096),
+                                       (3, 20001)])
+def test_layer_norm_of_an_infinite_variance(ft, rows, cols):
+    """A variance beyond float32 is infinite in the formula's float32: rstd = 0 and out = bias."""
+    x = randn(34, rows, cols, scale=1e20)
+    x[1] = randn(35, cols)
+    w, b = randn(36, cols), randn(37, cols)
+    y, rstd = torch.empty_like(x), torch.empty(rows, device="cuda")
+    ft.layer_norm(y, x, w, b, rstd=rstd)
+    far = torch.arange(rows, device="cuda") != 1
+    assert (rstd[far] == 0).all() and torch.equal(y[far], b.expand(rows, cols)[far])
+    one = torch.empty((1, cols), device="cuda")
+    ft.layer_norm(one, x[1:2], w, b)
+    torch.testing.assert_close(y[1:2], one, rtol=1e-5, atol=1e-5)
