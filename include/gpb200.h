@@ -499,9 +499,11 @@ int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activati
  * (the projections are recomputed, nothing is kept from the forward call):
  * dx [rows][inner], dw_gate and dw_up [outer][inner], db_gate and db_up
  * [outer], each optional (NULL). Outputs overlap neither inputs nor one
- * another. rows = 0 writes zero weight and bias gradients. Where out's own
- * factors (dout up act', dout act) are not finite, the gradients that depend
- * on them are infinite or NaN. */
+ * another. rows = 0 writes zero weight and bias gradients. Where the factors
+ * of the gradients (dout up act', dout act) are not finite in float32, the
+ * gradients that depend on them are infinite or NaN. In float16 the factors are
+ * kept as float16 parts times a power of two of the call: they may pass
+ * float16's range, and one below 2^-21 of the call's largest counts as 0. */
 int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t activation,
                             int64_t rows, int64_t inner, int64_t outer, const void* dout_dev,
                             int64_t dout_ld, const void* x_dev, int64_t x_ld,

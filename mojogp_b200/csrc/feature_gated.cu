@@ -371,6 +371,14 @@ __global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__
 template <typename T, typename D, int PD, bool BACK>
 __global__ void __launch_bounds__(1024) gated_finish_kernel(const __grid_constant__ GgArgs A) {
   __shared__ float sums[32][2][33];
+  float scale = 1.f;  // of float16 factors
+  if constexpr (kGgScaled<D> && BACK) {
+    if (A.redo) {
+      const int k = gg_factor_exp(*A.largest);
+      if (k == 0) return;
+      scale = gg_pow2(k);
+    }
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t n = (int64_t)blockIdx.x * 32 + lane, ld = (A.N + 15) / 16 * 16;
   const bool in = n < A.N;
@@ -397,7 +405,7 @@ __global__ void __launch_bounds__(1024) gated_finish_kernel(const __grid_constan
       su = d[1];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float rest = d[h];
+        float rest = d[h] * scale;
 #pragma unroll
         for (int p = 0; p < PD; ++p) {
           const D part = from_f<D>(rest);
@@ -410,6 +418,11 @@ __global__ void __launch_bounds__(1024) gated_finish_kernel(const __grid_constan
     }
   }
   if constexpr (BACK) {
+    if constexpr (kGgScaled<D>) {
+      const uint32_t top =
+          __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(gg_magnitude(sg), gg_magnitude(su))));
+      if (lane == 0 && !A.redo && top > 0) atomicMax(A.largest, top);
+    }
     if (!A.col_sums) return;
     sums[warp][0][lane] = sg;
     sums[warp][1][lane] = su;
@@ -531,6 +544,7 @@ struct GatedPlan {
   int splits_x = 1, kb_per_x = 1;      // GG_DX
   int64_t partial_x = 0;
   int64_t sums = 0;                    // column sums of dgate and dup
+  int64_t largest = 0;                 // float16: bits of the largest |dgate|, |dup|
   int ranges_x = 1;                    // dx of few rows
 };
 
@@ -645,6 +659,7 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
     P.splits_x = (int)ceil_div(kbx, P.kb_per_x);
     P.partial_x = take(at, P.splits_x > 1 ? P.splits_x * rows * round_up(inner, 16) * 4 : 0);
     P.sums = take(at, 4 * ceil_div(rows, kGgBM) * 2 * outer * 4);
+    P.largest = take(at, dtype == GPB_DTYPE_F16 ? 4 : 0);
   }
   P.total = at;
   return P;
@@ -757,11 +772,14 @@ static int gated_project(const GatedArgs& A, const GatedPlan& P, char* ws, const
         return (int)GPB_ERR_UNSUPPORTED;
     }
   };
-  GPB_TRY(run());
-  if (G.splits > 1) {
-    const dim3 grid((unsigned)ceil_div(A.outer, 32), (unsigned)(4 * ceil_div(A.rows, kGgBM)));
-    gated_finish_kernel<T, D, PD, BACK><<<grid, 1024, 0, st>>>(G);
-    GPB_CHECK_CUDA(cudaGetLastError());
+  constexpr int passes = BACK && kGgScaled<D> ? 2 : 1;  // the second one scales, where it has to
+  for (G.redo = 0; G.redo < passes; ++G.redo) {
+    if (G.redo == 0 || G.splits == 1) GPB_TRY(run());
+    if (G.splits > 1) {
+      const dim3 grid((unsigned)ceil_div(A.outer, 32), (unsigned)(4 * ceil_div(A.rows, kGgBM)));
+      gated_finish_kernel<T, D, PD, BACK><<<grid, 1024, 0, st>>>(G);
+      GPB_CHECK_CUDA(cudaGetLastError());
+    }
   }
   return GPB_OK;
 }
@@ -865,6 +883,8 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
   Operand x, wg, wu;
   GPB_TRY((gated_operands<T, D>(A, P, ws, &x, &wg, &wu, st)));
   float* partial = (float*)(ws + P.partial);
+  uint32_t* largest = (uint32_t*)(ws + P.largest);
+  if constexpr (kGgScaled<D>) GPB_CHECK_CUDA(cudaMemsetAsync(largest, 0, sizeof(*largest), st));
   Operand dg, du;
   dg.p = ws + P.dg;
   du.p = ws + P.du;
@@ -875,6 +895,7 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
   dg.plane = du.plane = P.plane_d;
   {
     GgArgs G{};
+    G.largest = largest;
     G.out[0] = ws + P.dg;
     G.out[1] = ws + P.du;
     G.out_ld = P.ldn;
@@ -885,6 +906,7 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
   }
   if (R.dx) {
     GgArgs G{};
+    G.largest = largest;
     const int nb = plain_tile(A.inner, PL == 3);
     G.M = A.rows;
     G.N = A.inner;
@@ -906,6 +928,7 @@ static int gated_backward_tc(const GatedArgs& A, const GatedGrads& R, char* ws, 
   }
   if (R.dwg || R.dwu) {
     GgArgs G{};
+    G.largest = largest;
     const bool joined = A.outer <= 64;
     G.M = A.outer;
     G.N = A.inner;

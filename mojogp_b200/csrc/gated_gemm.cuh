@@ -153,6 +153,8 @@ struct GgArgs {
   const void* bu;
   const void* dout;
   float* col_sums;     // backward GG_PROJ: [4 tiles_m][2][N] column sums of dgate and dup, or null
+  uint32_t* largest;   // float16 backward: bits of the largest |dgate|, |dup| (gg_factor_exp)
+  int32_t redo;        // float16 backward GG_PROJ: the pass that writes scaled factors
   int64_t dout_ld;
   int32_t act;
   int32_t vec;         // output rows (backward GG_PROJ: dout rows) are 2: 32-byte, 1: 16-byte aligned
@@ -367,6 +369,26 @@ __device__ __forceinline__ void gg_store_rows(T* out, int64_t ld, int64_t row0, 
   __syncwarp();
 }
 
+// float16 dgate and dup are written as they are, and their largest magnitude is found on the way. If that
+// is 2^15 or more, where float16 ends, or below 2^-4, where the half of its smallest step (2^-25) is more
+// than 2^-21 of it, a second pass writes them times 2^k, the largest one then in [2^13, 2^14); GG_DX and GG_DW
+// divide by it again. The second pass ends at once where k is 0. (A maximum is the same in any order, so
+// results repeat.) Unscaled, a finite factor beyond 65504 made a row of dx and a column of dW NaN, and a
+// small gradient vanished. Backward 8192 x 1024 -> 4096: bf16, which needs none of this, 329 us, fp16 348, and
+// 482 where it scales; 16 x 2048 -> 8192 75, 82 and 95. k, from the largest magnitude's bits; 0 where all factors are.
+template <typename D>
+constexpr bool kGgScaled = std::is_same<D, __half>::value;
+__device__ __forceinline__ int gg_factor_exp(uint32_t bits) {
+  if (bits == 0) return 0;
+  const int e = (int)(bits >> 23) - 127;
+  return e >= -4 && e < 15 ? 0 : min(13 - e, 126);
+}
+// A factor's part in the maximum: one that is not finite stays its own and has none.
+__device__ __forceinline__ float gg_magnitude(float v) {
+  return fabsf(v) < __int_as_float(0x7F800000) ? fabsf(v) : 0.f;
+}
+__device__ __forceinline__ float gg_pow2(int k) { return __int_as_float((k + 127) << 23); }
+
 // 16 columns of the lane's row m to the output's type; vec: 2 = 32-byte aligned rows, 1 = 16-byte, 0 =
 // neither. The whole warp takes part.
 template <typename T>
@@ -471,7 +493,7 @@ template <typename T, typename D, int PD, bool BACK>
 __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int split, int64_t m, int64_t n,
                                               const float* bias, int step, const GgRow<T>& dy,
                                               float* col_sums, float* tile, int lane, float (&g)[16],
-                                              float (&u)[16]) {
+                                              float (&u)[16], float scale, float& largest) {
   const int64_t left = A.N - n;
   if (A.splits > 1) {
     const int64_t ld = (A.N + 15) / 16 * 16;
@@ -506,6 +528,10 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int split, int64_
 #pragma unroll
       for (int i = 0; i < 16; ++i) g[i] = u[i] = 0.f;
     }
+    if constexpr (kGgScaled<D>) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) largest = fmaxf(largest, fmaxf(gg_magnitude(g[i]), gg_magnitude(u[i])));
+    }
     if (col_sums && left > 0) {  // uniform over the warp
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -522,7 +548,10 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int split, int64_
       D* dst = (D*)A.out[h] + m * A.out_ld + n;
       float2 x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = make_float2(v[2 * i], v[2 * i + 1]);
+      for (int i = 0; i < 8; ++i) {
+        x[i] = make_float2(v[2 * i], v[2 * i + 1]);
+        if constexpr (kGgScaled<D>) x[i] = __fmul2_rn(x[i], make_float2(scale, scale));
+      }
 #pragma unroll
       for (int p = 0; p < PD; ++p) {
         uint32_t w[8];
@@ -537,9 +566,14 @@ __device__ __forceinline__ void gg_proj_store(const GgArgs& A, int split, int64_
 
 // Epilogue of 16 columns of a GG_DX or GG_DW tile. The warp's 32 rows belong to one weight (halves of a
 // shared tile are 64 rows).
-template <typename T, int MODE>
+template <typename T, typename D, int MODE>
 __device__ __forceinline__ void gg_plain_store(const GgArgs& A, int split, int mt, int lane_row,
-                                               int64_t n, float (&v)[16], float* tile, int lane) {
+                                               int64_t n, float (&v)[16], float* tile, int lane,
+                                               float scale) {
+  if constexpr (kGgScaled<D>) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] *= scale;
+  }
   int half = 0;
   int64_t m;
   if constexpr (MODE == GG_DW) {
@@ -616,6 +650,14 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
   __shared__ uint32_t tmem_base;
   __shared__ __align__(16) float bias_tile[kGgEpiWarps][MODE == GG_PROJ ? 2 * (BN / 2) : 4];
   __shared__ float row_tile[kGgEpiWarps][kGgTile];
+  float scale = 1.f, largest = 0.f;  // of float16 factors
+  if constexpr (kGgScaled<D> && (BACK || MODE != GG_PROJ)) {
+    if (MODE != GG_PROJ || A.redo) {
+      const int k = gg_factor_exp(*A.largest);
+      if (MODE == GG_PROJ && k == 0) return;  // the whole grid
+      scale = gg_pow2(MODE == GG_PROJ ? k : -k);
+    }
+  }
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t raw = base + STAGES * S::kStage;
   constexpr int BK = S::kBK;
@@ -891,12 +933,13 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
                 g[i] = __uint_as_float(rg[i]);
                 u[i] = __uint_as_float(ru[i]);
               }
-              gg_proj_store<T, D, PD, BACK>(A, I.split, m, n + c, bias + c, HC, dy, col_sums, tile, lane, g, u);
+              gg_proj_store<T, D, PD, BACK>(A, I.split, m, n + c, bias + c, HC, dy, col_sums, tile, lane, g, u,
+                                            scale, largest);
             } else {
               float v[16];
               tmem_ld16(t + c, v);
               release();
-              gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v, tile, lane);
+              gg_plain_store<T, D, MODE>(A, I.split, mt, lane_row, n + c, v, tile, lane, scale);
             }
           }
           __syncwarp();  // this tile's biases are read before the next tile's are written
@@ -948,9 +991,9 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
                 if (c + 16 < HC) dy_next.load(A, m, n + c + 16, tile, lane);
               }
               gg_proj_store<T, D, PD, BACK>(A, I.split, m, n + c, bias + c, HC, dy, col_sums, tile, lane, v[0],
-                                            v[R - 1]);
+                                            v[R - 1], scale, largest);
             } else {
-              gg_plain_store<T, MODE>(A, I.split, mt, lane_row, n + c, v[0], tile, lane);
+              gg_plain_store<T, D, MODE>(A, I.split, mt, lane_row, n + c, v[0], tile, lane, scale);
             }
           }
           __syncwarp();
@@ -958,6 +1001,10 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
       }
     }
     if (!ok) atomicExch(A.err, DEV_WAIT_TIMEOUT);
+    if constexpr (kGgScaled<D> && MODE == GG_PROJ && BACK) {
+      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
+      if (lane == 0 && !A.redo && A.splits == 1 && top > 0) atomicMax(A.largest, top);
+    }
   }
   tc_fence_before();
   if constexpr (PAIR)

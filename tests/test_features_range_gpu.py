@@ -70,3 +70,134 @@ def test_layer_norm_of_an_infinite_variance(ft, rows, cols):
     one = torch.empty((1, cols), device="cuda")
     ft.layer_norm(one, x[1:2], w, b)
     torch.testing.assert_close(y[1:2], one, rtol=1e-5, atol=1e-5)
+
+
+# ------------------------------------------------------------------- gated unit
+def gated_grads_in_range(ft, rows, inner, outer, act, x_scale, w_scale, up_bias, dy_scale, want):
+    """float16 gradients `want` of factors dout up act' and dout act that float16 itself does not hold.
+    They are kept as float16 parts of their values times one power of two: off by half a step of the
+    type (U), or by half the smallest step: 2^-25 where the largest factor is 2^-4 to 2^15, 2^-37
+    of the largest otherwise."""
+    t, u = torch.float16, half_step(torch.float16)
+    x = randn(41, rows, inner, dtype=t, scale=x_scale)
+    wg, wu = (randn(s, outer, inner, dtype=t, scale=w_scale) for s in (42, 43))
+    bg = randn(44, outer, dtype=t, scale=0.3)
+    bu = randn(45, outer, dtype=t, scale=0.2 * up_bias, shift=up_bias)
+    dy = randn(46, rows, outer, dtype=t, scale=dy_scale)
+    out = {"dx": torch.zeros_like(x), "dw_gate": torch.zeros_like(wg), "dw_up": torch.zeros_like(wu),
+           "db_gate": torch.zeros_like(bg), "db_up": torch.zeros_like(bu)}
+    out = {k: out[k] for k in want}
+    ws = torch.full((ft.gated_unit_workspace(rows, inner, outer, t, backward=True),), 0xFF,
+                    dtype=torch.uint8, device="cuda")
+    ft.gated_unit_backward(dy, x, wg, wu, bg, bu, activation=act, workspace=ws, **out)
+    X, G, U, D = x.double(), wg.double(), wu.double(), dy.double()
+    gate, up = X @ G.T + bg.double(), X @ U.T + bu.double()
+    e = sum_error(inner, False)
+    eg = e * (X.abs() @ G.abs().T) + E23 * gate.abs()
+    eu = e * (X.abs() @ U.abs().T) + E23 * up.abs()
+    val, slope = act_ref(act, gate)
+    ev = 1.13 * eg + 2.0 ** -22 * (4 + gate * gate) * val.abs()
+    es = eg + 2.0 ** -21 * (1 + gate.abs())
+    dg, du = D * up * slope, D * val
+    largest = max(dg.abs().max().item(), du.abs().max().item())
+    tiny = max(2.0 ** -37 * largest, 2.0 ** -25 if largest > 0.06 else 0.0)
+    edg = D.abs() * (slope.abs() * eu + up.abs() * es + es * eu) + 2.0 ** -22 * dg.abs()
+    edg = edg + u * (dg.abs() + edg) + tiny
+    edu = D.abs() * ev + E23 * du.abs()
+    edu = edu + u * (du.abs() + edu) + tiny
+    if "dx" in out:
+        ref = dg @ G + du @ U
+        e = sum_error(2 * outer, False)
+        bound = edg @ G.abs() + edu @ U.abs()
+        bound = bound + e * ((dg.abs() + edg) @ G.abs() + (du.abs() + edu) @ U.abs())
+        check(out["dx"], ref, bound + u * (ref.abs() + bound))
+    e = sum_error(rows, False)
+    for name, d, ed in (("gate", dg, edg), ("up", du, edu)):
+        if "dw_" + name in out:
+            ref = d.T @ X
+            bound = ed.T @ X.abs() + e * ((d.abs() + ed).T @ X.abs())
+            check(out["dw_" + name], ref, bound + u * (ref.abs() + bound))
+        if "db_" + name in out:
+            ref = d.sum(0)
+            bound = ed.sum(0) + (rows + 20) * E24 * (d.abs() + ed).sum(0)
+            check(out["db_" + name], ref, bound + u * (ref.abs() + bound))
+    return dg, du, largest, out
+
+
+# On both sides of the CUDA-core path's bound, with split and unsplit projections, unaligned rows, both
+# weights in one tile, and on CTA pairs with one part per factor.
+RANGE_SHAPES = [(2, 520, 520), (3, 520, 520), (9, 64, 48), (100, 64, 48), (33, 71, 65), (140, 2100, 130),
+                (300, 96, 300), (2660, 1800, 1000)]
+
+
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+@pytest.mark.parametrize("rows,inner,outer", RANGE_SHAPES)
+def test_gated_unit_float16_factors_beyond_the_type(ft, rows, inner, outer, act):
+    """up of some 300 under a gradient of some 200: factors up to 10^6, gradients within float16."""
+    s = 0.02 / math.sqrt(max(1, max(inner, outer, rows) / 100))
+    dg, _, largest, _ = gated_grads_in_range(ft, rows, inner, outer, act, s, s, 300.0,
+                                             200.0 if act == "silu" else 400.0,
+                                             ["dx", "dw_gate", "dw_up"])
+    assert largest > 65504
+
+
+@pytest.mark.parametrize("rows,inner,outer", RANGE_SHAPES)
+def test_gated_unit_float16_factors_below_the_type(ft, rows, inner, outer):
+    """A gradient of a few of float16's smallest steps, 2^-24, against large weights (dx) and large inputs
+    (the weight gradients)."""
+    w = 2.0 ** 10
+    for names, xs, wscale in ((["dx"], 2.0 ** -10 / math.sqrt(inner), w),
+                              (["dw_gate", "dw_up"], w, 2.0 ** -10 / math.sqrt(inner))):
+        _, _, largest, _ = gated_grads_in_range(ft, rows, inner, outer, "silu", xs, wscale, 0.5,
+                                                2.0 ** -22, names)
+        assert largest < 2.0 ** -15
+
+
+def test_gated_unit_float16_factors_repeat_and_in_a_graph(ft):
+    """A captured call follows its inputs: the factors' scale is found anew at each replay."""
+    rows, inner, outer, t = 200, 64, 96, torch.float16
+    x, dy = randn(1, rows, inner, dtype=t, scale=0.02), randn(2, rows, outer, dtype=t)
+    wg, wu = randn(3, outer, inner, dtype=t, scale=0.02), randn(4, outer, inner, dtype=t, scale=0.02)
+    bg, bu = randn(5, outer, dtype=t), randn(6, outer, dtype=t, shift=300.0)
+    ws = torch.empty(ft.gated_unit_workspace(rows, inner, outer, t, backward=True), dtype=torch.uint8,
+                     device="cuda")
+
+    def call(out, stream=None):
+        ft.gated_unit_backward(dy, x, wg, wu, bg, bu, dx=out[0], dw_gate=out[1], dw_up=out[2],
+                               workspace=ws, stream=stream)
+
+    new = lambda: [torch.zeros_like(x), torch.zeros_like(wg), torch.zeros_like(wu)]
+    got = new()
+    call(got)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(got, torch.cuda.current_stream().cuda_stream)
+    for scale in (200.0, 2.0 ** -20, 0.0, 1.0, 200.0):
+        dy.copy_(randn(2, rows, outer, scale=scale))
+        want = new()
+        call(want)
+        graph.replay()
+        torch.cuda.synchronize()
+        for g, v in zip(got, want):
+            assert torch.isfinite(v).all() and torch.equal(g, v), scale
+            assert (v != 0).any() == (scale != 0)
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(100, 64, 48), (140, 2100, 130), (2660, 1800, 1000)])
+def test_gated_unit_float16_non_finite_factors_stay_their_own(ft, rows, inner, outer):
+    """A row with an infinite or NaN gradient leaves the other rows' dx as it is, scaled or not."""
+    t = torch.float16
+    x, dy = randn(1, rows, inner, dtype=t, scale=0.02), randn(2, rows, outer, dtype=t, scale=200.0)
+    wg, wu = (randn(s, outer, inner, dtype=t, scale=0.2 / math.sqrt(inner)) for s in (3, 4))
+    bg, bu = randn(5, outer, dtype=t), randn(6, outer, dtype=t, shift=300.0)
+    ws = torch.empty(ft.gated_unit_workspace(rows, inner, outer, t, backward=True), dtype=torch.uint8,
+                     device="cuda")
+    want, got = torch.zeros_like(x), torch.zeros_like(x)
+    ft.gated_unit_backward(dy, x, wg, wu, bg, bu, dx=want, workspace=ws)
+    dy[3, 5], dy[rows - 2, 7] = float("inf"), float("nan")
+    ft.gated_unit_backward(dy, x, wg, wu, bg, bu, dx=got, workspace=ws)
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+    rest[3] = rest[rows - 2] = False
+    assert torch.isfinite(want).all() and torch.equal(got[rest], want[rest])
+    assert not torch.isfinite(got[3]).any() and not torch.isfinite(got[rows - 2]).any()
