@@ -367,7 +367,8 @@ __global__ void __launch_bounds__(256) gated_pack_kernel(const __grid_constant__
   }
 }
 
-// Joins a projection's ranges and runs its epilogue: 32 rows x 32 columns to a block, a warp to a row.
+// Joins a projection's ranges and runs its epilogue: 32 rows x 32 columns to a block (blocks along the
+// columns first), a warp to a row.
 template <typename T, typename D, int PD, bool BACK>
 __global__ void __launch_bounds__(1024) gated_finish_kernel(const __grid_constant__ GgArgs A) {
   __shared__ float sums[32][2][33];
@@ -380,12 +381,13 @@ __global__ void __launch_bounds__(1024) gated_finish_kernel(const __grid_constan
     }
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t n = (int64_t)blockIdx.x * 32 + lane, ld = (A.N + 15) / 16 * 16;
+  const unsigned across = (unsigned)((A.N + 31) / 32), by = blockIdx.x / across, bx = blockIdx.x - by * across;
+  const int64_t n = (int64_t)bx * 32 + lane, ld = (A.N + 15) / 16 * 16;
   const bool in = n < A.N;
   const float bg = in && A.bg ? to_f(((const T*)A.bg)[n]) : 0.f;
   const float bu = in && A.bu ? to_f(((const T*)A.bu)[n]) : 0.f;
   float sg = 0.f, su = 0.f;
-  const int64_t m = (int64_t)blockIdx.y * 32 + warp;
+  const int64_t m = (int64_t)by * 32 + warp;
   if (m < A.M && in) {
     const float* src = A.partial + m * ld + n;
     float gate = 0.f, up = 0.f;
@@ -428,12 +430,12 @@ __global__ void __launch_bounds__(1024) gated_finish_kernel(const __grid_constan
     sums[warp][1][lane] = su;
     __syncthreads();
     // Warp w adds column w's rows, one per lane.
-    const int64_t c = (int64_t)blockIdx.x * 32 + warp;
+    const int64_t c = (int64_t)bx * 32 + warp;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float s = sums[lane][h][warp];
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0 && c < A.N) A.col_sums[((int64_t)blockIdx.y * 2 + h) * A.N + c] = s;
+      if (lane == 0 && c < A.N) A.col_sums[((int64_t)by * 2 + h) * A.N + c] = s;
     }
   }
 }
@@ -567,6 +569,12 @@ static int64_t take(int64_t& at, int64_t bytes) {
 // cost half the call's time or more, and the outputs' sums are long enough to average the rounding.
 constexpr int64_t kTwoPlanes = (int64_t)1 << 31;
 
+// Stages of a 16-bit product's reduction that one accumulator takes. The tensor core truncates every term
+// at 2^-25 of the accumulator, half of that on average, so k terms of one sign lose some k 2^-27: 16384 terms
+// 2^-13, half of float16's own rounding (2^20 terms in one range came out 6e-3 short). Longer reductions
+// split into ranges whose partial sums are added in fp32 (16 bytes an output for every 65536 operations).
+static int64_t longest_range(int planes) { return 16384 / kGgBK / planes; }
+
 // Rows of an A tile that a single row tile loads: whole groups of 8 (the swizzle's unit).
 static int tile_rows(int64_t rows) {
   return rows < kGgBM ? (int)round_up(rows, 8) : kGgBM;
@@ -630,7 +638,8 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
     // 256 for fp32 (8192 -> 1024 bf16 at 16 rows: 44 us in one range, 23.5 in four).
     const int64_t kb = ceil_div(inner, f32 ? kGgSplitBK : kGgBK);
     const int64_t tiles = ceil_div(rows, kGgBM) * ceil_div(outer, proj_tile(rows, outer, f32) / 2);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles, inner / (f32 ? 256 : 1024)));
+    int64_t want = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles, inner / (f32 ? 256 : 1024)));
+    if (!f32) want = std::max(want, ceil_div(kb, longest_range(1)));
     P.kb_per_p = (int)ceil_div(kb, want);
     P.splits_p = (int)ceil_div(kb, P.kb_per_p);
     P.partial_p = take(at, P.splits_p > 1 ? P.splits_p * 2 * rows * round_up(outer, 16) * 4 : 0);
@@ -645,7 +654,8 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
     const int bk = f32 ? kGgSplitBK : kGgBK;
     const int64_t kb = ceil_div(rows, bk);
     // At least 8 stages per range; as many ranges as fill the SMs twice.
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * kFeatSMs / tiles, kb / 8));
+    int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * kFeatSMs / tiles, kb / 8));
+    if (!f32) want = std::max(want, ceil_div(kb, longest_range(P.planes_d)));
     P.kb_per = (int)ceil_div(kb, want);
     P.splits = (int)ceil_div(kb, P.kb_per);
     P.partial = take(at, P.splits > 1 ? P.splits * 2 * outer * round_up(inner, 16) * 4 : 0);
@@ -654,7 +664,8 @@ static GatedPlan gated_plan(int64_t rows, int64_t inner, int64_t outer, int32_t 
     // 16 rows, 2048 -> 8192: 8 tiles, 159 us in one range).
     const int64_t kbx = 2 * ceil_div(outer, kGgBK);
     const int64_t tiles_x = ceil_div(rows, kGgBM) * ceil_div(inner, P.tile_n);
-    const int64_t want_x = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles_x, kbx / (f32 ? 4 : 8)));
+    int64_t want_x = std::max<int64_t>(1, std::min<int64_t>(kFeatSMs / tiles_x, kbx / (f32 ? 4 : 8)));
+    if (!f32) want_x = std::max(want_x, ceil_div(kbx, longest_range(P.planes_d)));
     P.kb_per_x = (int)ceil_div(kbx, want_x);
     P.splits_x = (int)ceil_div(kbx, P.kb_per_x);
     P.partial_x = take(at, P.splits_x > 1 ? P.splits_x * rows * round_up(inner, 16) * 4 : 0);
@@ -776,7 +787,7 @@ static int gated_project(const GatedArgs& A, const GatedPlan& P, char* ws, const
   for (G.redo = 0; G.redo < passes; ++G.redo) {
     if (G.redo == 0 || G.splits == 1) GPB_TRY(run());
     if (G.splits > 1) {
-      const dim3 grid((unsigned)ceil_div(A.outer, 32), (unsigned)(4 * ceil_div(A.rows, kGgBM)));
+      const unsigned grid = (unsigned)(ceil_div(A.outer, 32) * 4 * ceil_div(A.rows, kGgBM));
       gated_finish_kernel<T, D, PD, BACK><<<grid, 1024, 0, st>>>(G);
       GPB_CHECK_CUDA(cudaGetLastError());
     }

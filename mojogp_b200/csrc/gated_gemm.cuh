@@ -6,8 +6,9 @@
 //            activation and the product (or, for the backward pass, forms dgate and dup);
 //   GG_DX    dx = dgate Wg + dup Wu      one accumulation over two segments;
 //   GG_DW    dWg = dgate' x, dWu = dup' x   the reduction runs over rows.
-// A product with too few tiles for the SMs splits its reduction over CTAs (fp32 partial sums, joined in
-// split order; GG_PROJ's epilogue then runs in the join).
+// A product with too few tiles for the SMs, or a 16-bit one with a longer reduction than an accumulator that
+// truncates should take, splits its reduction over CTAs (fp32 partial sums, joined in split order; GG_PROJ's
+// epilogue then runs in the join).
 // x and the weights are read where they lie. A product whose reduction index is not the contiguous
 // one takes its operand MN-major: the tensor core transposes, nothing is copied.
 //
@@ -16,7 +17,7 @@
 // bytes an element from HBM instead of a pass of 10 and 6 per use), and
 // a product keeps the six plane pairs above 2^-24 of it: hi hi apart from the five small ones, which
 // have their own accumulator. The tensor core truncates where it adds, about 2^-26 of the accumulator
-// per MMA, so after every kGgWindow blocks of the reduction the epilogue warps add both accumulators
+// per term, so after every kGgWindow blocks of the reduction the epilogue warps add both accumulators
 // to registers in fp32 and the MMAs start again from zero.
 //
 // Wide 16-bit products run on CTA pairs (cta_group::2): one MMA covers 256 rows x 256 columns, each

@@ -201,3 +201,56 @@ def test_gated_unit_float16_non_finite_factors_stay_their_own(ft, rows, inner, o
     rest[3] = rest[rows - 2] = False
     assert torch.isfinite(want).all() and torch.equal(got[rest], want[rest])
     assert not torch.isfinite(got[3]).any() and not torch.isfinite(got[rows - 2]).any()
+
+
+# Reductions of one sign, in sizes whose tiles alone fill the SMs. The tensor core truncates each term at 2^-25
+# of the accumulator, which holds half of its final value on average: a range of 2^14 terms is at most
+# 2^-12 short of its sum of magnitudes. The joins add 2^-24 a range, the activation 2^-21.
+SHORT = 2.0 ** -12 + 2.0 ** -16 + 2.0 ** -21
+
+
+def positive(seed, *shape):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.rand(shape, generator=g, device="cuda", dtype=torch.float16) * 2.0 ** -6
+
+
+def test_gated_unit_long_reduction(ft):
+    t = torch.float16
+    rows, inner, outer = 1280, 1 << 20, 1000
+    x, wu = positive(3, rows, inner), positive(4, outer, inner)
+    wg = torch.zeros_like(wu)  # sigmoid(0) = 1/2
+    ws = torch.empty(ft.gated_unit_workspace(rows, inner, outer, t), dtype=torch.uint8, device="cuda")
+    out = torch.empty((rows, outer), dtype=t, device="cuda")
+    ft.gated_unit(out, x, wg, wu, activation="sigmoid", workspace=ws)
+    i, j = torch.arange(0, rows, 161, device="cuda"), torch.arange(0, outer, 99, device="cuda")
+    ref = 0.5 * torch.stack([(x[a].double()[None] * wu[j].double()).sum(1) for a in i])
+    check(out[i][:, j], ref, SHORT * ref + half_step(t) * (1 + SHORT) * ref)
+
+
+def test_gated_unit_long_reduction_of_the_weight_gradients(ft):
+    t = torch.float16
+    rows, inner, outer = 1 << 18, 2432, 1000
+    x, dy, wu = positive(5, rows, inner), positive(6, rows, outer), positive(7, outer, inner)
+    wg, dwu = torch.zeros_like(wu), torch.zeros_like(wu)
+    ws = torch.empty(ft.gated_unit_workspace(rows, inner, outer, t, backward=True), dtype=torch.uint8,
+                     device="cuda")
+    ft.gated_unit_backward(dy, x, wg, wu, dw_up=dwu, activation="sigmoid", workspace=ws)
+    i, j = torch.arange(0, inner, 97, device="cuda"), torch.arange(0, outer, 61, device="cuda")
+    ref = (dy[:, j].double() / 2).T @ x[:, i].double()
+    # dup = dout / 2 is exact in float16 but for its smallest steps, whatever the factors' scale.
+    bound = SHORT * ref + 2.0 ** -25 * x[:, i].double().sum(0)
+    check(dwu[j][:, i], ref, bound + half_step(t) * (ref + bound))
+
+
+def test_gated_unit_long_reduction_of_the_input_gradient(ft):
+    t = torch.float16
+    rows, inner, outer = 2432, 1000, 1 << 18
+    x, dy, wu = positive(8, rows, inner), positive(9, rows, outer), positive(10, outer, inner)
+    wg, dx = torch.zeros_like(wu), torch.zeros_like(x)
+    ws = torch.empty(ft.gated_unit_workspace(rows, inner, outer, t, backward=True), dtype=torch.uint8,
+                     device="cuda")
+    ft.gated_unit_backward(dy, x, wg, wu, dx=dx, activation="sigmoid", workspace=ws)
+    i, j = torch.arange(0, inner, 97, device="cuda"), torch.arange(0, rows, 61, device="cuda")
+    ref = (dy[j].double() / 2) @ wu[:, i].double()
+    bound = SHORT * ref + 2.0 ** -25 * wu[:, i].double().sum(0)
+    check(dx[j][:, i], ref, bound + half_step(t) * (ref + bound))
