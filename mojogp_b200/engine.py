@@ -13,7 +13,7 @@ from typing import Optional
 
 import numpy as np
 
-from . import _lib
+from . import _lib, features
 from .provider import DeviceBuffer, Provider
 
 
@@ -182,7 +182,8 @@ def train_features(provider: Provider, feature_map, X: np.ndarray, y: np.ndarray
     for it in range(max_iterations):
         t0 = time.perf_counter()
         feats = feature_map.forward(data, training=True, step=it)
-        provider.set_inputs(feats)
+        provider.set_inputs(feats)  # complete on return
+        features.check_device(provider.device)
         # Untrained parameters (a polynomial's degree) keep their value bit for bit.
         params = np.where(mask > 0, _softplus(raw[:P]), provider.params).astype(np.float32)
         provider.update_params(params)
@@ -231,6 +232,7 @@ def train_features(provider: Provider, feature_map, X: np.ndarray, y: np.ndarray
     provider.update_params(params)
     provider.update_noise(float(_softplus(best["raw"][P])) if learn_noise else 0.0)
     provider.set_inputs(feature_map.forward(data))
+    features.check_device(provider.device)
     feature_map.release()
     return {
         "final_nll": float(best["nll"]), "noise": provider.get_noise(), "mean": best["mean"],

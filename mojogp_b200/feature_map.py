@@ -180,7 +180,9 @@ class FeatureMap:
 
     def forward(self, x: DeviceBuffer, *, training: bool = False, step: int = 0) -> DeviceBuffer:
         """Features [n, output_dim], float32, of the rows of x (from `upload`);
-        the buffer is the map's own and holds until the next call. With
+        the buffer is the map's own and holds until the next call. Asynchronous
+        on the default stream: `features.check_device` after it (as `backward`
+        and `transform` do) raises if a kernel's bounded wait gave up. With
         `training`, dropout is drawn from (seed, step) and the activations are
         kept for `backward`."""
         if self.input_dim is None or tuple(x.shape[1:]) != (self.input_dim,):
@@ -274,7 +276,9 @@ class FeatureMap:
                 # The layer's input also reaches its output directly where the widths agree.
                 features.dropout(below, lay["dunit"], 0.0, 0,
                                  residual=lay["dout"] if lay["joined"] else None)
-        return [g.get() / np.float32(scale) for g in out]
+        grads = [g.get() / np.float32(scale) for g in out]
+        features.check_device(device)
+        return grads
 
     def transform(self, X: np.ndarray, device: int = 0, block: int = 65536) -> np.ndarray:
         """Features of host rows (no dropout), `block` rows at a time."""
@@ -284,6 +288,7 @@ class FeatureMap:
         out = np.empty((X.shape[0], self.output_dim), np.float32)
         for b in range(0, X.shape[0], block):
             out[b:b + block] = self.forward(self.upload(X[b:b + block], device)).download()
+            features.check_device(device)
         return out
 
     # -------------------------------------------------------------- persist
