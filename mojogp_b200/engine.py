@@ -129,6 +129,12 @@ def _inv_softplus(y):
     return np.where(y > 20.0, y, np.log(np.expm1(np.minimum(np.maximum(y, 1e-30), 20.0))))
 
 
+def _clip(g) -> np.ndarray:
+    """A gradient as `train` takes it: within +-100; 0 where it is NaN or beyond 1e30."""
+    g = np.asarray(g, np.float64)
+    return np.clip(np.where(np.abs(g) <= 1e30, g, 0.0), -100.0, 100.0)
+
+
 class _Adam:
     """Adam on a list of host arrays, in place (the moments and constants of `train`)."""
 
@@ -137,14 +143,18 @@ class _Adam:
         self.v = [np.zeros(a.shape) for a in arrays]
         self.t = 0
 
+    def state(self) -> tuple:
+        return list(self.m), list(self.v), self.t  # a step makes new moments
+
+    def restore(self, state: tuple) -> None:
+        self.m, self.v, self.t = list(state[0]), list(state[1]), state[2]
+
     def step(self, arrays, grads, lr: float) -> None:
         self.t += 1
         c1, c2 = 1.0 - 0.9 ** self.t, 1.0 - 0.999 ** self.t
-        for a, g, m, v in zip(arrays, grads, self.m, self.v):
-            g = np.clip(np.nan_to_num(np.asarray(g, np.float64), nan=0.0, posinf=0.0, neginf=0.0),
-                        -100.0, 100.0)
-            m += 0.1 * (g - m)
-            v += 0.001 * (g * g - v)
+        for i, (a, g) in enumerate(zip(arrays, grads)):
+            self.m[i] = m = 0.9 * self.m[i] + 0.1 * g
+            self.v[i] = v = 0.999 * self.v[i] + 0.001 * g * g
             a -= (lr * (m / c1) / (np.sqrt(v / c2) + 1e-8)).astype(a.dtype)
 
 
@@ -160,7 +170,9 @@ def train_features(provider: Provider, feature_map, X: np.ndarray, y: np.ndarray
     X to the provider's inputs, takes one BBMM step with the gradient by those
     inputs, and follows it back through the map; kernel parameters, noise and
     mean move as in `train`, the map's weights with `feature_learning_rate`
-    (default: learning_rate). The best iteration's state is restored and the
+    (default: learning_rate) under the same rules: gradients are clipped, an
+    iteration whose NLL is NaN goes back to the best state, moments included,
+    with half the rates. The best iteration's state is restored and the
     provider left at the map's outputs without dropout. The result's keys are
     `train`'s; the preconditioner is rebuilt every iteration, since the inputs
     move."""
@@ -175,10 +187,16 @@ def train_features(provider: Provider, feature_map, X: np.ndarray, y: np.ndarray
     kernel_adam, map_adam = _Adam([raw, mean]), _Adam(feature_map.parameters)
     data = feature_map.upload(X, provider.device)
     x_grad = DeviceBuffer((n, provider.d), provider.device)
-    best = {"nll": np.inf, "raw": raw.copy(), "mean": float(mean[0]),
-            "map": feature_map.snapshot()}
+    best = {}
+
+    def keep(nll):
+        best.update(nll=nll, raw=raw.copy(), mean=float(mean[0]), map=feature_map.snapshot(),
+                    moments=(kernel_adam.state(), map_adam.state()))
+
+    keep(1e30)
     history, times, cg_its = [], [], []
-    stop_best, stale, converged = np.inf, 0, False
+    stop_best, stale, converged = 1e30, 0, False
+    halved = 1.0  # of the constant schedule, after each NaN
     for it in range(max_iterations):
         t0 = time.perf_counter()
         feats = feature_map.forward(data, training=True, step=it)
@@ -194,26 +212,31 @@ def train_features(provider: Provider, feature_map, X: np.ndarray, y: np.ndarray
         nll = res["nll"]
         history.append(nll)
         cg_its.append(res["cg_iters"])
-        if nll < best["nll"]:
-            best = {"nll": nll, "raw": raw.copy(), "mean": float(mean[0]),
-                    "map": feature_map.snapshot()}
-        if np.isfinite(nll):
-            map_grads = feature_map.backward(x_grad)
-            slope = 1.0 / (1.0 + np.exp(-raw))
-            g = res["grads"] * slope
-            g[:P] *= mask
-            if not learn_noise:
-                g[P] = 0.0
-            scale = 1.0
-            if use_cosine_lr:
-                scale = 0.05 + 0.475 * (1.0 + np.cos(np.pi * it / max(max_iterations, 1)))
-            kernel_adam.step([raw, mean], [g, np.array([res["mean_grad"]])], learning_rate * scale)
-            np.clip(raw, -20.0, 20.0, out=raw)
-            map_adam.step(feature_map.parameters, map_grads, flr * scale)
-        else:  # back to the best state, with smaller steps
+        if np.isnan(nll):
+            halved *= 0.5
+            if verbose:
+                print(f"  NaN NLL at iteration {it} - halving LR to {learning_rate * halved:g}")
             raw[:], mean[0] = best["raw"], best["mean"]
+            kernel_adam.restore(best["moments"][0])
+            map_adam.restore(best["moments"][1])
             feature_map.restore(best["map"])
-            learning_rate, flr = 0.5 * learning_rate, 0.5 * flr
+            times.append((time.perf_counter() - t0) * 1e3)
+            continue
+        if nll < best["nll"]:
+            keep(nll)
+        map_grads = feature_map.backward(x_grad)
+        g = _clip(res["grads"]) / (1.0 + np.exp(-raw))  # clipped, then through softplus
+        g[:P] *= mask
+        if not learn_noise:
+            g[P] = 0.0
+        scale = halved
+        if use_cosine_lr:
+            scale = 0.05 + 0.475 * (1.0 + np.cos(np.pi * it / max(max_iterations, 1)))
+        kernel_adam.step([raw, mean], [g, _clip([res["mean_grad"]])], learning_rate * scale)
+        np.clip(raw, -20.0, 20.0, out=raw)
+        if not abs(mean[0]) <= 1000.0:
+            mean[0] = init_mean
+        map_adam.step(feature_map.parameters, [_clip(g) for g in map_grads], flr * scale)
         feature_map.parameters_changed()
         times.append((time.perf_counter() - t0) * 1e3)
         if verbose and (it % 10 == 0 or it == max_iterations - 1):

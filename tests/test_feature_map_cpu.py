@@ -97,3 +97,106 @@ def test_training_ends_where_a_wait_gave_up(host, monkeypatch, at):
     if at < 4:  # two checks a step, before the step's own update
         assert all(np.array_equal(a, b) for a, b in zip(fm.parameters, checks[-1]))
     prov.handle = None
+
+
+# ------------------------------------------------------------- the training loop's rules
+def script(seed, count, nan_at, params, shapes):
+    """What `count` steps find: NLLs (NaN at nan_at), gradients, some beyond the clip or not finite."""
+    rng = np.random.default_rng(seed)
+    steps = []
+    for i in range(count):
+        g = rng.standard_normal(params + 1) * 3
+        g[i % (params + 1)] *= 100  # clipped before the softplus factor
+        if i == 1:
+            g[0] = np.nan
+        if i == 4:
+            g[1] = np.inf
+        maps = [rng.standard_normal(s) * (200 if i % 3 == 0 else 1) for s in shapes]
+        steps.append(dict(nll=float("nan") if i in nan_at else 5.0 - i + (3.0 if i == 2 else 0.0), grads=g,
+                          mean_grad=[0.7, -250.0, float("nan")][i % 3], cg_iters=1, maps=maps))
+    return steps
+
+
+def restated(steps, raw, mean, weights, lr, flr, cosine, init_mean):
+    """The rules of the library's own loop (gpb_train) with the map's weights beside: the state that each
+    step starts from, and the best one."""
+    clip = lambda g: 0.0 if g != g or abs(g) > 1e30 else max(-100.0, min(100.0, g))
+    vec = np.concatenate([raw, [mean]] + [w.ravel() for w in weights]).astype(np.float64)
+    k = len(raw)
+    m, v, t = np.zeros_like(vec), np.zeros_like(vec), 0
+    best, seen, half, states = (1e30, vec.copy(), m.copy(), v.copy(), 0), [], 1.0, []
+    for i, s in enumerate(steps):
+        states.append(vec.copy())
+        if np.isnan(s["nll"]):
+            half *= 0.5
+            _, vec, m, v, t = best
+            vec, m, v = vec.copy(), m.copy(), v.copy()
+            continue
+        if s["nll"] < best[0]:
+            best = (s["nll"], vec.copy(), m.copy(), v.copy(), t)
+        g = np.concatenate([s["grads"], [s["mean_grad"]]] + [a.ravel() for a in s["maps"]])
+        g = np.array([clip(float(x)) for x in g])
+        g[:k] *= 1 / (1 + np.exp(-vec[:k]))
+        t += 1
+        m, v = 0.9 * m + 0.1 * g, 0.999 * v + 0.001 * g * g
+        rate = np.full(vec.shape, lr)
+        rate[k + 1:] = flr
+        low = 1 / 20
+        rate *= low + 0.5 * (1 - low) * (1 + np.cos(np.pi * i / len(steps))) if cosine else half
+        vec = vec - rate * (m / (1 - 0.9 ** t)) / (np.sqrt(v / (1 - 0.999 ** t)) + 1e-8)
+        vec[:k] = np.clip(vec[:k], -20, 20)
+        if not abs(vec[k]) <= 1000:
+            vec[k] = init_mean
+    return states, best
+
+
+@pytest.mark.parametrize("cosine", [False, True])
+@pytest.mark.parametrize("nan_at", [(), (0,), (3,), (3, 4, 7)])
+@pytest.mark.parametrize("lr", [0.05, 400.0])  # the second one drives the mean away
+def test_training_moves_as_the_library_does(host, monkeypatch, nan_at, cosine, lr):
+    fm = FeatureMap([3, 2], seed=2).build(4)
+    X = np.random.default_rng(0).standard_normal((6, 4)).astype(np.float32)
+    prov = Provider(np.zeros((6, 2), np.float32), RBF(), np.array([0.8, 1.3], np.float32), 0.1)
+    start = fm.snapshot()
+    steps = script(3, 9, nan_at, prov.num_params, [p.shape for p in start])
+    states, at = [], iter(steps)
+    now = {}
+
+    def step(provider, y, x_grad, **kw):
+        now.update(next(at))
+        states.append(np.concatenate([np.append(provider.params, provider._noise), [-float(y[0])]]
+                                     + [p.ravel() for p in fm.parameters]).astype(np.float64))
+        return {k: now[k] for k in ("nll", "grads", "mean_grad", "cg_iters")}
+
+    monkeypatch.setattr(engine, "bbmm_inputs", step)
+    monkeypatch.setattr(fm, "backward", lambda grad: now["maps"])
+    out = fit(fm, prov, X, len(steps), learning_rate=lr, feature_learning_rate=0.01, use_cosine_lr=cosine,
+              init_mean=0.5)
+    softplus = lambda r: np.logaddexp(0.0, r)
+    raw = np.log(np.expm1(np.array([0.8, 1.3, 0.1], np.float32).astype(np.float64)))
+    want, best = restated(steps, raw, 0.5, start, lr, 0.01, cosine, 0.5)
+    for i, (got, ref) in enumerate(zip(states, want, strict=True)):
+        # float32 weights and parameters: a rounding per step of each
+        ref = np.concatenate([softplus(ref[:3]), ref[3:]])
+        np.testing.assert_allclose(got, ref, rtol=20 * 2.0 ** -24, atol=20 * 2.0 ** -24 * (1 + 0.05 * lr),
+                                   err_msg=str(i))
+    assert out["final_nll"] == best[0] and out["iterations"] == len(steps)
+    np.testing.assert_allclose(out["params"], softplus(best[1][:2]), rtol=2e-6)
+    np.testing.assert_allclose(np.concatenate([p.ravel() for p in fm.parameters]), best[1][4:], rtol=2e-6,
+                               atol=2e-6)
+    assert abs(out["mean"] - best[1][3]) < 1e-4
+    assert len(out["iter_times_ms"]) == len(steps)
+    prov.handle = None
+
+
+def test_training_skips_a_nan_in_the_early_stop_count(host, monkeypatch):
+    fm = FeatureMap([2]).build(4)
+    X = np.ones((6, 4), np.float32)
+    prov = Provider(np.zeros((6, 2), np.float32), RBF(), np.ones(2, np.float32), 0.1)
+    nlls = iter([3.0, float("nan"), float("nan"), 4.0, float("nan"), 5.0, 6.0])
+    zero = dict(grads=np.zeros(3), mean_grad=0.0, cg_iters=1)
+    monkeypatch.setattr(engine, "bbmm_inputs", lambda *a, **kw: dict(zero, nll=next(nlls)))
+    monkeypatch.setattr(fm, "backward", lambda grad: [np.zeros(p.shape) for p in fm.parameters])
+    out = fit(fm, prov, X, 7, enable_early_stopping=True, early_stop_patience=2)
+    assert out["converged"] and out["iterations"] == 6
+    prov.handle = None
