@@ -80,6 +80,7 @@ class FeatureMap:
         self._run: Optional[dict] = None
         self._device = 0
         self._stale = True  # the device copies are older than `parameters`
+        self.version = 0  # counts the weights' changes
 
     # ------------------------------------------------------------- weights
     @property
@@ -122,8 +123,12 @@ class FeatureMap:
         self.parameters_changed()
 
     def parameters_changed(self) -> None:
-        """The host weights moved: the device copies follow at the next forward."""
+        """The host weights moved: the device copies follow at the next forward,
+        which `backward` needs first (it recomputes from the weights)."""
         self._stale = True
+        self.version += 1
+        if self._run is not None:
+            self._run["ready"] = False
 
     def _params(self, device: int) -> list:
         if self._device_params is None or self._device != device:

@@ -226,7 +226,9 @@ class SingleOutputGP:
                  feature_map: Optional[FeatureMap] = None):
         """`feature_map` puts a learned map under the kernel (no reference
         counterpart): the kernel sees its outputs, and fit() trains it with the
-        kernel's parameters on one GPU (a second fit continues from its weights)."""
+        kernel's parameters on one GPU (a second fit continues from its weights).
+        A model answers with the weights of its own fit: once they change, by
+        another model's fit say, predict() and save() raise."""
         if not isinstance(kernel, KernelNode):
             raise TypeError(
                 f"kernel must be a KernelNode instance (e.g. RBF(), Matern52()), got "
@@ -234,6 +236,7 @@ class SingleOutputGP:
         if feature_map is not None and not isinstance(feature_map, FeatureMap):
             raise TypeError(f"feature_map must be a FeatureMap, got {type(feature_map).__name__}")
         self.feature_map = feature_map
+        self._map_version: Optional[int] = None  # of the weights that the provider's inputs come from
         self.kernel_spec = kernel
         self.kernel: Optional[KernelNode] = None
         self.ard = kernel.has_ard()
@@ -382,6 +385,7 @@ class SingleOutputGP:
         else:
             res = engine.train_features(self._provider, fm, X, y,
                                         feature_learning_rate=feature_learning_rate, **options)
+            self._map_version = fm.version
         self._train_info = {"max_cg_iterations": cg["max_cg_iter"], "cg_tolerance": cg["cg_tol"],
                             "max_tridiag_iter": cg["max_tridiag_iter"],
                             "precond_rank": res["precond_rank"],
@@ -401,6 +405,11 @@ class SingleOutputGP:
     def _kernel_inputs(self, X: np.ndarray) -> np.ndarray:
         """What the kernel sees of input rows: the feature map's outputs, or the rows."""
         return X if self.feature_map is None else self.feature_map.transform(X, self.device)
+
+    def _check_map(self) -> None:
+        if self.feature_map is not None and self.feature_map.version != self._map_version:
+            raise RuntimeError("the feature map's weights changed after this model's fit (another model's "
+                               "fit, or restore()): fit again, or give each model its own map")
 
     # ---------------------------------------------------------------- predict
     def _solver_config(self, max_cg_iterations=None, cg_tolerance=None,
@@ -467,6 +476,7 @@ class SingleOutputGP:
         if Xt.ndim == 1 and self.dim == 1:
             Xt = Xt[:, None]
         _check_test_inputs(Xt, self.dim)
+        self._check_map()
         Xt = self._kernel_inputs(Xt)
         want_var = variance_method == "love"
         cache = self.prepare_prediction_cache("love" if want_var else "mean_only",
@@ -622,6 +632,7 @@ class SingleOutputGP:
         dropped, as in the reference."""
         if not self._is_trained:
             raise RuntimeError("GP must be trained before saving.")
+        self._check_map()
         base = _artifact_base(path)
         tr = self._training_result
         with open(f"{base}_config.json", "w") as f:
@@ -699,6 +710,7 @@ class SingleOutputGP:
             params=params, noise=config["noise"], mean=config.get("mean", 0.0),
             nll=config["nll"], iterations=config["iterations"], converged=config["converged"],
             lanczos_root=arrays.get("lanczos_root"), lanczos_rank=config["lanczos_rank"])
+        gp._map_version = None if fm is None else fm.version
         gp._provider = Provider(gp._kernel_inputs(X), gp.kernel, params, float(config["noise"]),
                                 device=device, noise_vector=gp._obs_noise)
         return gp

@@ -200,3 +200,46 @@ def test_training_skips_a_nan_in_the_early_stop_count(host, monkeypatch):
     out = fit(fm, prov, X, 7, enable_early_stopping=True, early_stop_patience=2)
     assert out["converged"] and out["iterations"] == 6
     prov.handle = None
+
+
+# ------------------------------------------------------------- whose weights a result has
+def test_a_model_refuses_another_fits_weights(host, monkeypatch, tmp_path):
+    """Two models over one map: the first one's training inputs came from weights that the second one's fit
+    moved, so its answers would mix both."""
+    from mojogp_b200 import SingleOutputGP
+    monkeypatch.setattr(engine, "bbmm_inputs", lambda provider, *a, **kw: dict(
+        nll=1.0, grads=np.ones(provider.num_params + 1), mean_grad=0.1, cg_iters=1))
+    fm = FeatureMap([4, 2])
+    rng = np.random.default_rng(0)
+    X, y = rng.standard_normal((8, 5)).astype(np.float32), np.ones(8, np.float32)
+    one, two = SingleOutputGP(RBF(), feature_map=fm), SingleOutputGP(RBF(), feature_map=fm)
+    one.fit(X, y, max_iterations=2, method="matrix_free")
+    one._check_map()
+    one.save(str(tmp_path / "one"))
+    two.fit(X, y, max_iterations=2, method="matrix_free")
+    two._check_map()
+    for call in (lambda: one.predict(X), lambda: one.predict(X, return_std=True),
+                 lambda: one.score(X, y), lambda: one.save(str(tmp_path / "again"))):
+        with pytest.raises(RuntimeError, match="weights changed"):
+            call()
+    fm.restore(fm.snapshot())
+    with pytest.raises(RuntimeError, match="weights changed"):
+        two.predict(X)
+    loaded = SingleOutputGP.load(str(tmp_path / "one"))
+    loaded._check_map()
+    one._provider.handle = None
+    one.fit(X, y, max_iterations=1, method="matrix_free")
+    one._check_map()
+    for gp in (one, two, loaded):
+        gp._provider.handle = None
+
+
+def test_backward_needs_the_weights_of_its_forward(host):
+    fm = FeatureMap([3, 2]).build(4)
+    grad = DeviceBuffer.from_host(np.ones((5, 2), np.float32))
+    fm.forward(fm.upload(np.ones((5, 4), np.float32)), training=True)
+    fm.backward(grad)
+    fm.parameters[2] += 1.0
+    fm.parameters_changed()
+    with pytest.raises(RuntimeError, match="forward"):
+        fm.backward(grad)
