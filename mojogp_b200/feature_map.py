@@ -19,6 +19,7 @@ from .provider import DeviceBuffer
 
 MAX_OUTPUTS = 64  # input dimensions a provider takes (GPB_MAX_DIM)
 _EPS = 1e-5
+_KEEP = 1 << 26  # bytes of activations that a prediction leaves for the next one (a new buffer costs some 0.1 ms)
 
 
 def _to_bfloat16_bits(a: np.ndarray) -> np.ndarray:
@@ -153,27 +154,39 @@ class FeatureMap:
         self.build(X.shape[1])
         return _Array(X.shape, device, self.dtype).put(X)
 
-    def _buffers(self, n: int, device: int) -> dict:
-        """Activations, gradients and the workspace for n rows, kept between calls of one size."""
-        if self._run is not None and self._run["n"] == n and self._run["device"] == device:
-            return self._run
-        run = {"n": n, "device": device, "layers": [], "grads": None, "ready": False}
-        inner = self.input_dim
-        need = 16
+    def _workspace_bytes(self, n: int, training: bool) -> int:
+        need, inner = 16, self.input_dim
         for outer in self.widths:
-            lay = {"out": _Array((n, outer), device, self.dtype)}
-            if self.norm:
-                lay["norm"] = _Array((n, inner), device, self.dtype)
-                lay["mean"], lay["rstd"] = (_Array((n,), device, "float32") for _ in range(2))
-                need = max(need, features.layer_norm_workspace(n, inner))
-            for backward in (False, True):
-                need = max(need, features.gated_unit_workspace(n, inner, outer, self.dtype, backward))
-            run["layers"].append(lay)
+            need = max(need, features.gated_unit_workspace(n, inner, outer, self.dtype))
+            if training:
+                need = max(need, features.gated_unit_workspace(n, inner, outer, self.dtype, backward=True),
+                           features.layer_norm_workspace(n, inner) if self.norm else 0)
             inner = outer
-        if self.dtype != "float32":
-            run["features"] = DeviceBuffer((n, self.output_dim), device)
-        run["workspace"] = DeviceBuffer((need,), device, np.uint8)
-        self._run = run
+        return need
+
+    def _buffers(self, n: int, device: int, training: bool) -> dict:
+        """Activations, gradients and the workspace for n rows, kept between calls of one size; the
+        backward pass's share of the workspace only where it is trained."""
+        run = self._run
+        if run is None or run["n"] != n or run["device"] != device:
+            self._run = None
+            run = {"n": n, "device": device, "layers": [], "grads": None, "ready": False,
+                   "workspace": None}
+            inner = self.input_dim
+            for outer in self.widths:
+                lay = {"out": _Array((n, outer), device, self.dtype)}
+                if self.norm:
+                    lay["norm"] = _Array((n, inner), device, self.dtype)
+                    lay["mean"], lay["rstd"] = (_Array((n,), device, "float32") for _ in range(2))
+                run["layers"].append(lay)
+                inner = outer
+            if self.dtype != "float32":
+                run["features"] = DeviceBuffer((n, self.output_dim), device)
+            self._run = run
+        need = self._workspace_bytes(n, training)
+        if run["workspace"] is None or run["workspace"].nbytes < need:
+            run["workspace"] = None
+            run["workspace"] = DeviceBuffer((need,), device, np.uint8)
         return run
 
     def release(self) -> None:
@@ -194,7 +207,7 @@ class FeatureMap:
             raise ValueError(f"x must be [n, {self.input_dim}], got {tuple(x.shape)}")
         n, device = x.shape[0], x.device
         params = self._params(device)
-        run = self._buffers(n, device)
+        run = self._buffers(n, device, training)
         run["ready"] = False
         ws, last = run["workspace"], len(self.widths) - 1
         cur = x
@@ -294,6 +307,9 @@ class FeatureMap:
         for b in range(0, X.shape[0], block):
             out[b:b + block] = self.forward(self.upload(X[b:b + block], device)).download()
             features.check_device(device)
+        held = self._run["layers"] if self._run is not None else []
+        if sum(b.nbytes for lay in held for b in lay.values() if isinstance(b, DeviceBuffer)) > _KEEP:
+            self.release()
         return out
 
     # -------------------------------------------------------------- persist

@@ -243,3 +243,26 @@ def test_backward_needs_the_weights_of_its_forward(host):
     fm.parameters_changed()
     with pytest.raises(RuntimeError, match="forward"):
         fm.backward(grad)
+
+
+# ------------------------------------------------------------- device memory
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_predictions_take_no_training_memory(host, dtype):
+    fm = FeatureMap([256, 8], dtype=dtype).build(20)
+    backward = max(features.gated_unit_workspace(3000, k, n, dtype, backward=True)
+                   for k, n in ((20, 256), (256, 8)))
+    forward = max(features.gated_unit_workspace(3000, k, n, dtype) for k, n in ((20, 256), (256, 8)))
+    assert forward < backward
+    host.memory.clear()
+    fm.transform(np.zeros((3000, 20), np.float32))
+    assert fm._run["workspace"].nbytes == forward
+    kept = fm._run["layers"][0]["out"].ptr
+    fm.transform(np.zeros((3000, 20), np.float32))
+    assert fm._run["layers"][0]["out"].ptr == kept  # a small prediction's buffers serve the next one
+    grad = DeviceBuffer.from_host(np.zeros((3000, 8), np.float32))
+    fm.forward(fm.upload(np.zeros((3000, 20), np.float32)), training=True)
+    assert fm._run["workspace"].nbytes >= backward and fm._run["layers"][0]["out"].ptr == kept
+    fm.backward(grad)
+    wide = FeatureMap([512, 8], dtype=dtype).build(300)
+    wide.transform(np.zeros((40000, 300), np.float32))
+    assert wide._run is None  # some 100 MB go back
