@@ -1006,6 +1006,9 @@ int gpb_layer_norm_backward(int32_t device, void* stream, int32_t dtype, int32_t
   GPB_REQUIRE((dx_dev == x_dev && dx_ld == x_ld) ||
                   !overlaps(dx_dev, dxb, x_dev, span_bytes(rows, cols, x_ld, es)),
               GPB_ERR_INVALID, "dx overlaps x (in place needs the same pointer and stride)");
+  GPB_REQUIRE(!overlaps(dx_dev, dxb, weight_dev, cols * ps) && !overlaps(dx_dev, dxb, mean_dev, rows * 4) &&
+                  !overlaps(dx_dev, dxb, rstd_dev, rows * 4),
+              GPB_ERR_INVALID, "dx overlaps weight, mean or rstd");
   if (params) {
     const int64_t need = (int64_t)norm_blocks(rows, cols) * 2 * cols * (int64_t)sizeof(float);
     GPB_REQUIRE(workspace_dev && workspace_bytes >= need, GPB_ERR_INVALID,

@@ -49,3 +49,13 @@ def test_gated_workspace_of_any_allowed_alignment_is_taken(ft):
         refuse("aligned", ft.gated_unit_backward, y, x, w, u, dx=arr((64, 8), 5, **n), workspace=ws)
     short = FakeArray((need - 1,), dtype="uint8", ptr=512 * MB, **n)
     refuse("workspace", ft.gated_unit_backward, y, x, w, u, dx=arr((64, 8), 5, **n), workspace=short)
+
+
+def test_layer_norm_backward_keeps_dx_off_its_other_inputs(ft):
+    """Rows of dx are written while other rows still read weight, mean and rstd."""
+    x, d, dx = arr((4, 8)), arr((4, 8), 2), arr((4, 8), 3)
+    w, m, r = arr((8,), 4), arr((4,), 5), arr((4,), 6)
+    inside = lambda n: FakeArray((n,), ptr=dx.data_ptr() + 64)
+    refuse("dx overlaps weight", ft.layer_norm_backward, dx, d, x, m, r, inside(8))
+    refuse("dx overlaps weight", ft.layer_norm_backward, dx, d, x, inside(4), r, w)
+    refuse("dx overlaps weight", ft.layer_norm_backward, dx, d, x, m, inside(4))
