@@ -50,8 +50,8 @@ extern "C" int gpb_cast(int32_t device, void* stream, int32_t out_dtype, int32_t
   const int os = dtype_bytes(out_dtype), xs = dtype_bytes(x_dtype);
   GPB_REQUIRE(elem_aligned(out_dev, os) && elem_aligned(x_dev, xs), GPB_ERR_INVALID,
               "pointer is not aligned to its element type");
-  GPB_REQUIRE(!overlaps(out_dev, span_bytes(rows, cols, out_ld, os), x_dev,
-                        span_bytes(rows, cols, x_ld, xs)),
+  GPB_REQUIRE(!overlaps(block_extent(out_dev, rows, cols, out_ld, os),
+                        block_extent(x_dev, rows, cols, x_ld, xs)),
               GPB_ERR_INVALID, "out overlaps x");
   GPB_DEVICE_SCOPE(device);
   cudaStream_t st = (cudaStream_t)stream;

@@ -156,12 +156,12 @@ extern "C" int gpb_dropout(int32_t device, void* stream, int32_t dtype, int64_t 
               GPB_ERR_INVALID, "leading dimension below the %lld columns", (long long)cols);
   GPB_REQUIRE(elem_aligned(out_dev, es) && elem_aligned(x_dev, es) && elem_aligned(residual_dev, es),
               GPB_ERR_INVALID, "pointer is not aligned to its element type");
-  const int64_t ob = span_bytes(rows, cols, out_ld, es);
+  const Extent out = block_extent(out_dev, rows, cols, out_ld, es);
   GPB_REQUIRE((out_dev == x_dev && out_ld == x_ld) ||
-                  !overlaps(out_dev, ob, x_dev, span_bytes(rows, cols, x_ld, es)),
+                  !overlaps(out, block_extent(x_dev, rows, cols, x_ld, es)),
               GPB_ERR_INVALID, "out overlaps x (in place needs the same pointer and stride)");
   GPB_REQUIRE((out_dev == residual_dev && out_ld == residual_ld) ||
-                  !overlaps(out_dev, ob, residual_dev, span_bytes(rows, cols, residual_ld, es)),
+                  !overlaps(out, block_extent(residual_dev, rows, cols, residual_ld, es)),
               GPB_ERR_INVALID, "out overlaps residual (in place needs the same pointer and stride)");
   GPB_DEVICE_SCOPE(device);
   DropoutArgs A{};

@@ -1057,25 +1057,23 @@ int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activati
                   elem_aligned(w_up_dev, es) && elem_aligned(b_gate_dev, es) &&
                   elem_aligned(b_up_dev, es),
               GPB_ERR_INVALID, "pointer is not aligned to its element type");
-  const int64_t ob = span_bytes(rows, outer, out_ld, es), wb = span_bytes(outer, inner, w_ld, es);
-  GPB_REQUIRE(!overlaps(out_dev, ob, x_dev, span_bytes(rows, inner, x_ld, es)) &&
-                  !overlaps(out_dev, ob, w_gate_dev, wb) && !overlaps(out_dev, ob, w_up_dev, wb) &&
-                  !overlaps(out_dev, ob, b_gate_dev, outer * es) &&
-                  !overlaps(out_dev, ob, b_up_dev, outer * es),
-              GPB_ERR_INVALID, "out overlaps an input");
+  const Extent out = block_extent(out_dev, rows, outer, out_ld, es);
+  const Extent in[] = {block_extent(x_dev, rows, inner, x_ld, es),
+                       block_extent(w_gate_dev, outer, inner, w_ld, es),
+                       block_extent(w_up_dev, outer, inner, w_ld, es), flat_extent(b_gate_dev, outer * es),
+                       flat_extent(b_up_dev, outer * es)};
+  for (const Extent& i : in)
+    GPB_REQUIRE(!overlaps(out, i), GPB_ERR_INVALID, "out overlaps an input");
   const GatedPlan P = gated_plan(rows, inner, outer, dtype, false);
   const int64_t need = workspace_need(P);
   GPB_REQUIRE(need == 0 || (workspace_dev && workspace_bytes >= need), GPB_ERR_INVALID,
               "gated unit needs a workspace of %lld bytes, got %lld", (long long)need,
               (long long)(workspace_dev ? workspace_bytes : 0));
   GPB_REQUIRE(aligned16(workspace_dev), GPB_ERR_INVALID, "workspace is not 16-byte aligned");
-  GPB_REQUIRE(!overlaps(workspace_dev, need, out_dev, ob) &&
-                  !overlaps(workspace_dev, need, x_dev, span_bytes(rows, inner, x_ld, es)) &&
-                  !overlaps(workspace_dev, need, w_gate_dev, wb) &&
-                  !overlaps(workspace_dev, need, w_up_dev, wb) &&
-                  !overlaps(workspace_dev, need, b_gate_dev, outer * es) &&
-                  !overlaps(workspace_dev, need, b_up_dev, outer * es),
-              GPB_ERR_INVALID, "the workspace overlaps an input or out");
+  const Extent ws_extent = flat_extent(workspace_dev, need);
+  bool shared = overlaps(ws_extent, out);
+  for (const Extent& i : in) shared = shared || overlaps(ws_extent, i);
+  GPB_REQUIRE(!shared, GPB_ERR_INVALID, "the workspace overlaps an input or out");
   GPB_DEVICE_SCOPE(device);
   GatedArgs A{};
   A.x = x_dev;
@@ -1147,20 +1145,22 @@ int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t
   GPB_REQUIRE(aligned16(workspace_dev), GPB_ERR_INVALID, "workspace is not 16-byte aligned");
   {
     // Outputs and the workspace are written while inputs are still read: none may share memory.
-    const int64_t wb = span_bytes(outer, inner, w_ld, es), bb = outer * es;
-    const struct { const void* p; int64_t n; } in[] = {
-        {dout_dev, span_bytes(rows, outer, dout_ld, es)}, {x_dev, span_bytes(rows, inner, x_ld, es)},
-        {w_gate_dev, wb}, {w_up_dev, wb}, {b_gate_dev, bb}, {b_up_dev, bb}};
-    const int64_t dwb = span_bytes(outer, inner, dw_ld, es);
-    const struct { const void* p; int64_t n; } out[] = {
-        {dx_dev, span_bytes(rows, inner, dx_ld, es)}, {dw_gate_dev, dwb}, {dw_up_dev, dwb},
-        {db_gate_dev, bb}, {db_up_dev, bb}, {workspace_dev, need}};
+    const int64_t bb = outer * es;
+    const Extent in[] = {block_extent(dout_dev, rows, outer, dout_ld, es),
+                         block_extent(x_dev, rows, inner, x_ld, es),
+                         block_extent(w_gate_dev, outer, inner, w_ld, es),
+                         block_extent(w_up_dev, outer, inner, w_ld, es), flat_extent(b_gate_dev, bb),
+                         flat_extent(b_up_dev, bb)};
+    const Extent out[] = {block_extent(dx_dev, rows, inner, dx_ld, es),
+                          block_extent(dw_gate_dev, outer, inner, dw_ld, es),
+                          block_extent(dw_up_dev, outer, inner, dw_ld, es), flat_extent(db_gate_dev, bb),
+                          flat_extent(db_up_dev, bb), flat_extent(workspace_dev, need)};
     for (int o = 0; o < 6; ++o) {
-      for (const auto& i : in)
-        GPB_REQUIRE(!overlaps(out[o].p, out[o].n, i.p, i.n), GPB_ERR_INVALID,
+      for (const Extent& i : in)
+        GPB_REQUIRE(!overlaps(out[o], i), GPB_ERR_INVALID,
                     "an output or the workspace overlaps an input");
       for (int q = 0; q < o; ++q)
-        GPB_REQUIRE(!overlaps(out[o].p, out[o].n, out[q].p, out[q].n), GPB_ERR_INVALID,
+        GPB_REQUIRE(!overlaps(out[o], out[q]), GPB_ERR_INVALID,
                     "two outputs (or an output and the workspace) overlap");
     }
   }

@@ -922,22 +922,21 @@ int gpb_layer_norm(int32_t device, void* stream, int32_t dtype, int32_t param_dt
                   elem_aligned(mean_dev, 4) && elem_aligned(rstd_dev, 4),
               GPB_ERR_INVALID, "pointer is not aligned to its element type");
   GPB_REQUIRE((out_dev == x_dev && out_ld == x_ld) ||
-                  !overlaps(out_dev, span_bytes(rows, cols, out_ld, es), x_dev,
-                            span_bytes(rows, cols, x_ld, es)),
+                  !overlaps(block_extent(out_dev, rows, cols, out_ld, es),
+                            block_extent(x_dev, rows, cols, x_ld, es)),
               GPB_ERR_INVALID, "out overlaps x (in place needs the same pointer and stride)");
   {
     // The statistics are written while rows, weight and bias are still read.
-    const struct { const void* p; int64_t n; } used[] = {
-        {out_dev, span_bytes(rows, cols, out_ld, es)}, {x_dev, span_bytes(rows, cols, x_ld, es)},
-        {weight_dev, cols * ps}, {bias_dev, cols * ps}};
-    for (const auto& u : used)
-      GPB_REQUIRE(!overlaps(mean_dev, rows * 4, u.p, u.n) && !overlaps(rstd_dev, rows * 4, u.p, u.n),
-                  GPB_ERR_INVALID, "mean or rstd overlaps another argument");
-    GPB_REQUIRE(!overlaps(mean_dev, rows * 4, rstd_dev, rows * 4), GPB_ERR_INVALID,
-                "mean and rstd overlap");
+    const Extent used[] = {block_extent(out_dev, rows, cols, out_ld, es),
+                           block_extent(x_dev, rows, cols, x_ld, es), flat_extent(weight_dev, cols * ps),
+                           flat_extent(bias_dev, cols * ps)};
+    const Extent mean = flat_extent(mean_dev, rows * 4), rstd = flat_extent(rstd_dev, rows * 4);
+    for (const Extent& u : used)
+      GPB_REQUIRE(!overlaps(mean, u) && !overlaps(rstd, u), GPB_ERR_INVALID,
+                  "mean or rstd overlaps another argument");
+    GPB_REQUIRE(!overlaps(mean, rstd), GPB_ERR_INVALID, "mean and rstd overlap");
     for (int i = 2; i < 4; ++i)
-      GPB_REQUIRE(!overlaps(out_dev, used[0].n, used[i].p, used[i].n), GPB_ERR_INVALID,
-                  "out overlaps weight or bias");
+      GPB_REQUIRE(!overlaps(used[0], used[i]), GPB_ERR_INVALID, "out overlaps weight or bias");
   }
   GPB_DEVICE_SCOPE(device);
   NormArgs A{};
@@ -999,34 +998,31 @@ int gpb_layer_norm_backward(int32_t device, void* stream, int32_t dtype, int32_t
                   elem_aligned(weight_dev, ps) && elem_aligned(mean_dev, 4) &&
                   elem_aligned(rstd_dev, 4),
               GPB_ERR_INVALID, "pointer is not aligned to its element type");
-  const int64_t dxb = dx_dev ? span_bytes(rows, cols, dx_ld, es) : 0;
-  GPB_REQUIRE((dx_dev == dout_dev && dx_ld == dout_ld) ||
-                  !overlaps(dx_dev, dxb, dout_dev, span_bytes(rows, cols, dout_ld, es)),
+  const Extent dx = block_extent(dx_dev, rows, cols, dx_ld, es),
+               dout = block_extent(dout_dev, rows, cols, dout_ld, es),
+               x = block_extent(x_dev, rows, cols, x_ld, es), weight = flat_extent(weight_dev, cols * ps),
+               mean = flat_extent(mean_dev, rows * 4), rstd = flat_extent(rstd_dev, rows * 4);
+  GPB_REQUIRE((dx_dev == dout_dev && dx_ld == dout_ld) || !overlaps(dx, dout),
               GPB_ERR_INVALID, "dx overlaps dout (in place needs the same pointer and stride)");
-  GPB_REQUIRE((dx_dev == x_dev && dx_ld == x_ld) ||
-                  !overlaps(dx_dev, dxb, x_dev, span_bytes(rows, cols, x_ld, es)),
+  GPB_REQUIRE((dx_dev == x_dev && dx_ld == x_ld) || !overlaps(dx, x),
               GPB_ERR_INVALID, "dx overlaps x (in place needs the same pointer and stride)");
-  GPB_REQUIRE(!overlaps(dx_dev, dxb, weight_dev, cols * ps) && !overlaps(dx_dev, dxb, mean_dev, rows * 4) &&
-                  !overlaps(dx_dev, dxb, rstd_dev, rows * 4),
-              GPB_ERR_INVALID, "dx overlaps weight, mean or rstd");
+  GPB_REQUIRE(!overlaps(dx, weight) && !overlaps(dx, mean) && !overlaps(dx, rstd), GPB_ERR_INVALID,
+              "dx overlaps weight, mean or rstd");
   if (params) {
     const int64_t need = (int64_t)norm_blocks(rows, cols) * 2 * cols * (int64_t)sizeof(float);
     GPB_REQUIRE(workspace_dev && workspace_bytes >= need, GPB_ERR_INVALID,
                 "the weight gradients need a workspace of %lld bytes, got %lld", (long long)need,
                 (long long)(workspace_dev ? workspace_bytes : 0));
     GPB_REQUIRE(aligned16(workspace_dev), GPB_ERR_INVALID, "workspace is not 16-byte aligned");
-    const int64_t pb = cols * ps;
-    const struct { const void* p; int64_t n; } in[] = {
-        {dout_dev, span_bytes(rows, cols, dout_ld, es)}, {x_dev, span_bytes(rows, cols, x_ld, es)},
-        {weight_dev, pb}, {mean_dev, rows * 4}, {rstd_dev, rows * 4}};
-    const struct { const void* p; int64_t n; } out[] = {
-        {dx_dev, dxb}, {dweight_dev, pb}, {dbias_dev, pb}, {workspace_dev, need}};
+    const Extent in[] = {dout, x, weight, mean, rstd};
+    const Extent out[] = {dx, flat_extent(dweight_dev, cols * ps), flat_extent(dbias_dev, cols * ps),
+                          flat_extent(workspace_dev, need)};
     for (int o = 1; o < 4; ++o) {
-      for (const auto& i : in)
-        GPB_REQUIRE(!overlaps(out[o].p, out[o].n, i.p, i.n), GPB_ERR_INVALID,
+      for (const Extent& i : in)
+        GPB_REQUIRE(!overlaps(out[o], i), GPB_ERR_INVALID,
                     "dweight, dbias or the workspace overlaps an input");
       for (int q = 0; q < o; ++q)
-        GPB_REQUIRE(!overlaps(out[o].p, out[o].n, out[q].p, out[q].n), GPB_ERR_INVALID,
+        GPB_REQUIRE(!overlaps(out[o], out[q]), GPB_ERR_INVALID,
                     "two outputs (or an output and the workspace) overlap");
     }
   }

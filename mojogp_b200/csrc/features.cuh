@@ -46,14 +46,33 @@ inline int dtype_bytes(int32_t dt) { return dt == GPB_DTYPE_F32 ? 4 : 2; }
 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-// Bytes from the first to one past the last element of a [rows][cols] block of leading dimension ld.
-inline int64_t span_bytes(int64_t rows, int64_t cols, int64_t ld, int esize) {
-  return rows > 0 && cols > 0 ? ((rows - 1) * ld + cols) * esize : 0;
-}
 inline bool overlaps(const void* a, int64_t abytes, const void* b, int64_t bbytes) {
   if (!a || !b || abytes <= 0 || bbytes <= 0) return false;
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
   return x < y + (uintptr_t)bbytes && y < x + (uintptr_t)abytes;
+}
+
+// Memory of a [rows][cols] block of leading dimension ld, or of a vector, in bytes.
+struct Extent {
+  const void* p;
+  int64_t rows, width, stride;
+};
+inline Extent block_extent(const void* p, int64_t rows, int64_t cols, int64_t ld, int esize) {
+  return {p, rows, cols * esize, ld * esize};
+}
+inline Extent flat_extent(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+// Two blocks with one row stride may lie side by side (column ranges of one matrix): then no row of one
+// reaches the columns of the other.
+inline bool overlaps(const Extent& a, const Extent& b) {
+  auto span = [](const Extent& e) {
+    return e.rows > 0 && e.width > 0 ? (e.rows - 1) * e.stride + e.width : 0;
+  };
+  if (!overlaps(a.p, span(a), b.p, span(b))) return false;
+  const int64_t stride = a.rows > 1 ? a.stride : b.stride;
+  if (b.rows > 1 && b.stride != stride) return true;
+  int64_t right = (int64_t)((uintptr_t)b.p - (uintptr_t)a.p) % stride;  // of b's rows from a's
+  if (right < 0) right += stride;
+  return right < a.width || right + b.width > stride;
 }
 // Natural alignment of the element type (a view of a byte buffer may miss it).
 inline bool elem_aligned(const void* p, int esize) { return ((uintptr_t)p % (uintptr_t)esize) == 0; }

@@ -59,3 +59,38 @@ def test_layer_norm_backward_keeps_dx_off_its_other_inputs(ft):
     refuse("dx overlaps weight", ft.layer_norm_backward, dx, d, x, m, r, inside(8))
     refuse("dx overlaps weight", ft.layer_norm_backward, dx, d, x, inside(4), r, w)
     refuse("dx overlaps weight", ft.layer_norm_backward, dx, d, x, m, inside(4))
+
+
+def columns(ptr, first, count, rows=4, ld=24, **kw):
+    """Columns [first, first + count) of a float32 matrix with `ld` columns."""
+    return FakeArray((rows, count), ptr=ptr + 4 * first, strides=(ld, 1), device=64, **kw)
+
+
+def test_column_ranges_of_one_matrix_do_not_overlap(ft):
+    big, other, n = 64 * MB, 128 * MB, dict(device=64)
+    m, r, v = (FakeArray((k,), ptr=i * 64 * MB, **n) for k, i in ((4, 3), (4, 4), (8, 5)))
+    ws = FakeArray((1 << 20,), dtype="uint8", ptr=512 * MB, **n)
+    a, b, c = (columns(big, f, 8) for f in (0, 8, 16))
+    for x, y in ((a, b), (b, a), (a, c), (c, b)):
+        no_device(ft.layer_norm, y, x)
+        no_device(ft.dropout, y, x, 0.5, 1)
+        no_device(ft.dropout, y, x, 0.5, 1, residual=y)
+        no_device(ft.cast, y, x)
+        no_device(ft.layer_norm_backward, y, x, columns(other, 0, 8), m, r, dweight=v, workspace=ws)
+    w, u = (FakeArray((8, 8), ptr=i * 64 * MB, **n) for i in (6, 7))
+    no_device(ft.gated_unit, b, a, w, u)
+    no_device(ft.gated_unit_backward, b, a, w, u, dx=c, workspace=ws)
+    no_device(ft.gated_unit_backward, b, a, w, u, dw_gate=columns(other, 0, 8, 8),
+              dw_up=columns(other, 8, 8, 8), workspace=ws)
+    # One column shared, from either side; rows that wrap around; other strides.
+    for first in (1, 7, 23):
+        y = columns(big, 16 + first, 8) if first == 1 else columns(big, first, 8)
+        refuse("overlap", ft.layer_norm, y, columns(big, 0, 8) if first != 1 else c)
+        refuse("overlap", ft.gated_unit, y, columns(big, 0, 8) if first != 1 else c, w, u)
+    refuse("overlap", ft.layer_norm, columns(big, 8, 8, ld=32), a)
+    refuse("overlap", ft.dropout, b, columns(other, 0, 8), 0.5, 1, residual=columns(big, 9, 8))
+    refuse("two outputs", ft.gated_unit_backward, b, a, w, u, dw_gate=columns(other, 0, 8, 8),
+           dw_up=columns(other, 4, 8, 8), workspace=ws)
+    # A single row between two others' columns.
+    no_device(ft.layer_norm, columns(big, 24 + 8, 8, rows=1), columns(big, 24 + 16, 8, rows=1))
+    refuse("overlap", ft.layer_norm, columns(big, 24 + 8, 8, rows=1), columns(big, 24 + 12, 8, rows=1))
