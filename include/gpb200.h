@@ -485,9 +485,10 @@ int gpb_layer_norm_backward(int32_t device, void* stream, int32_t dtype, int32_t
  * [outer][inner] with one leading dimension, biases [outer] or NULL, out
  * [rows][outer], all of one type; `activation` is GPB_ACT_*. out must not
  * overlap an input. float32 products are formed from three bfloat16 parts per
- * value (float32 accuracy): with more than 4 rows, an input beyond 3.3895e38
- * or not finite makes the outputs that depend on it NaN. (Up to 8 rows may be
- * computed without the tensor cores, depending on the sizes.) */
+ * value (float32 accuracy; values below 2^-100 lose digits): with more than 4
+ * rows, an input beyond 3.3895e38 or not finite makes the outputs that depend
+ * on it NaN. (Up to 8 rows may be computed without the tensor cores, depending
+ * on the sizes.) */
 int gpb_gated_unit_workspace(int32_t dtype, int64_t rows, int64_t inner, int64_t outer,
                              int32_t backward, int64_t* bytes_out);
 int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activation, int64_t rows,
@@ -501,7 +502,9 @@ int gpb_gated_unit(int32_t device, void* stream, int32_t dtype, int32_t activati
  * [outer], each optional (NULL). Outputs overlap neither inputs nor one
  * another. rows = 0 writes zero weight and bias gradients. Where the factors
  * of the gradients (dout up act', dout act) are not finite in float32, the
- * gradients that depend on them are infinite or NaN. In float16 the factors are
+ * gradients that depend on them are infinite or NaN. With 16-bit types the
+ * factors are rounded to two parts of the type (16 bits and more) where
+ * rows * inner * outer is at most 2^31, and to one above. In float16 they are
  * kept as float16 parts times a power of two of the call: they may pass
  * float16's range, and one below 2^-21 of the call's largest counts as 0. */
 int gpb_gated_unit_backward(int32_t device, void* stream, int32_t dtype, int32_t activation,
