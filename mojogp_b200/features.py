@@ -250,7 +250,10 @@ def gated_unit_backward(dout, x, w_gate, w_up, b_gate=None, b_up=None, *, dx=Non
                         workspace=None, stream=None) -> None:
     """Gradients of gated_unit from dout [rows, outer] and the forward inputs
     (the projections are recomputed): dx, dw_gate, dw_up, db_gate and db_up are
-    written where given, in x's element type."""
+    written where given, in x's element type. With 16-bit types the gradients'
+    factors dout up act' and dout act are rounded to two parts of the type where
+    rows * inner * outer is at most 2^31, to one above; in float16 times a power
+    of two of the call, so that they may pass its range."""
     act = _activation(activation)
     (xp, rows, inner, x_ld, code, dev), g, u, bg, bu = _gated_inputs(x, w_gate, w_up, b_gate, b_up)
     outer = g[1]
