@@ -13,6 +13,13 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def give_memory_back():
+    yield
+    if torch.cuda.memory_reserved() > 8 << 30:
+        torch.cuda.empty_cache()
+
+
 def philox_words(first_block, blocks, seed, offset):
     """Philox4x32-10 in NumPy uint64, from any block."""
     lo, s32 = np.uint64(0xFFFFFFFF), np.uint64(32)

@@ -12,6 +12,13 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def give_memory_back():
+    yield
+    if torch.cuda.memory_reserved() > 8 << 30:
+        torch.cuda.empty_cache()
+
+
 @pytest.fixture(scope="module")
 def ft(gpb_lib):
     from mojogp_b200 import features
